@@ -1,0 +1,222 @@
+// Writing and reading the 8-bit key/value cache, for sm_100a. No counterpart in the reference, whose caches are fp16
+// (src/model.rs:440-446). The cache holds, per sequence and head, `cap` rows of 64 one-byte codes and one fp32 scale
+// for every `block` of them: value = code * scale.
+//
+// kv8_write, tokens x at positions pos .. pos + n: for each block touched
+//     a = max |x| over the block's new tokens,  s = a / Q  (Q = 127 for int8, 448 for e4m3)
+//     s = max(s, the block's earlier scale)  where the block has tokens before pos
+//     code = round_to_even(x * r),  r = 1 / s  (0 where s is 0: an all-zero block)
+// and, where s grew, the earlier tokens' codes become round_to_even(code * (s_old * r)): a scale only grows while its
+// block fills, so a code is rounded again at most as often as the block's maximum grows. All of it in fp32: quotients
+// and products each rounded once.
+//
+// Bound by memory: 2 bytes read and 1 written per value. A warp takes 32 tokens of one block (8 lanes to a token, 16
+// bytes each), so that its 8 loads are all in flight before the maximum is known and the values are read once; blocks
+// of 64 and 128 tokens are shared by 2 and 4 warps of the CTA, which exchange their maxima in shared memory.
+#include "fp8_cache.cuh"
+#include "launch.h"
+
+namespace mmz {
+namespace kv8 {
+constexpr int NT = 128;
+
+// where a cache's codes (bytes) and scales (floats) of sequence b and head h start
+struct Cache {
+    uint8_t *k, *v;
+    float *ks, *vs;
+    long c_seq, c_head, s_seq, s_head;
+};
+
+__device__ __forceinline__ float finite(float x) {  // fp16 infinities count as the largest finite number
+    return fabsf(x) > 65504.f ? copysignf(65504.f, x) : x;
+}
+}  // namespace kv8
+using namespace kv8;
+
+// grid: items / (4 / W) CTAs, an item = one (sequence, head, k or v, block); W warps to an item
+template <int KIND>
+__global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* __restrict__ k, const h16* __restrict__ v, long x_seq,
+                                                       long x_tok, long x_head, Cache c, const int* __restrict__ pos,
+                                                       int heads, int n, int cap, int block, int nblk, long items) {
+    __shared__ float wmax[4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int W = block <= 32 ? 1 : block / 32, tw = block < 32 ? block : 32;  // warps to an item, tokens to a warp
+    const long item = (long)blockIdx.x * (4 / W) + warp / W;
+    griddep_wait();
+    const bool live = item < items;
+    const int ib = (int)(live ? item % nblk : 0);
+    const long rest = live ? item / nblk : 0;
+    const int isv = (int)(rest & 1), hd = (int)((rest >> 1) % heads);
+    const long b = (rest >> 1) / heads;
+    const int p0 = pos ? pos[b] : 0;
+    // the first block with a new token at a position >= 0; blocks past the capacity or the last token have nothing
+    const long first = p0 > 0 ? p0 / block : 0;
+    const long blk = first + ib;
+    const long t0 = blk * block + (warp % W) * tw;  // this warp's first position
+    const long end = min((long)p0 + n, (long)cap);
+    const bool any = live && blk * block < end;
+    const h16* x = (isv ? v : k) + b * x_seq + hd * x_head;
+    uint8_t* codes = (isv ? c.v : c.k) + b * c.c_seq + hd * c.c_head;
+    float* scale = (isv ? c.vs : c.ks) + b * c.s_seq + hd * c.s_head + blk;
+    const int sub = lane >> 3, d0 = (lane & 7) * 8;
+    uint4 val[8];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const long j = t0 + 4 * i + sub;
+        val[i] = make_uint4(0, 0, 0, 0);
+        if (any && 4 * i < tw && j >= p0 && j < end) val[i] = *reinterpret_cast<const uint4*>(x + (j - p0) * x_tok + d0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t w[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float2 p = h2_to_f2(w[q]);
+            amax = fmaxf(amax, fmaxf(fabsf(finite(p.x)), fabsf(finite(p.y))));  // fmaxf drops a NaN
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffff, amax, o));
+    const bool older = any && blk * block < p0;
+    const float s_old = older ? *scale : 0.f;
+    if (W > 1) {
+        if (lane == 0) wmax[warp] = amax;
+        __syncthreads();  // every warp of the CTA comes here; the earlier scale is read before it and written after it
+        const int w0 = warp / W * W;
+        for (int i = 0; i < W; i++) amax = fmaxf(amax, wmax[w0 + i]);
+    } else {
+        __syncwarp();
+    }
+    if (!any) return;
+    const float s = fmaxf(__fdiv_rn(amax, kv8_top<KIND>()), s_old);
+    const float r = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    if (lane == 0 && warp % W == 0) *scale = s;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const long j = t0 + 4 * i + sub;
+        if (4 * i >= tw || j < p0 || j >= end) continue;
+        const uint32_t w[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
+        uint2 o;
+        uint32_t* op = &o.x;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const float2 a = h2_to_f2(w[2 * q]), e = h2_to_f2(w[2 * q + 1]);
+            const float y[4] = {__fmul_rn(finite(a.x), r), __fmul_rn(finite(a.y), r), __fmul_rn(finite(e.x), r),
+                                __fmul_rn(finite(e.y), r)};
+            op[q] = kv8_store4<KIND>(y);
+        }
+        *reinterpret_cast<uint2*>(codes + j * HD + d0) = o;
+    }
+    if (older && s != s_old) {  // the scale grew: the block's earlier codes on the new one
+        const float f = __fmul_rn(s_old, r);
+        for (long j = t0 + sub; j < min(t0 + tw, (long)p0); j += 4) {
+            uint2* at = reinterpret_cast<uint2*>(codes + j * HD + d0);
+            uint2 o = *at;
+            uint32_t* op = &o.x;
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                float y[4];
+                kv8_load4<KIND>(op[q], y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = __fmul_rn(y[e], f);
+                op[q] = kv8_store4<KIND>(y);
+            }
+            *at = o;
+        }
+    }
+}
+
+// thread = 8 values of one token and head, of k and then of v
+template <int KIND>
+__global__ void __launch_bounds__(256) kv8_read_kernel(Cache c, h16* __restrict__ k, h16* __restrict__ v, long y_seq,
+                                                       long y_tok, long y_head, const int* __restrict__ pos,
+                                                       const int* __restrict__ lens, int heads, int n, int cap,
+                                                       int block, long items) {
+    const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
+    griddep_wait();
+    if (i >= items) return;
+    const int d0 = (int)(i & 7) * 8;
+    long rest = i >> 3;
+    const int t = (int)(rest % n);
+    rest /= n;
+    const int isv = (int)(rest & 1), hd = (int)((rest >> 1) % heads);
+    const long b = (rest >> 1) / heads;
+    const long j = (long)(pos ? pos[b] : 0) + t, end = lens ? min(lens[b], cap) : cap;
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (j >= 0 && j < end) {
+        const uint2 w = *reinterpret_cast<const uint2*>((isv ? c.v : c.k) + b * c.c_seq + hd * c.c_head + j * HD + d0);
+        const float s = ((isv ? c.vs : c.ks) + b * c.s_seq + hd * c.s_head)[j / block];
+        float y[4];
+        __half2* op = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            kv8_load4<KIND>(q ? w.y : w.x, y);
+            op[2 * q] = __floats2half2_rn(__fmul_rn(y[0], s), __fmul_rn(y[1], s));
+            op[2 * q + 1] = __floats2half2_rn(__fmul_rn(y[2], s), __fmul_rn(y[3], s));
+        }
+    }
+    *reinterpret_cast<uint4*>((isv ? v : k) + b * y_seq + t * y_tok + hd * y_head + d0) = o;
+}
+
+// what both calls ask of their arguments; 0 or the last error set
+static int kv8_check(const char* what, const void* k, const void* v, const void* k8, const void* v8, const void* ks,
+                     const void* vs, long long x_seq, long long x_tok, long long x_head, long long c_seq,
+                     long long c_head, int batch, int heads, int n, int cap, int block, int kind) {
+    if (batch < 0 || heads < 1 || n < 0 || cap < 1) return failf("%s: batch >= 0, heads >= 1, n >= 0, cap >= 1", what);
+    if (!kv8_block_ok(block)) return failf("%s: block is 16, 32, 64 or 128", what);
+    if (kind != KV8_INT8 && kind != KV8_E4M3) return failf("%s: kind is 0 (int8) or 1 (e4m3)", what);
+    if (batch == 0 || n == 0) return 0;
+    if (!k || !v || !k8 || !v8 || !ks || !vs) return failf("%s: null pointer", what);
+    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)k8 | (uintptr_t)v8) & 15)
+        return failf("%s: k, v and the cache 16-byte aligned", what);
+    if ((x_seq | x_tok | x_head) & 7) return failf("%s: strides of k and v multiples of 8 values", what);
+    if ((c_seq | c_head) & 15) return failf("%s: strides of the cache multiples of 16 bytes", what);
+    return 0;
+}
+
+int launch_kv8_write(const void* k, const void* v, long long x_seq, long long x_tok, long long x_head, void* k8,
+                     void* v8, float* ks, float* vs, long long c_seq, long long c_head, long long s_seq,
+                     long long s_head, const int* pos, int batch, int heads, int n, int cap, int block, int kind,
+                     cudaStream_t st) {
+    if (kv8_check("kv8_write", k, v, k8, v8, ks, vs, x_seq, x_tok, x_head, c_seq, c_head, batch, heads, n, cap, block,
+                  kind))
+        return -1;
+    if (batch == 0 || n == 0) return 0;
+    // blocks that n tokens can touch, from any position
+    const int most = (cap + block - 1) / block;
+    const long touched = pos ? ((long)n + block - 2) / block + 1 : ((long)n + block - 1) / block;
+    const int nblk = (int)(touched < most ? touched : most);
+    const long items = (long)batch * heads * 2 * nblk;
+    const int per = block <= 32 ? 4 : 128 / block;
+    const long grid = (items + per - 1) / per;
+    if (grid > 0x7fffffffl) return fail("kv8_write: more than 2^31 blocks in one call");
+    DevCtx& dc = dev_ctx();
+    if (!dc.ok) return fail(dc.err);
+    const Cache c{(uint8_t*)k8, (uint8_t*)v8, ks, vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head};
+    auto* fn = kind == KV8_INT8 ? kv8_write_kernel<KV8_INT8> : kv8_write_kernel<KV8_E4M3>;
+    return check_pdl(launch_pdl(fn, dim3((unsigned)grid), dim3(NT), 0, st, (const h16*)k, (const h16*)v, (long)x_seq,
+                                (long)x_tok, (long)x_head, c, pos, heads, n, cap, block, nblk, items),
+                     "kv8_write");
+}
+
+int launch_kv8_read(const void* k8, const void* v8, const float* ks, const float* vs, long long c_seq, long long c_head,
+                    long long s_seq, long long s_head, void* k, void* v, long long y_seq, long long y_tok,
+                    long long y_head, const int* pos, const int* lens, int batch, int heads, int n, int cap, int block,
+                    int kind, cudaStream_t st) {
+    if (kv8_check("kv8_read", k, v, k8, v8, ks, vs, y_seq, y_tok, y_head, c_seq, c_head, batch, heads, n, cap, block,
+                  kind))
+        return -1;
+    if (batch == 0 || n == 0) return 0;
+    const long items = (long)batch * heads * 2 * n * 8, grid = (items + 255) / 256;
+    if (grid > 0x7fffffffl) return fail("kv8_read: more than 2^31 blocks in one call");
+    DevCtx& dc = dev_ctx();
+    if (!dc.ok) return fail(dc.err);
+    const Cache c{(uint8_t*)k8, (uint8_t*)v8, (float*)ks, (float*)vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head};
+    auto* fn = kind == KV8_INT8 ? kv8_read_kernel<KV8_INT8> : kv8_read_kernel<KV8_E4M3>;
+    return check_pdl(launch_pdl(fn, dim3((unsigned)grid), dim3(256), 0, st, c, (h16*)k, (h16*)v, (long)y_seq,
+                                (long)y_tok, (long)y_head, pos, lens, heads, n, cap, block, items),
+                     "kv8_read");
+}
+
+}  // namespace mmz

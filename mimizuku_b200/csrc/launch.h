@@ -5,6 +5,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "attn8.h"
+#include "logprobs.h"
+
 namespace mmz {
 
 struct DevCtx {
@@ -110,6 +113,29 @@ int launch_dtw_times(const void* cost, const int* rows, const int* cols, int n, 
 size_t log_mel_work_bytes(int count);
 int launch_log_mel(const float* audio, const int* lens, int count, int n_mels, float* out, void* work,
                    size_t work_bytes, cudaStream_t st);
+
+// the 8-bit key/value cache (kv8.cu): n tokens of k and v (fp16, strides in values) quantised into the cache at
+// pos[b].. (null: 0), and read back; cache strides in bytes, scale strides in floats; kind 0 int8, 1 e4m3
+int launch_kv8_write(const void* k, const void* v, long long x_seq, long long x_tok, long long x_head, void* k8,
+                     void* v8, float* ks, float* vs, long long c_seq, long long c_head, long long s_seq,
+                     long long s_head, const int* pos, int batch, int heads, int n, int cap, int block, int kind,
+                     cudaStream_t st);
+int launch_kv8_read(const void* k8, const void* v8, const float* ks, const float* vs, long long c_seq, long long c_head,
+                    long long s_seq, long long s_head, void* k, void* v, long long y_seq, long long y_tok,
+                    long long y_head, const int* pos, const int* lens, int batch, int heads, int n, int cap, int block,
+                    int kind, cudaStream_t st);
+// attention over that cache (attn8.cu); scratch of attn8_scratch_bytes, no initial contents required
+size_t attn8_scratch_bytes(int batch, int rows, int q_heads, int kv_heads, int cap, int slots);
+int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, cudaStream_t st);
+// log probabilities of given tokens, entropy and alternatives: of rows of logits (logprobs.cu; type 0 fp16, 1 fp32) and
+// of hidden states against an embedding (linear_logprobs.cu; scratch of linear_logprobs_scratch_bytes)
+int logp_check(const char* what, const LogpOut& o);
+int launch_token_logprobs(const void* x, long long ldx, int type, int rows, int V, const unsigned char* sup,
+                          const LogpOut& o, cudaStream_t st);
+size_t linear_logprobs_scratch_bytes(int rows, int V, int d);
+int launch_linear_logprobs(const void* x, long long ldx, const void* emb, int rows, int V, int d,
+                           const unsigned char* sup, const LogpOut& o, void* scratch, size_t scratch_bytes,
+                           cudaStream_t st);
 
 // engine-side elementwise and token kernels (misc.cu)
 int launch_embed(const int* tok, const int* ctr, const void* emb, const void* pe, void* x, int batch, int maxT, int d,

@@ -1,0 +1,74 @@
+// What the two log-probability operators (logprobs.cu, linear_logprobs.cu) share: their outputs, the running softmax
+// statistics of a row and how two parts of a row join.
+#pragma once
+#include "common.cuh"
+#include "logprobs.h"
+
+namespace mmz {
+
+// Over a set of logits x: m the largest, s = sum e^(x - m), u = sum e^(x - m) (x - m). Then
+//   lse = m + log s,   entropy = log s - u / s,   log p(t) = x_t - lse.
+// The empty set, and one of -infinities only, has m = -inf and s = u = 0; a NaN makes s NaN.
+struct RowStat {
+    float m, s, u;
+};
+
+__device__ __forceinline__ RowStat stat_none() { return {-INFINITY, 0.f, 0.f}; }
+
+__device__ __forceinline__ RowStat stat_join(const RowStat& a, const RowStat& b) {
+    if (b.m == -INFINITY && b.s == 0.f) return a;
+    if (a.m == -INFINITY && a.s == 0.f) return b;
+    const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m, ea = __expf(da), eb = __expf(db);
+    // e^(x - m) (x - m) = e^(x - a) e^(a - m) ((x - a) + (a - m)); nothing where e is 0 (a NaN stays in s)
+    const float ua = ea > 0.f ? ea * (a.u + da * a.s) : 0.f, ub = eb > 0.f ? eb * (b.u + db * b.s) : 0.f;
+    return {m, ea * a.s + eb * b.s, ua + ub};
+}
+__device__ __forceinline__ void stat_add(RowStat& a, float x) {
+    if (x == -INFINITY) return;
+    if (x > a.m) {
+        const float d = a.m - x, e = __expf(d);  // a.m = -inf: e = 0
+        a.u = e > 0.f ? e * (a.u + d * a.s) : 0.f;  // d * s may overflow where e = 0
+        a.s = a.s * e + 1.f;
+        a.m = x;
+    } else {
+        const float d = x - a.m, e = __expf(d);
+        a.s += e;
+        a.u += e > 0.f ? e * d : 0.f;
+    }
+}
+
+// (value, lower id first) as one unsigned comparison; 0 stands for no candidate. -0 counts as +0. A NaN and -inf are no
+// candidates.
+__device__ __forceinline__ unsigned long long top_key(float v, int id) {
+    if (!(v > -INFINITY)) return 0ull;
+    uint32_t u = __float_as_uint(v + 0.f);
+    u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return ((unsigned long long)u << 32) | (0xffffffffu - (uint32_t)id);
+}
+__device__ __forceinline__ int key_id(unsigned long long k) { return (int)(0xffffffffu - (uint32_t)k); }
+__device__ __forceinline__ float key_value(unsigned long long k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+
+// the row's outputs except its alternatives; tgt: the target's logit (read only where the target is in [0, V))
+__device__ __forceinline__ float store_row(const LogpOut& o, long at, const RowStat& a, bool has_target, float tgt) {
+    const bool none = a.m == -INFINITY && a.s == 0.f;
+    const float ls = logf(a.m == INFINITY ? NAN : a.s), lse = none ? -INFINITY : a.m + ls;
+    if (o.logp) o.logp[at] = !has_target ? 0.f : (tgt == -INFINITY && lse == lse) ? -INFINITY : tgt - lse;
+    if (o.entropy) o.entropy[at] = none ? 0.f : ls - a.u / a.s;
+    if (o.lse) o.lse[at] = lse;
+    return lse;
+}
+// the index of row r's outputs; -1 where the column counter points outside them
+__device__ __forceinline__ long row_at(const LogpOut& o, long r) {
+    const int c = o.col ? *o.col : 0;
+    return c >= 0 && c < o.ld ? r * o.ld + c : -1;
+}
+// one alternative of the row at `at`; key 0: none
+__device__ __forceinline__ void store_top(const LogpOut& o, long at, int i, unsigned long long key, float lse) {
+    if (o.top_id) o.top_id[at * o.top + i] = key ? key_id(key) : -1;
+    if (o.top_logp) o.top_logp[at * o.top + i] = key ? key_value(key) - lse : -INFINITY;
+}
+
+}  // namespace mmz

@@ -1,0 +1,180 @@
+"""The 8-bit key/value cache (write, read back, attention) and the token log probabilities, over torch CUDA tensors.
+
+Every call works on the current device and stream (or `stream`), checks its tensors on the host (MmzError) and returns
+without waiting; outputs are tensors that the caller gives."""
+import torch
+
+from . import MmzError, _check, _stream, lib
+
+_KIND = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_I32, _F16, _F32 = torch.int32, torch.float16, torch.float32
+
+
+def _tensor(what, name, t, dtype, shape=None, last=True):
+    """A CUDA tensor of the current device with that dtype and shape (None: any length), its last dimension dense."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise MmzError(f"{what}: {name} is not a CUDA tensor")
+    if t.dtype is not dtype:
+        raise MmzError(f"{what}: {name} is {t.dtype}, not {dtype}")
+    if t.get_device() != torch.cuda.current_device():
+        raise MmzError(f"{what}: {name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if shape is not None:
+        got = t.shape
+        if len(got) != len(shape) or any(n is not None and n != g for n, g in zip(shape, got)):
+            raise MmzError(f"{what}: {name} is {tuple(got)}, not {tuple(shape)}")
+        if last and got and got[-1] > 1 and t.stride(-1) != 1:
+            raise MmzError(f"{what}: the last dimension of {name} is not dense")
+    return t.data_ptr()
+
+
+def _dense(what, name, t, dtype, shape):
+    p = _tensor(what, name, t, dtype, shape)
+    if not t.is_contiguous():
+        raise MmzError(f"{what}: {name} is not contiguous")
+    return p
+
+
+def _cache(what, k8, v8, ks, vs, block):
+    """(batch, heads, cap, kind, pointers, strides) of a cache."""
+    if not isinstance(k8, torch.Tensor) or k8.dtype not in _KIND or k8.dim() != 4 or k8.shape[3] != 64:
+        raise MmzError(f"{what}: k8 is an int8 or float8_e4m3fn tensor [batch][heads][cap][64]")
+    b, h, cap, _ = k8.shape
+    if block not in (16, 32, 64, 128):
+        raise MmzError(f"{what}: block is 16, 32, 64 or 128")
+    nb = (cap + block - 1) // block
+    ptrs = (_tensor(what, "k8", k8, k8.dtype, (b, h, cap, 64)), _tensor(what, "v8", v8, k8.dtype, (b, h, cap, 64)),
+            _tensor(what, "ks", ks, _F32, (b, h, nb)), _tensor(what, "vs", vs, _F32, (b, h, nb)))
+    cs, ss = k8.stride(), ks.stride()
+    if cap > 1 and cs[2] != 64:
+        raise MmzError(f"{what}: a head's rows of the cache lie one after another")
+    if v8.stride() != cs or vs.stride() != ss:
+        raise MmzError(f"{what}: keys and values of the cache have the same strides")
+    return b, h, cap, _KIND[k8.dtype], ptrs, (cs[0], cs[1], ss[0], ss[1])
+
+
+def _pair(what, k, v, b, h):
+    """Pointers, token count and shared strides of k and v [batch][n][heads][64] fp16."""
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise MmzError(f"{what}: k is a tensor [batch][n][heads][64]")
+    n = k.shape[1]
+    pk, pv = _tensor(what, "k", k, _F16, (b, n, h, 64)), _tensor(what, "v", v, _F16, (b, n, h, 64))
+    s = k.stride()
+    if v.stride() != s:
+        raise MmzError(f"{what}: k and v have the same strides")
+    return pk, pv, n, s
+
+
+def kv8_write(k, v, k8, v8, ks, vs, block=64, pos=None, stream=None):
+    """Quantises the tokens k, v [b][n][heads][64] fp16 into the cache k8, v8 [b][heads][cap][64] (int8 or
+    float8_e4m3fn) with the scales ks, vs [b][heads][ceil(cap / block)] float32, at positions pos[b].. (int32 [b]; None:
+    from 0). A block that already has tokens keeps at least its scale; its codes are rounded again when it grows."""
+    b, h, cap, kind, c, cs = _cache("kv8_write", k8, v8, ks, vs, block)
+    pk, pv, n, s = _pair("kv8_write", k, v, b, h)
+    at = _dense("kv8_write", "pos", pos, _I32, (b,)) if pos is not None else None
+    _check(lib.mmz_kv8_write(pk, pv, s[0], s[1], s[2], *c, *cs, at, b, h, n, cap, block, kind, _stream(stream)),
+           "kv8_write")
+
+
+def kv8_read(k8, v8, ks, vs, k, v, block=64, pos=None, lens=None, stream=None):
+    """The cache's values at positions pos[b].. (None: from 0) into k, v [b][n][heads][64] fp16, zeros from position
+    min(lens[b], cap) on (lens None: cap)."""
+    b, h, cap, kind, c, cs = _cache("kv8_read", k8, v8, ks, vs, block)
+    pk, pv, n, s = _pair("kv8_read", k, v, b, h)
+    at = _dense("kv8_read", "pos", pos, _I32, (b,)) if pos is not None else None
+    ln = _dense("kv8_read", "lens", lens, _I32, (b,)) if lens is not None else None
+    _check(lib.mmz_kv8_read(*c, *cs, pk, pv, s[0], s[1], s[2], at, ln, b, h, n, cap, block, kind, _stream(stream)),
+           "kv8_read")
+
+
+def attn8_scratch_bytes(batch, rows, q_heads, kv_heads, cap, slots=0):
+    """Bytes of device scratch attn8 needs for such a call (0: none)."""
+    return lib.mmz_attn8_scratch_bytes(batch, rows, q_heads, kv_heads, cap, slots)
+
+
+def attn8(q, k8, v8, ks, vs, out, block=64, lens=None, causal=False, scale=0.125, probs=None, pslot=None, scratch=None,
+          stream=None):
+    """Attention of q [b][rows][q_heads][64] fp16 over the cache's first lens[b] positions (int32 [b]; None: all of
+    them), into out of the same shape; causal: the rows are the sequence's last ones, row i sees lens - rows + i + 1
+    positions. A row that sees nothing gives zeros. probs [b][slots][rows][cap] fp16 receives the probabilities of the
+    heads with pslot[head] >= 0 (int32 [q_heads]). scratch: a uint8 tensor of attn8_scratch_bytes(...) (allocated here
+    when None and needed)."""
+    b, h, cap, kind, c, cs = _cache("attn8", k8, v8, ks, vs, block)
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise MmzError("attn8: q is a tensor [batch][rows][q_heads][64]")
+    rows, hq = q.shape[1], q.shape[2]
+    pq = _tensor("attn8", "q", q, _F16, (b, rows, hq, 64))
+    po = _tensor("attn8", "out", out, _F16, (b, rows, hq, 64))
+    ln = _dense("attn8", "lens", lens, _I32, (b,)) if lens is not None else None
+    pp = ps = None
+    slots = 0
+    if probs is not None:
+        slots = probs.shape[1] if isinstance(probs, torch.Tensor) and probs.dim() == 4 else None
+        pp = _dense("attn8", "probs", probs, _F16, (b, slots, rows, cap))
+        ps = _dense("attn8", "pslot", pslot, _I32, (hq,))
+    need = lib.mmz_attn8_scratch_bytes(b, rows, hq, h, cap, slots)
+    if need and scratch is None:
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    sp, sb = _scratch("attn8", scratch)
+    s, o = q.stride(), out.stride()
+    _check(lib.mmz_attn8(pq, s[0], s[1], s[2], *c, *cs, ln, po, o[0], o[1], o[2], b, rows, hq, h, cap, block, kind,
+                         int(causal), scale, pp, ps, slots, sp, sb, _stream(stream)), "attn8")
+
+
+def _scratch(what, t):
+    return (None, 0) if t is None else (_dense(what, "scratch", t, torch.uint8, None), t.numel())
+
+
+def _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col):
+    """The pointers of the outputs, alternatives and their stride: [rows], or [rows][steps] with a column counter."""
+    if not isinstance(logp, torch.Tensor) or logp.dim() != (1 if col is None else 2):
+        raise MmzError(f"{what}: logp is a tensor [rows], or [rows][steps] with col")
+    shape = (rows,) if col is None else (rows, logp.shape[1])
+    ld = 1 if col is None else logp.shape[1]
+    got = [_dense(what, "target", target, _I32, shape), _dense(what, "logp", logp, _F32, shape)]
+    for name, t in (("entropy", entropy), ("lse", lse)):
+        got.append(None if t is None else _dense(what, name, t, _F32, shape))
+    one = top_id if top_id is not None else top_logp
+    top = one.shape[-1] if isinstance(one, torch.Tensor) and one.dim() else 0
+    got.append(None if top_id is None else _dense(what, "top_id", top_id, _I32, shape + (top,)))
+    got.append(None if top_logp is None else _dense(what, "top_logp", top_logp, _F32, shape + (top,)))
+    ps = None if sup is None else _dense(what, "sup", sup, torch.uint8, (vocab,))
+    pc = None if col is None else _dense(what, "col", col, _I32, None)
+    return ps, got + [top, ld, pc]
+
+
+def token_logprobs(logits, target, logp, entropy=None, lse=None, top_id=None, top_logp=None, sup=None, col=None,
+                   stream=None):
+    """Per row of logits [rows][vocab] (fp16 or fp32): logp[r] = log p(target[r]), the entropy, log sum e^x, and the
+    ids and log probabilities of the largest logits (top_id int32, top_logp float32 [rows][top <= 8]; ties to the lower
+    id). sup [vocab] uint8: ids left out. With col (an int32 device scalar) target and outputs are [rows][steps] and
+    column col[0] is read and written. A target outside the vocabulary has logp 0."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (_F16, _F32) or logits.dim() != 2:
+        raise MmzError("token_logprobs: logits is an fp16 or fp32 tensor [rows][vocab]")
+    rows, vocab = logits.shape
+    px = _tensor("token_logprobs", "logits", logits, logits.dtype, (rows, vocab))
+    ps, o = _outputs("token_logprobs", rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col)
+    ldx = logits.stride(0) if rows > 1 else vocab
+    _check(lib.mmz_token_logprobs(px, ldx, int(logits.dtype is _F32), rows, vocab, ps, *o, _stream(stream)),
+           "token_logprobs")
+
+
+def linear_logprobs_scratch_bytes(rows, vocab, d):
+    """Bytes of device scratch linear_logprobs needs for such a call."""
+    return lib.mmz_linear_logprobs_scratch_bytes(rows, vocab, d)
+
+
+def linear_logprobs(x, emb, target, logp, entropy=None, lse=None, top_id=None, top_logp=None, sup=None, col=None,
+                    scratch=None, stream=None):
+    """token_logprobs of the logits x . emb^T (x [rows][d], emb [vocab][d] fp16), in fp32 from the product on. scratch:
+    a uint8 tensor of linear_logprobs_scratch_bytes(rows, vocab, d) (allocated here when None)."""
+    what = "linear_logprobs"
+    if not isinstance(x, torch.Tensor) or not isinstance(emb, torch.Tensor) or x.dim() != 2 or emb.dim() != 2:
+        raise MmzError("linear_logprobs: x [rows][d] and emb [vocab][d] are tensors")
+    (rows, d), vocab = x.shape, emb.shape[0]
+    px, pe = _tensor(what, "x", x, _F16, (rows, d)), _dense(what, "emb", emb, _F16, (vocab, d))
+    ps, o = _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col)
+    if scratch is None:
+        scratch = torch.empty(lib.mmz_linear_logprobs_scratch_bytes(rows, vocab, d), dtype=torch.uint8, device=x.device)
+    sp, sb = _scratch(what, scratch)
+    ldx = x.stride(0) if rows > 1 else d
+    _check(lib.mmz_linear_logprobs(px, ldx, pe, rows, vocab, d, ps, *o, sp, sb, _stream(stream)), what)

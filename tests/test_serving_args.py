@@ -1,0 +1,114 @@
+"""The 8-bit cache and the log probabilities refuse bad arguments on the host, before a device is touched."""
+import pytest
+
+import mimizuku_b200 as m
+
+L = m.lib
+A = 1 << 20  # an aligned address that nothing reads
+
+
+def write(k=A, v=A, xs=(64, 64, 64), k8=A, v8=A, ks=A, vs=A, cs=(6400, 6400), batch=1, heads=1, n=1, cap=100, block=64,
+          kind=0):
+    return L.mmz_kv8_write(k, v, *xs, k8, v8, ks, vs, *cs, 2, 2, None, batch, heads, n, cap, block, kind, None)
+
+
+def read(k=A, v=A, xs=(64, 64, 64), k8=A, v8=A, ks=A, vs=A, cs=(6400, 6400), batch=1, heads=1, n=1, cap=100, block=64,
+         kind=0):
+    return L.mmz_kv8_read(k8, v8, ks, vs, *cs, 2, 2, k, v, *xs, None, None, batch, heads, n, cap, block, kind, None)
+
+
+@pytest.mark.parametrize("fn,name", [(write, b"kv8_write"), (read, b"kv8_read")])
+@pytest.mark.parametrize("bad,word", [
+    (dict(block=0), b"block"), (dict(block=48), b"block"), (dict(block=256), b"block"), (dict(kind=2), b"kind"),
+    (dict(kind=-1), b"kind"), (dict(batch=-1), b"batch"), (dict(heads=0), b"heads"), (dict(n=-1), b"n >= 0"),
+    (dict(cap=0), b"cap"), (dict(k=None), b"null"), (dict(ks=None), b"null"), (dict(v8=None), b"null"),
+    (dict(k=A + 8), b"aligned"), (dict(k8=A + 4), b"aligned"), (dict(xs=(64, 60, 64)), b"strides"),
+    (dict(cs=(6400, 6392)), b"strides"), (dict(batch=1 << 20, heads=1 << 12, n=99), b"2^31")])
+def test_cache_calls_refuse(fn, name, bad, word):
+    assert fn(**bad) == -1
+    msg = L.mmz_last_error()
+    assert name in msg and word in msg
+
+
+def test_nothing_to_do_is_no_error():
+    assert write(batch=0, k=None) == 0 and write(n=0, k=None) == 0
+    assert read(batch=0) == 0 and read(n=0) == 0
+    assert attend(batch=0, q=None) == 0 and attend(rows=0) == 0
+    assert logits(rows=0, x=None) == 0 and hidden(rows=0, x=None) == 0
+
+
+def attend(q=A, qs=(64, 64, 64), k8=A, cs=(6400, 6400), ks=A, out=A, os=(64, 64, 64), batch=1, rows=1, hq=1, hkv=1, cap=100,
+           block=64, kind=0, probs=None, pslot=None, slots=0, scratch=None, sb=0):
+    return L.mmz_attn8(q, *qs, k8, A, ks, A, *cs, 2, 2, None, out, *os, batch, rows, hq, hkv, cap, block, kind, 0, 0.125,
+                       probs, pslot, slots, scratch, sb, None)
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(block=8), b"block"), (dict(kind=3), b"kind"), (dict(hq=3, hkv=2), b"multiple of kv_heads"),
+    (dict(hkv=0), b"heads"), (dict(batch=-1), b"batch"), (dict(rows=-1), b"rows"), (dict(cap=0), b"cap"),
+    (dict(slots=-1), b"cap"), (dict(q=None), b"null"), (dict(out=None), b"null"), (dict(ks=None), b"null"),
+    (dict(probs=A), b"pslot"), (dict(q=A + 2), b"aligned"), (dict(out=A + 8), b"aligned"),
+    (dict(probs=A + 8, pslot=A, slots=1), b"aligned"), (dict(qs=(64, 64, 63)), b"strides"),
+    (dict(os=(64, 4, 64)), b"strides"), (dict(cs=(6401, 6400)), b"strides")])
+def test_attention_refuses(bad, word):
+    assert attend(**bad) == -1
+    msg = L.mmz_last_error()
+    assert b"attn8" in msg and word in msg
+
+
+def logits(x=A, ldx=100, type=0, rows=1, vocab=100, target=A, logp=A, top=0, ld=1):
+    return L.mmz_token_logprobs(x, ldx, type, rows, vocab, None, target, logp, None, None, None, None, top, ld, None, None)
+
+
+def hidden(x=A, ldx=64, emb=A, rows=1, vocab=100, d=64, target=A, logp=A, top=0, ld=1, scratch=None, sb=0):
+    return L.mmz_linear_logprobs(x, ldx, emb, rows, vocab, d, None, target, logp, None, None, None, None, top, ld, None,
+                                 scratch, sb, None)
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(type=2), b"type"), (dict(rows=-1), b"rows"), (dict(vocab=0), b"vocab"), (dict(ldx=99), b"ldx"),
+    (dict(top=9), b"alternatives"), (dict(top=-1), b"alternatives"), (dict(ld=0), b"stride"),
+    (dict(target=None), b"target"), (dict(x=None), b"null"), (dict(x=A + 1), b"aligned"),
+    (dict(x=A + 2, type=1), b"aligned")])
+def test_token_logprobs_refuses(bad, word):
+    assert logits(**bad) == -1
+    msg = L.mmz_last_error()
+    assert b"token_logprobs" in msg and word in msg
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(d=96), b"width"), (dict(d=0), b"width"), (dict(rows=-1), b"rows"), (dict(vocab=0), b"vocab"),
+    (dict(top=9), b"alternatives"), (dict(ld=0), b"stride"), (dict(target=None), b"target"), (dict(x=None), b"aligned"),
+    (dict(emb=A + 8), b"aligned"), (dict(ldx=56), b"ldx"), (dict(ldx=68), b"pitch"), (dict(scratch=None), b"scratch"),
+    (dict(scratch=A, sb=1), b"scratch"), (dict(scratch=A + 8, sb=1 << 30), b"scratch")])
+def test_linear_logprobs_refuses(bad, word):
+    assert hidden(**bad) == -1
+    msg = L.mmz_last_error()
+    assert b"linear_logprobs" in msg and word in msg
+
+
+def test_scratch_sizes():
+    assert L.mmz_attn8_scratch_bytes(0, 1, 1, 1, 1, 0) == 0 and L.mmz_attn8_scratch_bytes(1, 1, 1, 2, 1, 0) == 0
+    assert L.mmz_linear_logprobs_scratch_bytes(0, 1, 64) == 0 and L.mmz_linear_logprobs_scratch_bytes(1, 1, 0) == 0
+    assert m.linear_logprobs_scratch_bytes(7, 51866, 1280) % 16 == 0
+
+
+def test_python_calls_refuse_what_is_no_cuda_tensor():
+    import torch
+    k8 = torch.zeros((1, 2, 8, 64), dtype=torch.int8)
+    s = torch.zeros((1, 2, 1))
+    x = torch.zeros((1, 1, 2, 64), dtype=torch.float16)
+    with pytest.raises(m.MmzError, match="not a CUDA tensor"):
+        m.kv8_write(x, x, k8, k8, s, s)
+    with pytest.raises(m.MmzError, match="int8 or float8"):
+        m.attn8(x, x, x, s, s, x)
+    with pytest.raises(m.MmzError, match="block is"):
+        m.kv8_read(k8, k8, s, s, x, x, block=20)
+    with pytest.raises(m.MmzError, match="fp16 or fp32"):
+        m.token_logprobs(k8[0, 0], s, s)
+    with pytest.raises(m.MmzError, match="are tensors"):
+        m.linear_logprobs(None, x, s, s)
+    with pytest.raises(m.MmzError, match="not a CUDA tensor"):
+        m.linear_logprobs(x[0, 0], x[0, 0], s[0, 0], s[0, 0])
+    with pytest.raises(AttributeError):
+        m.no_such_call
