@@ -75,6 +75,7 @@ static void init_ctx(DevCtx& c, int dev) {
     init_gemm_attrs(c);
     init_gemv_attrs();
     init_align_attrs();
+    init_attn8_attrs();
     cudaGetLastError();
     c.ok = true;
     c.err = "";
