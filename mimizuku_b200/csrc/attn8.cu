@@ -13,10 +13,15 @@
 //     rows; no code is moved between lanes, and P^T is S^T's own layout after one 8 x 8 transpose.
 //   * a running maximum and sum per row; p carries a factor 2^10 (it cancels against the sum) and is split into a high
 //     and a low fp16 part, each multiplied: what is lost of p is below 2^-21 of it, and below 2^-35 of the row's
-//     largest p, so the one rounding that counts stays that of the output.
+//     largest p, so the one rounding that counts stays that of the output. Up to 4 rows the two parts are columns
+//     r and r + 4 of one product (the lanes of columns 4-7 hold the same scores and keep the low part).
 //   * the scales of a block apply in fp32: ks to the scores, vs to the sums of the positions that share it.
-// The 4 warps of a CTA join in shared memory, the CTAs of a cluster (up to 8 along the sequence) through distributed
-// shared memory, and where one cluster is too little for a long cache, clusters through scratch and a second kernel.
+// Two ways through the cache (plan() chooses):
+//   flat     many chunks, up to 8 rows: a fixed number of warps, each with an equal share of all sequences' and heads'
+//            chunks in a row, whatever the lengths; a pair's parts on several warps join in a second kernel
+//   cluster  few chunks, or more rows: a CTA to a (pair, row block), its warps along the positions (up to 32 rows) or
+//            along the rows; CTAs of a cluster split the sequence and join through distributed shared memory, and where
+//            one cluster is too little, clusters through scratch and a second kernel
 #include "attn8.h"
 #include "fp8_cache.cuh"
 #include "launch.h"
@@ -31,16 +36,14 @@ constexpr int KB = CH * HD;     // bytes of a chunk's keys (and of its values)
 constexpr int REC = HD + 2;     // a row's partial result: 64 sums, maximum, sum of p
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float PSHIFT = 10.f;  // p <= 2^10
+constexpr long FLAT_FROM = 2;   // chunks to a warp from which on the flat way is taken
 
-template <int NTL>
 struct Smem {
-    union {
-        uint8_t ring[WARPS][STG][2][KB];
-        float part[WARPS][8 * NTL][REC];  // after the last chunk
-    };
-    float join[8 * NTL][REC];             // this CTA's rows, read by the cluster
+    uint8_t ring[WARPS][STG][2][KB];
     uint64_t full[WARPS][STG];
-    int abort;
+    int abort, pad[3];
+    // cluster: followed by what the cluster's warps send this CTA for each of the block's rows: statistics float2
+    // [row][source], then sums float [row][source][64 / cs] of the dimensions that this CTA joins
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -90,109 +93,102 @@ __device__ __forceinline__ void load_q(const h16* row, int t, uint32_t (&q)[8]) 
     q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w, q[4] = y.x, q[5] = y.y, q[6] = y.z, q[7] = y.w;
 }
 
+__device__ __forceinline__ void st_dsmem_f32x4(uint32_t addr, float x, float y, float z, float w) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
+
 __device__ __forceinline__ float weight(float m, float M) { return m == -INFINITY ? 0.f : ex2_approx(m - M); }
+
+// 1 / the sum of a row's p: 0 for a row that saw nothing, NaN kept
+__device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.f / l : (l == l ? 0.f : l); }
 
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) {  // 0x80 in the bytes of w that hold e4m3's NaN
     return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
-}  // namespace a8
-using namespace a8;
-
-// grid: cluster rank fastest, then cluster along the sequence, row tile, (sequence, key head); cluster of cs CTAs.
-// part null: the cluster's rows go to out (and their statistics to stats, if not null); else to part
-template <int KIND, int NTL>
-__global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, int cs, int nclus, int tiles, float* part, float2* stats,
-                                                   unsigned* status, unsigned long long limit_ns) {
-    constexpr int RT = 8 * NTL;            // rows of a tile
-    constexpr int SUB = NTL == 1 ? 64 : 32;  // positions whose scores are in registers at a time
-    constexpr int NJ = SUB / 16;
-    extern __shared__ __align__(128) uint8_t raw[];
-    Smem<NTL>& sm = *reinterpret_cast<Smem<NTL>*>(raw);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rank = blockIdx.x % cs, clus = (blockIdx.x / cs) % nclus;
-    const int tile = (blockIdx.x / cs / nclus) % tiles;
-    const long pair = blockIdx.x / cs / nclus / tiles;
-    const int hk = (int)(pair % a.kv_heads), group = a.q_heads / a.kv_heads;
-    const long b = pair / a.kv_heads;
-    const int R = a.rows * group, r0 = tile * RT;
-    if (lane == 0)
-        for (int i = 0; i < STG; i++) mbar_init(&sm.full[warp][i], 1);
-    if (threadIdx.x == 0) sm.abort = 0;
-    fence_mbar_init();
-    __syncthreads();
-    griddep_wait();
-
-    const int L = a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap;
-    // what row r of the block sees; the tile's last row sees the most
-    auto limit = [&](int r) { return a.causal ? max(0, L - a.rows + r / group + 1) : L; };
-    const int most = limit(min(r0 + RT, R) - 1), least = limit(r0);
-    const int nch = (most + CH - 1) / CH;
-    const int ns = cs * nclus, per = (nch + ns - 1) / ns, split = clus * cs + rank;
-    const int c0 = min(split * per, nch), c1 = min(c0 + per, nch);
-    const uint8_t* k8 = a.k8 + b * a.c_seq + hk * a.c_head;
-    const uint8_t* v8 = a.v8 + b * a.c_seq + hk * a.c_head;
-    const float* ks = a.ks + b * a.s_seq + hk * a.s_head;
-    const float* vs = a.vs + b * a.s_seq + hk * a.s_head;
-
-    uint64_t* full = sm.full[warp];
-    auto issue = [&](int c, int st) {  // lane 0
-        const uint32_t bytes = (uint32_t)min(CH, most - c * CH) * HD;
-        mbar_expect_tx(&full[st], 2 * bytes);
-        bulk_g2s(sm.ring[warp][st][0], k8 + (long)c * KB, bytes, &full[st]);
-        bulk_g2s(sm.ring[warp][st][1], v8 + (long)c * KB, bytes, &full[st]);
-    };
-    // lanes 0-3: the key scales of a chunk's four tiles of 16 positions, lanes 4-7 the value scales
-    auto scale_of = [&](int c) {
-        if (lane >= 8 || c >= c1) return 0.f;
-        const int j = min(c * CH + 16 * (lane & 3), most - 1);
-        return lane < 4 ? ks[j / a.block] * (a.scale * LOG2E) : vs[j / a.block];
-    };
-    int issued = c0 + warp;
-    if (lane == 0)
-        for (int i = 0; i < STG && c0 + warp + i * WARPS < c1; i++) issue(c0 + warp + i * WARPS, i);
-    float sc_next = scale_of(c0 + warp);
-
+// A warp's rows and their running results. MODE 0: up to 4 rows, columns 4-7 repeat columns 0-3; 1: up to 8; 4: up to 32.
+// Lane (g, t) of the warp (g = lane / 4, t = lane % 4) holds columns 8 n + 2 t + e of dimensions 8 g .. 8 g + 7.
+template <int KIND, int MODE>
+struct Rows {
+    static constexpr int NTL = MODE == 4 ? 4 : 1;        // column tiles of 8
+    static constexpr int SUB = NTL == 1 ? 64 : 32;       // positions whose scores are in registers at a time
+    static constexpr int NJ = SUB / 16;
     uint32_t q[NTL][8];
-    int lim[NTL][2];
-#pragma unroll
-    for (int n = 0; n < NTL; n++) {
-        const int r = r0 + 8 * n + g;
-        if (r < R) load_q(a.q + b * a.q_seq + (r / group) * a.q_row + (hk * group + r % group) * a.q_head, t, q[n]);
-        else
-            for (int i = 0; i < 8; i++) q[n][i] = 0;
-        lim[n][0] = limit(min(r0 + 8 * n + 2 * t, R - 1));
-        lim[n][1] = limit(min(r0 + 8 * n + 2 * t + 1, R - 1));
-    }
-    float m[NTL][2], l[NTL][2], o[4][NTL][4];
-#pragma unroll
-    for (int n = 0; n < NTL; n++) {
-        m[n][0] = m[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
-    }
+    float m[NTL][2], l[NTL][2], o[4][NTL][4];  // o[i][n][e + 2 k]: dimension 8 g + 2 i + k, column 8 n + 2 t + e
 
-    const int same = min(a.block, SUB) / 16 - 1;  // tiles of 16 that share a scale, less one: 0, 1 or 3
-    bool ok = true;
-    int it = 0;
-    for (int c = c0 + warp; c < c1; c += WARPS, it++) {
-        const int st = it % STG;
-        ok = __all_sync(0xffffffff, mbar_wait(&full[st], (it / STG) & 1, &sm.abort, limit_ns, status, K_ATTN8, 1));
-        if (!ok) break;
-        const float sc = sc_next;
-        sc_next = scale_of(c + WARPS);
-        const uint8_t* ck = sm.ring[warp][st][0];
-        uint8_t* cv = sm.ring[warp][st][1];
-        const int base = c * CH;
-        // the sequence's last chunk: the rows that were not copied hold what the ring held (nothing follows this chunk
-        // in the warp's ring). Their weights are 0, but a NaN times 0 would not be
+    // the row of column c of tile n
+    static __device__ __forceinline__ int row(int n, int c) { return MODE == 0 ? c & 3 : 8 * n + c; }
+    // rows r0 .. R - 1 of a pair (heads hk * group ..), query row r / group, head r % group
+    __device__ __forceinline__ void queries(const Attn8& a, long b, int hk, int group, int r0, int R, int lane) {
+#pragma unroll
+        for (int n = 0; n < NTL; n++) {
+            const int r = r0 + row(n, lane >> 2);
+            if (r < R) load_q(a.q + b * a.q_seq + (r / group) * a.q_row + (hk * group + r % group) * a.q_head, lane & 3, q[n]);
+            else
+                for (int i = 0; i < 8; i++) q[n][i] = 0;
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NTL; n++) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+        }
+    }
+    // O = O alpha + (the values' products with P). ONE: the SUB positions share one scale; else tiles of 16 that do are
+    // `same` + 1 in number (1 or 2)
+    template <bool ONE>
+    __device__ __forceinline__ void values(const uint2 (&w)[NJ][4], const uint32_t (&ph)[NJ][NTL][2],
+                                           const uint32_t (&pl)[NJ][NTL][2], const float (&alpha)[NTL][2], float sc,
+                                           int from, int same) {
+        const float v0 = __shfl_sync(0xffffffff, sc, from);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {  // dimensions 8 g + 2 i and 8 g + 2 i + 1
+#pragma unroll
+            for (int n = 0; n < NTL; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[i][n][e] *= alpha[n][e & 1];
+            float acc[NTL][4];
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                if (j == 0 || (!ONE && (j & same) == 0))
+#pragma unroll
+                    for (int n = 0; n < NTL; n++) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+                const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+                const uint32_t x = i < 2 ? __byte_perm(w[j][0].x, w[j][1].x, sel) : __byte_perm(w[j][0].y, w[j][1].y, sel);
+                const uint32_t y = i < 2 ? __byte_perm(w[j][2].x, w[j][3].x, sel) : __byte_perm(w[j][2].y, w[j][3].y, sel);
+                const uint32_t f[4] = {codes2<KIND>(x, false), codes2<KIND>(x, true), codes2<KIND>(y, false),
+                                       codes2<KIND>(y, true)};
+#pragma unroll
+                for (int n = 0; n < NTL; n++) {
+                    mma(acc[n], f, ph[j][n][0], ph[j][n][1]);
+                    if (MODE != 0) mma(acc[n], f, pl[j][n][0], pl[j][n][1]);
+                }
+                if (ONE ? j == NJ - 1 : ((j + 1) & same) == 0) {
+                    const float vsc = ONE ? v0 : __shfl_sync(0xffffffff, sc, from + j);
+#pragma unroll
+                    for (int n = 0; n < NTL; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[i][n][e] += vsc * acc[n][e];
+                }
+            }
+        }
+    }
+    // One chunk: codes at ck, cv (shared memory), positions base .. base + 63 of which those below `most` exist. sc:
+    // lanes 0-3 the key scales (times scale log2 e) of the four tiles of 16 positions, lanes 4-7 the value scales. lim:
+    // what the lane's columns see; whole: every row sees the whole chunk.
+    __device__ __forceinline__ void chunk(const uint8_t* ck, uint8_t* cv, int base, int most, bool whole, float sc,
+                                          const int (&lim)[NTL][2], int block, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        // the sequence's last chunk: the rows that were not copied hold what the ring held. Their weights are 0, but a
+        // NaN times 0 would not be
         if (base + CH > most) {
             for (int i = (most - base) * HD + lane * 16; i < KB; i += 512)
                 *reinterpret_cast<uint4*>(cv + i) = make_uint4(0, 0, 0, 0);
             __syncwarp();
         }
-        const bool whole = base + CH <= least;  // every row sees the whole chunk
 #pragma unroll
         for (int sub = 0; sub < CH / SUB; sub++) {
             const int sb = base + sub * SUB;
@@ -227,7 +223,7 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, int cs, int nclus, i
                 for (int e = 0; e < 2; e++) {
                     float mx = m[n][e];
 #pragma unroll
-                    for (int j = 0; j < NJ; j++) mx = fmaxf(mx, fmaxf(s[j][n][e], s[j][n][e + 2]));
+                    for (int j = 0; j < NJ; j++) mx = fmax3(mx, s[j][n][e], s[j][n][e + 2]);
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffff, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffff, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffff, mx, 16));
@@ -251,8 +247,13 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, int cs, int nclus, i
                         const __half2 hi = __floats2half2_rn(x, y);
                         const float2 back = __half22float2(hi);
                         const __half2 lo = __floats2half2_rn(x - back.x, y - back.y);
-                        ph[j][n][u] = transpose8(*reinterpret_cast<const uint32_t*>(&hi));
-                        pl[j][n][u] = transpose8(*reinterpret_cast<const uint32_t*>(&lo));
+                        const uint32_t h = *reinterpret_cast<const uint32_t*>(&hi), z = *reinterpret_cast<const uint32_t*>(&lo);
+                        if (MODE == 0) {
+                            ph[j][n][u] = transpose8(t < 2 ? h : z);
+                        } else {
+                            ph[j][n][u] = transpose8(h);
+                            pl[j][n][u] = transpose8(z);
+                        }
                     }
             }
             // values: lane (g, t) has dimensions 8 g .. 8 g + 7 of positions t, t + 4, t + 8, t + 12 of each tile
@@ -290,187 +291,544 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, int cs, int nclus, i
                     nanpos[d] = min(nanpos[d], __shfl_xor_sync(0xffffffff, nanpos[d], 2));
                 }
             }
+            if (block >= SUB) values<true>(w, ph, pl, alpha, sc, 4 + sub * NJ, 0);
+            else values<false>(w, ph, pl, alpha, sc, 4 + sub * NJ, block / 16 - 1);
+            if (nans) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {  // dimensions 8 g + 2 i and 8 g + 2 i + 1
-#pragma unroll
-                for (int n = 0; n < NTL; n++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[i][n][e] *= alpha[n][e & 1];
-                float acc[NTL][4];
-#pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    if ((j & same) == 0)
-#pragma unroll
-                        for (int n = 0; n < NTL; n++) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-                    const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
-                    const uint32_t x = i < 2 ? __byte_perm(w[j][0].x, w[j][1].x, sel) : __byte_perm(w[j][0].y, w[j][1].y, sel);
-                    const uint32_t y = i < 2 ? __byte_perm(w[j][2].x, w[j][3].x, sel) : __byte_perm(w[j][2].y, w[j][3].y, sel);
-                    const uint32_t f[4] = {codes2<KIND>(x, false), codes2<KIND>(x, true), codes2<KIND>(y, false),
-                                           codes2<KIND>(y, true)};
-#pragma unroll
-                    for (int n = 0; n < NTL; n++) {
-                        mma(acc[n], f, ph[j][n][0], ph[j][n][1]);
-                        mma(acc[n], f, pl[j][n][0], pl[j][n][1]);
-                    }
-                    if (((j + 1) & same) == 0) {
-                        const float vsc = __shfl_sync(0xffffffff, sc, 4 + sub * NJ + j);
-#pragma unroll
-                        for (int n = 0; n < NTL; n++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[i][n][e] += vsc * acc[n][e];
-                    }
-                }
-                if (nans) {
+                for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int n = 0; n < NTL; n++)
 #pragma unroll
                         for (int e = 0; e < 4; e++)
                             if (nanpos[2 * i + (e >> 1)] < lim[n][e & 1]) o[i][n][e] = NAN;
-                }
             }
         }
-        __syncwarp();
-        if (lane == 0 && c + STG * WARPS < c1) issue(c + STG * WARPS, st);
-        issued = c + WARPS;
     }
-    if (!ok && lane == 0) {  // let the copies in flight land before the shared memory is used for something else
-        for (int i = 0; i < STG; i++, it++)
-            if (issued + i * WARPS < c1)
-                mbar_wait(&full[it % STG], (it / STG) & 1, nullptr, limit_ns, nullptr, 0, 0);
+    // after the last chunk: the lanes' sums of p added up, and the two parts of MODE 0. Columns with have(t) are valid
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int n = 0; n < NTL; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                l[n][e] += __shfl_xor_sync(0xffffffff, l[n][e], 4);
+                l[n][e] += __shfl_xor_sync(0xffffffff, l[n][e], 8);
+                l[n][e] += __shfl_xor_sync(0xffffffff, l[n][e], 16);
+            }
+        if (MODE == 0)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[i][0][e] += __shfl_xor_sync(0xffffffff, o[i][0][e], 2);
     }
+    static __device__ __forceinline__ bool have(int t) { return MODE != 0 || t < 2; }
+    // the finished rows, divided by their sums, to out (and their statistics)
+    __device__ __forceinline__ void store(const Attn8& a, long b, int hk, int group, int r0, int R, float2* stats, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int n = 0; n < NTL; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int r = r0 + 8 * n + 2 * t + e;
+                if (!have(t) || r >= R) continue;
+                const float inv = inverse(l[n][e]);
+                uint4 x;
+                __half2* h = reinterpret_cast<__half2*>(&x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) h[i] = __floats2half2_rn(o[i][n][e] * inv, o[i][n][e + 2] * inv);
+                *reinterpret_cast<uint4*>(a.out + b * a.o_seq + (r / group) * a.o_row + (hk * group + r % group) * a.o_head +
+                                          8 * g) = x;
+                if (stats && g == 0) stats[(b * a.kv_heads + hk) * R + r] = make_float2(m[n][e], inv);
+            }
+    }
+};
 
-    // ---------------------------------------------------------------- the warps' rows joined
+// lanes 0-3: the key scales (times scale log2 e) of a chunk's four tiles of 16 positions, lanes 4-7 the value scales
+__device__ __forceinline__ float chunk_scale(const float* ks, const float* vs, int c, int most, int shift, float scale,
+                                             int lane) {
+    if (lane >= 8) return 0.f;
+    const int j = min(c * CH + 16 * (lane & 3), most - 1) >> shift;
+    return lane < 4 ? ks[j] * (scale * LOG2E) : vs[j];
+}
+
+// How a cluster call is laid out along its CTAs (plan() below).
+struct Lay {
+    int cs, nclus;  // CTAs of a cluster, clusters along the sequence
+    int wrows;      // 0: the warps of a CTA share its rows and split the positions; 1: each has rows of its own
+    int block;      // rows of a CTA that exist at most (what its shared memory holds)
+    int tiles;      // CTAs along the rows
+};
+
+}  // namespace a8
+using namespace a8;
+
+// grid: cluster rank fastest, then cluster along the sequence, row block, (sequence, key head); cluster of cs CTAs.
+// nclus 1: the cluster's rows go to out (and their statistics to stats, if not null); else to part
+template <int KIND, int MODE>
+__global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part, float2* stats, unsigned* status,
+                                                   unsigned long long limit_ns) {
+    constexpr int NTL = Rows<KIND, MODE>::NTL, RT = 8 * NTL;
+    extern __shared__ __align__(128) uint8_t raw[];
+    Smem& sm = *reinterpret_cast<Smem*>(raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int cs = lay.cs, wstep = lay.wrows ? 1 : WARPS;
+    unsigned x = blockIdx.x;
+    const int rank = x % cs;
+    x /= cs;
+    const int clus = x % lay.nclus;
+    x /= lay.nclus;
+    const int tile = lay.tiles - 1 - (int)(x % lay.tiles);  // the last rows first: with causal they have the most to do
+    const unsigned pair = x / lay.tiles;
+    const int hk = (int)(pair % a.kv_heads), group = a.q_heads / a.kv_heads;
+    const long b = pair / a.kv_heads;
+    const int R = a.rows * group;
+    const int b0 = tile * (lay.wrows ? WARPS * RT : RT);        // first row of the CTA
+    const int r0 = b0 + (lay.wrows ? warp * RT : 0);            // first row of the warp
+    if (lane == 0)
+        for (int i = 0; i < STG; i++) mbar_init(&sm.full[warp][i], 1);
+    if (threadIdx.x == 0) sm.abort = 0;
+    fence_mbar_init();
     __syncthreads();
+    if (cs > 1) cluster_arrive_relaxed();  // the cluster's CTAs have started before anything is sent to them
+    griddep_wait();
+    griddep_launch_dependents();
+
+    Rows<KIND, MODE> w;
+    w.queries(a, b, hk, group, r0, R, lane);
+    w.clear();
+    const int L = a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap;
+    // what row r sees; the warp's last row sees the most
+    auto limit = [&](int r) { return a.causal ? max(0, L - a.rows + r / group + 1) : L; };
+    const int most = r0 < R ? limit(min(r0 + RT, R) - 1) : 0, least = r0 < R ? limit(r0) : 0;
+    const int nch = (most + CH - 1) / CH;
+    const int ns = cs * lay.nclus, per = (nch + ns - 1) / ns, split = clus * cs + rank;
+    const int c0 = min(split * per, nch), c1 = min(c0 + per, nch);
+    const int cw = c0 + (lay.wrows ? 0 : warp);  // the warp's first chunk; then every wstep-th
+    const uint8_t* k8 = a.k8 + b * a.c_seq + hk * a.c_head;
+    const uint8_t* v8 = a.v8 + b * a.c_seq + hk * a.c_head;
+    const float* ks = a.ks + b * a.s_seq + hk * a.s_head;
+    const float* vs = a.vs + b * a.s_seq + hk * a.s_head;
+    const int shift = 31 - __clz(a.block);
+
+    uint64_t* full = sm.full[warp];
+    auto issue = [&](int c, int st) {  // lane 0
+        const uint32_t bytes = (uint32_t)min(CH, most - c * CH) * HD;
+        mbar_expect_tx(&full[st], 2 * bytes);
+        bulk_g2s(sm.ring[warp][st][0], k8 + (long)c * KB, bytes, &full[st]);
+        bulk_g2s(sm.ring[warp][st][1], v8 + (long)c * KB, bytes, &full[st]);
+    };
+    auto scale_of = [&](int c) { return c < c1 ? chunk_scale(ks, vs, c, most, shift, a.scale, lane) : 0.f; };
+    int at = cw;
+    if (lane == 0)
+        for (int i = 0; i < STG && cw + i * wstep < c1; i++) issue(cw + i * wstep, i);
+    float sc_next = scale_of(cw);
+    int lim[NTL][2];
+#pragma unroll
+    for (int n = 0; n < NTL; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) lim[n][e] = limit(min(r0 + w.row(n, 2 * t + e), R - 1));
+
+    bool ok = true;
+    int it = 0;
+    for (int c = cw; c < c1; c += wstep, it++) {
+        const int st = it % STG;
+        ok = __all_sync(0xffffffff, mbar_wait(&full[st], (it / STG) & 1, &sm.abort, limit_ns, status, K_ATTN8, 1));
+        if (!ok) break;
+        const float sc = sc_next;
+        sc_next = scale_of(c + wstep);
+        w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], c * CH, most, c * CH + CH <= least, sc, lim, a.block, lane);
+        __syncwarp();
+        if (lane == 0 && c + STG * wstep < c1) issue(c + STG * wstep, st);
+        at = c + wstep;
+    }
+    if (!ok && lane == 0) {  // a wait gave up: let the copies in flight land before the CTA ends
+        for (int i = 0; i < STG; i++, it++)
+            if (at + i * wstep < c1) mbar_wait(&full[it % STG], (it / STG) & 1, nullptr, limit_ns, nullptr, 0, 0);
+    }
+    w.finish();
+
+    const int nsrc = cs * wstep;
+    if (nsrc == 1 && lay.nclus == 1) {  // every warp has its rows' whole results
+        w.store(a, b, hk, group, r0, R, stats, lane);
+        return;
+    }
+    // ---------------------------------------------------------------- the parts of a row joined
+    // Each warp sends its rows' statistics to every CTA of the cluster and its sums to the CTA that joins those
+    // dimensions (the lane's 8 have one owner): stores, and one barrier, instead of loads that are waited for.
+    const int src = rank * wstep + (lay.wrows ? 0 : warp), share = HD / cs;
+    float2* ms = reinterpret_cast<float2*>(raw + sizeof(Smem));
+    float* sums = reinterpret_cast<float*>(ms + lay.block * nsrc + (lay.block * nsrc & 1));
+    if (cs > 1) cluster_wait();
 #pragma unroll
     for (int n = 0; n < NTL; n++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            float x = l[n][e];
-            x += __shfl_xor_sync(0xffffffff, x, 4);
-            x += __shfl_xor_sync(0xffffffff, x, 8);
-            x += __shfl_xor_sync(0xffffffff, x, 16);
-            float* rec = sm.part[warp][8 * n + 2 * t + e];
-            if (g == 0) rec[HD] = m[n][e], rec[HD + 1] = x;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                rec[8 * g + 2 * i] = o[i][n][e];
-                rec[8 * g + 2 * i + 1] = o[i][n][e + 2];
-            }
+            const int r = r0 - b0 + 8 * n + 2 * t + e;  // row of the block
+            if (!w.have(t) || r >= lay.block) continue;
+            if (g < cs) st_dsmem_f32x2(dsmem_addr(&ms[r * nsrc + src], g), make_float2(w.m[n][e], w.l[n][e]));
+            const uint32_t to = dsmem_addr(&sums[(r * nsrc + src) * share + 8 * g % share], 8 * g / share);
+            st_dsmem_f32x4(to, w.o[0][n][e], w.o[0][n][e + 2], w.o[1][n][e], w.o[1][n][e + 2]);
+            st_dsmem_f32x4(to + 16, w.o[2][n][e], w.o[2][n][e + 2], w.o[3][n][e], w.o[3][n][e + 2]);
         }
-    __syncthreads();
-    for (int i = threadIdx.x; i < RT * HD; i += NT) {
-        const int r = i / HD, d = i % HD;
-        float M = -INFINITY, S = 0.f, O = 0.f;
-        for (int w = 0; w < WARPS; w++) M = fmaxf(M, sm.part[w][r][HD]);
-        for (int w = 0; w < WARPS; w++) {
-            const float f = weight(sm.part[w][r][HD], M);
-            S += f * sm.part[w][r][HD + 1];
-            O += f * sm.part[w][r][d];
-        }
-        sm.join[r][d] = O;
-        if (d == 0) sm.join[r][HD] = M, sm.join[r][HD + 1] = S;
-    }
     if (cs > 1) cluster_sync();
     else __syncthreads();
-    // ---------------------------------------------------------------- and the cluster's CTAs', each for its share
-    for (int i = rank * NT + threadIdx.x; i < RT * (HD / 2); i += cs * NT) {
-        const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
-        if (r0 + r >= R) break;
+    for (int i = threadIdx.x; i < lay.block * (share / 2); i += NT) {
+        const int r = i / (share / 2), dl = 2 * (i % (share / 2)), d = rank * share + dl;
+        if (b0 + r >= R) break;
         float M = -INFINITY, S = 0.f;
         float2 O = make_float2(0.f, 0.f);
-        for (int w = 0; w < cs; w++) M = fmaxf(M, ld_dsmem_f32(dsmem_addr(&sm.join[r][HD], w)));
-        for (int w = 0; w < cs; w++) {
-            const float2 ms = ld_dsmem_f32x2(dsmem_addr(&sm.join[r][HD], w)), x = ld_dsmem_f32x2(dsmem_addr(&sm.join[r][d], w));
-            const float f = weight(ms.x, M);
-            S += f * ms.y;
+#pragma unroll 4
+        for (int w = 0; w < nsrc; w++) M = fmaxf(M, ms[r * nsrc + w].x);
+#pragma unroll 4
+        for (int w = 0; w < nsrc; w++) {
+            const float2 y = ms[r * nsrc + w], x = *reinterpret_cast<const float2*>(&sums[(r * nsrc + w) * share + dl]);
+            const float f = weight(y.x, M);
+            S += f * y.y;
             O.x += f * x.x;
             O.y += f * x.y;
         }
-        const long row = (pair * tiles + tile) * RT + r;
-        if (nclus > 1) {
-            float* rec = part + (((pair * tiles + tile) * nclus + clus) * RT + r) * REC;
+        const long row = (long)pair * R + b0 + r;
+        if (lay.nclus > 1) {
+            float* rec = part + (row * lay.nclus + clus) * REC;
             *reinterpret_cast<float2*>(rec + d) = O;
             if (d == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(M, S);
         } else {
-            const float inv = S > 0.f ? 1.f / S : (S == S ? 0.f : S);
-            const int qi = (r0 + r) / group, h = hk * group + (r0 + r) % group;
+            const float inv = inverse(S);
+            const int qi = (b0 + r) / group, h = hk * group + (b0 + r) % group;
             *reinterpret_cast<__half2*>(a.out + b * a.o_seq + qi * a.o_row + h * a.o_head + d) =
                 __floats2half2_rn(O.x * inv, O.y * inv);
             if (stats && d == 0) stats[row] = make_float2(M, inv);
         }
     }
-    if (cs > 1) cluster_sync();  // the others may still read this CTA's rows
 }
 
-// the clusters' partial rows joined: one CTA of 128 threads to a row tile
-template <int NTL>
-__global__ void __launch_bounds__(NT) attn8_join_kernel(Attn8 a, int nclus, int tiles, const float* __restrict__ part,
-                                                        float2* stats) {
-    constexpr int RT = 8 * NTL;
-    const int tile = blockIdx.x % tiles;
-    const long pair = blockIdx.x / tiles, b = pair / a.kv_heads;
-    const int hk = (int)(pair % a.kv_heads), group = a.q_heads / a.kv_heads, R = a.rows * group, r0 = tile * RT;
-    griddep_wait();
-    for (int i = threadIdx.x; i < RT * (HD / 2); i += NT) {
-        const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
-        if (r0 + r >= R) break;
-        const float* rec = part + ((pair * tiles + tile) * nclus * RT + r) * (long)REC;
-        float M = -INFINITY, S = 0.f;
-        float2 O = make_float2(0.f, 0.f);
-        for (int w = 0; w < nclus; w++) M = fmaxf(M, rec[(long)w * RT * REC + HD]);
-        for (int w = 0; w < nclus; w++) {
-            const float* x = rec + (long)w * RT * REC;
-            const float f = weight(x[HD], M);
-            S += f * x[HD + 1];
-            O.x += f * x[d];
-            O.y += f * x[d + 1];
+// ---------------------------------------------------------------- flat
+// All chunks of all (sequence, key head) pairs in one row, pairs in order, chunks in order. Of its T chunks each of the W
+// warps has T / W, the first T % W one more. Where a pair lies on several warps, the warp with its first chunk leaves its
+// part in record 2 w + 1, the others in 2 w. (T below 2^31: 32-bit divisions, the 64-bit ones cost microseconds here.)
+namespace a8 {
+constexpr int RECF = 8 * HD + 16;  // a record: [8 rows][64] sums, [8][2] statistics
+
+struct Share {
+    unsigned T, W, per, more;
+    __device__ __forceinline__ Share(unsigned T, unsigned W) : T(T), W(W), per(T / W), more(T % W) {}
+    __device__ __forceinline__ unsigned first(unsigned w) const { return w * per + min(w, more); }
+    __device__ __forceinline__ unsigned count(unsigned w) const { return per + (w < more ? 1 : 0); }
+    __device__ __forceinline__ unsigned owner(unsigned f) const {  // the warp that has chunk f
+        const unsigned big = more * (per + 1);
+        return f < big ? f / (per + 1) : more + (f - big) / per;
+    }
+};
+struct Flat {
+    const int* lens;
+    int cap, batch, kv_heads;
+    __device__ __forceinline__ int len(int b) const { return lens ? max(0, min(lens[b], cap)) : cap; }
+    __device__ __forceinline__ unsigned chunks(int b) const { return b < batch ? (unsigned)(len(b) + CH - 1) / CH : 0; }
+    // whole warp: the chunks of the sequences before b, and of all of them
+    __device__ __forceinline__ void before(int b, int lane, unsigned& upto, unsigned& all) const {
+        upto = all = 0;
+        if (!lens) {
+            upto = (unsigned)b * chunks(0) * kv_heads;
+            all = (unsigned)batch * chunks(0) * kv_heads;
+            return;
         }
-        const float inv = S > 0.f ? 1.f / S : (S == S ? 0.f : S);
-        const int qi = (r0 + r) / group, h = hk * group + (r0 + r) % group;
-        *reinterpret_cast<__half2*>(a.out + b * a.o_seq + qi * a.o_row + h * a.o_head + d) =
-            __floats2half2_rn(O.x * inv, O.y * inv);
-        if (stats && d == 0) stats[(pair * tiles + tile) * RT + r] = make_float2(M, inv);
+        for (int i = lane; i < batch; i += 32) {
+            const unsigned n = chunks(i);
+            all += n;
+            if (i < b) upto += n;
+        }
+        all = __reduce_add_sync(0xffffffff, all) * kv_heads;
+        upto = __reduce_add_sync(0xffffffff, upto) * kv_heads;
+    }
+    // whole warp: the sequence that chunk f of the whole row lies in; f becomes its place among that sequence's
+    __device__ __forceinline__ int find(unsigned& f, int lane) const {
+        if (!lens) {
+            const unsigned per = chunks(0) * kv_heads, b = f / per;
+            f -= b * per;
+            return (int)b;
+        }
+        for (int i = 0; i < batch; i += 32) {
+            const unsigned mine = chunks(i + lane) * kv_heads;
+            unsigned up = mine;  // through this lane's sequence
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned x = __shfl_up_sync(0xffffffff, up, o);
+                if (lane >= o) up += x;
+            }
+            const unsigned hit = __ballot_sync(0xffffffff, up > f);
+            if (hit) {
+                const int k = __ffs(hit) - 1;
+                f -= __shfl_sync(0xffffffff, up - mine, k);
+                return i + k;
+            }
+            f -= __shfl_sync(0xffffffff, up, 31);
+        }
+        return batch - 1;  // not reached: f is below the total
+    }
+};
+// where a warp stands in the row of chunks
+struct Place {
+    int b, hk, c, len, nch;
+    __device__ __forceinline__ void next(const Flat& f) {
+        if (++c < nch) return;
+        c = 0;
+        if (++hk < f.kv_heads) return;
+        hk = 0;
+        do b++;
+        while (b < f.batch && (nch = ((len = f.len(b)) + CH - 1) / CH) == 0);
+    }
+};
+}  // namespace a8
+
+template <int KIND, int MODE>
+__global__ void __launch_bounds__(NT) attn8_flat_kernel(Attn8 a, float* rec, float2* stats, unsigned* status,
+                                                        unsigned long long limit_ns) {
+    extern __shared__ __align__(128) uint8_t raw[];
+    Smem& sm = *reinterpret_cast<Smem*>(raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.q_heads / a.kv_heads, R = a.rows * group;
+    const Flat flat{a.lens, a.cap, a.batch, a.kv_heads};
+    uint64_t* full = sm.full[warp];
+    if (lane == 0)
+        for (int i = 0; i < STG; i++) mbar_init(&full[i], 1);
+    if (threadIdx.x == 0) sm.abort = 0;
+    fence_mbar_init();
+    __syncthreads();  // the last barrier of the CTA: from here on the warps are on their own
+    griddep_wait();
+    griddep_launch_dependents();
+    const unsigned me = blockIdx.x * WARPS + warp;
+    unsigned upto, all;
+    flat.before(0, lane, upto, all);
+    const Share share(all, gridDim.x * WARPS);
+    const unsigned n = share.count(me);
+    if (n == 0) return;
+    Place cur;
+    {
+        unsigned f = share.first(me);
+        cur.b = flat.find(f, lane);
+        cur.len = flat.len(cur.b);
+        cur.nch = (cur.len + CH - 1) / CH;
+        cur.hk = f / (unsigned)cur.nch;
+        cur.c = f % (unsigned)cur.nch;
+    }
+    Place ahead = cur;
+    const int shift = 31 - __clz(a.block);
+    float sc[STG];  // the scales of the chunks in the ring, the next one first
+    unsigned sent = 0;
+    auto issue = [&](int st) {  // the chunk at `ahead` into stage st; returns its scales
+        const long at = (long)ahead.b * a.c_seq + ahead.hk * a.c_head + (long)ahead.c * KB;
+        if (lane == 0) {
+            const uint32_t bytes = (uint32_t)min(CH, ahead.len - ahead.c * CH) * HD;
+            mbar_expect_tx(&full[st], 2 * bytes);
+            bulk_g2s(sm.ring[warp][st][0], a.k8 + at, bytes, &full[st]);
+            bulk_g2s(sm.ring[warp][st][1], a.v8 + at, bytes, &full[st]);
+        }
+        const long sat = (long)ahead.b * a.s_seq + ahead.hk * a.s_head;
+        const float x = chunk_scale(a.ks + sat, a.vs + sat, ahead.c, ahead.len, shift, a.scale, lane);
+        sent++;
+        if (sent < n) ahead.next(flat);
+        return x;
+    };
+#pragma unroll
+    for (int i = 0; i < STG; i++) sc[i] = sent < n ? issue(i) : 0.f;
+
+    Rows<KIND, MODE> w;
+    int lim[1][2], from = cur.c;  // the segment's first chunk
+    auto begin = [&]() {
+        w.queries(a, cur.b, cur.hk, group, 0, R, lane);
+        w.clear();
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int i = min(w.row(0, 2 * t + e), R - 1) / group;
+            lim[0][e] = a.causal ? max(0, cur.len - a.rows + i + 1) : cur.len;
+        }
+        from = cur.c;
+    };
+    begin();
+    bool ok = true;
+    unsigned it = 0;
+    for (; it < n; it++) {
+        const int st = it % STG;
+        ok = __all_sync(0xffffffff, mbar_wait(&full[st], (it / STG) & 1, &sm.abort, limit_ns, status, K_ATTN8, 2));
+        if (!ok) break;
+        const int base = cur.c * CH, least = a.causal ? max(0, cur.len - a.rows + 1) : cur.len;
+        w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], base, cur.len, base + CH <= least, sc[0], lim, a.block, lane);
+        if (base + CH > cur.len) fence_proxy_async_smem();  // zeros written behind the end, before the next copy
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i + 1 < STG; i++) sc[i] = sc[i + 1];
+        if (sent < n) sc[STG - 1] = issue(st);
+        const bool last = cur.c + 1 == cur.nch;
+        if (last || it + 1 == n) {
+            w.finish();
+            if (last && from == 0) {
+                w.store(a, cur.b, cur.hk, group, 0, R, stats, lane);
+            } else {
+                float* to = rec + (2 * me + (from == 0 ? 1 : 0)) * (long)RECF;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int r = 2 * t + e;
+                    if (!w.have(t) || r >= R) continue;
+                    float4* x = reinterpret_cast<float4*>(to + r * HD + 8 * g);
+                    x[0] = make_float4(w.o[0][0][e], w.o[0][0][e + 2], w.o[1][0][e], w.o[1][0][e + 2]);
+                    x[1] = make_float4(w.o[2][0][e], w.o[2][0][e + 2], w.o[3][0][e], w.o[3][0][e + 2]);
+                    if (g == 0) *reinterpret_cast<float2*>(to + 8 * HD + 2 * r) = make_float2(w.m[0][e], w.l[0][e]);
+                }
+            }
+            if (it + 1 < n) {
+                cur.next(flat);
+                begin();
+            }
+        } else {
+            cur.c++;
+        }
+    }
+    if (!ok && lane == 0)  // a wait gave up: let the copies in flight land before the CTA ends
+        for (unsigned i = it; i < sent; i++) mbar_wait(&full[i % STG], (i / STG) & 1, nullptr, limit_ns, nullptr, 0, 0);
+}
+
+// ---------------------------------------------------------------- after the main kernel: parts joined, probabilities
+namespace a8 {
+
+// Where a row's parts lie: the k-th at (k ? more + k * step : one), its statistics `st` and its sums `so` floats in
+struct Parts {
+    const float *one, *more;
+    int step, n, st, so;  // n 0: one warp or cluster had the row, which is written; -1: an empty sequence, zeros
+    unsigned w0, none;    // flat: warps from `none` on have no chunks (fewer chunks than warps); the first is w0
+    __device__ __forceinline__ const float* at(int k) const { return k ? more + (long)k * step : one; }
+    __device__ __forceinline__ bool some(int k) const { return w0 + k < none; }
+};
+// (b, hk, r): the row's sequence, key head and place among the pair's R rows
+__device__ __forceinline__ Parts parts_of(const Attn8& a, const float* part, int nclus, unsigned W, int b, int hk, int r,
+                                          int R, int lane) {
+    Parts p;
+    p.w0 = 0, p.none = 0xffffffffu;
+    if (W == 0) {
+        p.one = p.more = part + (((long)b * a.kv_heads + hk) * R + r) * nclus * REC;
+        p.step = REC, p.n = nclus > 1 ? nclus : 0, p.st = HD, p.so = 0;
+        return p;
+    }
+    const Flat flat{a.lens, a.cap, a.batch, a.kv_heads};
+    unsigned upto, all;
+    flat.before(b, lane, upto, all);
+    const unsigned nch = flat.chunks(b);
+    p.st = 8 * HD + 2 * r, p.so = r * HD, p.n = -1;
+    if (nch == 0) return p;
+    const Share share(all, W);
+    const unsigned f0 = upto + hk * nch;
+    p.w0 = share.owner(f0);
+    p.n = (int)(share.owner(f0 + nch - 1) - p.w0 + 1);
+    if (p.n == 1) p.n = 0;
+    if (share.per == 0) p.none = share.more;
+    p.one = part + (2 * p.w0 + 1) * (long)RECF;
+    p.more = part + 2 * p.w0 * (long)RECF;
+    p.step = 2 * RECF;
+    return p;
+}
+// whole warp: parts `first`, `first` + 32 stride.. of a row joined into (M, S) and, SUMS, the lane's two dimensions
+template <bool SUMS>
+__device__ __forceinline__ void join_parts(const Parts& p, int first, int stride, int lane, float& M, float& S, float2& O) {
+    M = -INFINITY, S = 0.f, O = make_float2(0.f, 0.f);
+    for (int k0 = first; k0 < p.n; k0 += stride) {
+        const int k = k0 + lane;
+        float2 y = make_float2(-INFINITY, 0.f);
+        if (k < p.n && p.some(k)) y = *reinterpret_cast<const float2*>(p.at(k) + p.st);
+        float m = fmaxf(M, y.x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, o));
+        const float f = weight(M, m), g = weight(y.x, m);
+        M = m;
+        float s = g * y.y;  // (0 where a part saw nothing; a NaN stays)
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffff, s, o);
+        S = S * f + s;
+        if constexpr (SUMS) {
+            O.x *= f, O.y *= f;
+            const int n = min(32, p.n - k0);
+#pragma unroll 8
+            for (int j = 0; j < n; j++) {
+                const float gj = __shfl_sync(0xffffffff, g, j);
+                const bool have = __shfl_sync(0xffffffff, y.x, j) != -INFINITY;
+                const float2 x = have ? *reinterpret_cast<const float2*>(p.at(k0 + j) + p.so + 2 * lane) : make_float2(0.f, 0.f);
+                O.x += gj * x.x;
+                O.y += gj * x.y;
+            }
+        }
     }
 }
+}  // namespace a8
 
-// The probabilities of the chosen heads, from the rows' statistics: the scores again (the same products in the same
-// order), p = 2^(s - M) / S. grid: (256 positions, 8 rows) tiles of each (sequence, slot); a warp takes 64 positions
+// Blocks 0 .. jblocks - 1: a row each, its parts joined (the warps share them) and written; the others: the
+// probabilities of 8 rows and 256 positions of a (sequence, slot), p = 2^(s - M) / S with the scores computed again (the
+// same products in the same order). All but the parts and statistics is read before the wait for the main kernel, which
+// lets this one start once it has waited for what came before.
 template <int KIND>
-__global__ void __launch_bounds__(NT) attn8_probs_kernel(Attn8 a, int tiles, int rt, const float2* __restrict__ stats) {
+__global__ void __launch_bounds__(NT) attn8_post_kernel(Attn8 a, unsigned jblocks, int nclus, unsigned W,
+                                                        const float* part, const float2* stats) {
+    __shared__ float red[WARPS][REC];
+    __shared__ float2 rowms[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.q_heads / a.kv_heads, R = a.rows * group;
+    if (blockIdx.x < jblocks) {
+        const int r = blockIdx.x % R;
+        const unsigned pair = blockIdx.x / R;
+        const int hk = pair % a.kv_heads, b = pair / a.kv_heads;
+        const Parts p = parts_of(a, part, nclus, W, b, hk, r, R, lane);
+        griddep_wait();
+        griddep_launch_dependents();
+        if (p.n == 0) return;
+        float M, S;
+        float2 O;
+        join_parts<true>(p, 32 * warp, 32 * WARPS, lane, M, S, O);
+        red[warp][2 * lane] = O.x;
+        red[warp][2 * lane + 1] = O.y;
+        if (lane == 0) red[warp][HD] = M, red[warp][HD + 1] = S;
+        __syncthreads();
+        if (warp) return;
+        float m = M;
+        for (int w = 1; w < WARPS; w++) m = fmaxf(m, red[w][HD]);
+        S = 0.f, O = make_float2(0.f, 0.f);
+        for (int w = 0; w < WARPS; w++) {
+            const float f = weight(red[w][HD], m);
+            S += f * red[w][HD + 1];
+            O.x += f * red[w][2 * lane];
+            O.y += f * red[w][2 * lane + 1];
+        }
+        const float inv = inverse(S);
+        const int h = hk * group + r % group;
+        *reinterpret_cast<__half2*>(a.out + (long)b * a.o_seq + (r / group) * a.o_row + h * a.o_head + 2 * lane) =
+            __floats2half2_rn(O.x * inv, O.y * inv);
+        return;
+    }
     const int pt = (a.cap + 255) / 256, nrt = (a.rows + 7) / 8;
-    const int pblk = blockIdx.x % pt, rtile = (blockIdx.x / pt) % nrt, slot = (blockIdx.x / pt / nrt) % a.slots;
-    const long b = blockIdx.x / pt / nrt / a.slots;
-    griddep_wait();
-    int h = -1;
+    unsigned x = blockIdx.x - jblocks;
+    const int pblk = x % pt;
+    x /= pt;
+    const int rtile = x % nrt;
+    x /= nrt;
+    const int slot = x % a.slots;
+    const long b = x / a.slots;
+    int h = 0x7fffffff;
     for (int i = lane; i < a.q_heads; i += 32)
-        if (h < 0 && a.pslot[i] == slot) h = i;
-    h = __reduce_min_sync(0xffffffff, h < 0 ? 0x7fffffff : h);
-    if (h >= a.q_heads) return;
-    const int group = a.q_heads / a.kv_heads, hk = h / group;
+        if (h == 0x7fffffff && a.pslot[i] == slot) h = i;
+    h = __reduce_min_sync(0xffffffff, h);
+    const bool live = h < a.q_heads;  // a slot that no head has is left as it is
+    const int hk = live ? h / group : 0, r0 = rtile * 8;
     const int L = a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap;
     const uint8_t* k8 = a.k8 + b * a.c_seq + hk * a.c_head;
     const float* ks = a.ks + b * a.s_seq + hk * a.s_head;
     uint32_t q[1][8];
-    const int r0 = rtile * 8;
-    if (r0 + g < a.rows) load_q(a.q + b * a.q_seq + (r0 + g) * a.q_row + h * a.q_head, t, q[0]);
+    if (live && r0 + g < a.rows) load_q(a.q + b * a.q_seq + (r0 + g) * a.q_row + h * a.q_head, t, q[0]);
     else
         for (int i = 0; i < 8; i++) q[0][i] = 0;
-    float2 ms[2];
-    int lim[2];
-    for (int e = 0; e < 2; e++) {
-        const int i = min(r0 + 2 * t + e, a.rows - 1), r = i * group + h % group;
-        ms[e] = stats[((b * a.kv_heads + hk) * tiles + r / rt) * (long)rt + r % rt];
-        lim[e] = a.causal ? max(0, L - a.rows + i + 1) : L;
-    }
     const int last = a.causal ? max(0, L - a.rows + min(r0 + 8, a.rows)) : L;  // positions that some row sees
+    float s[4][1][4];
+#pragma unroll
     for (int j = 0; j < 4; j++) {
         const int base = pblk * 256 + warp * 64 + j * 16;
-        if (base >= a.cap) break;
-        float s[1][4] = {};
-        if (base + 16 <= last) {
-            scores16<KIND, 1>(k8 + (long)base * HD, lane, q, s);
-        } else if (base < last) {  // rows past the cache's end are not read: the last visible one instead
+        s[j][0][0] = s[j][0][1] = s[j][0][2] = s[j][0][3] = 0.f;
+        if (live && base + 16 <= last) {
+            scores16<KIND, 1>(k8 + (long)base * HD, lane, q, s[j]);
+        } else if (live && base < last) {  // rows past the sequence's end are not read: its last one instead
             const int p0 = min(base + place(g), last - 1), p1 = min(base + place(g) + 8, last - 1);
             const uint4 lo = *reinterpret_cast<const uint4*>(k8 + (long)p0 * HD + 16 * t);
             const uint4 hi = *reinterpret_cast<const uint4*>(k8 + (long)p1 * HD + 16 * t);
@@ -479,70 +837,117 @@ __global__ void __launch_bounds__(NT) attn8_probs_kernel(Attn8 a, int tiles, int
             for (int e = 0; e < 4; e++) {
                 const uint32_t f[4] = {codes2<KIND>(wl[e], false), codes2<KIND>(wh[e], false), codes2<KIND>(wl[e], true),
                                        codes2<KIND>(wh[e], true)};
-                mma(s[0], f, q[0][2 * e], q[0][2 * e + 1]);
+                mma(s[j][0], f, q[0][2 * e], q[0][2 * e + 1]);
             }
         }
-        const float f = base < last ? ks[base / a.block] * (a.scale * LOG2E) : 0.f;
+        const float f = live && base < last ? ks[base / a.block] * (a.scale * LOG2E) : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[j][0][e] *= f;
+    }
+    const long prow = (b * a.kv_heads + hk) * R + h % group;  // the head's row 0; row i lies i * group on
+    const int i0 = r0 + 2 * warp;                             // the warp's two rows
+    Parts p[2];
+    for (int e = 0; e < 2; e++)
+        if (live && i0 + e < a.rows) p[e] = parts_of(a, part, nclus, W, (int)b, hk, (i0 + e) * group + h % group, R, lane);
+    griddep_wait();
+    griddep_launch_dependents();
+    if (!live) return;
+    for (int e = 0; e < 2; e++)
+        if (i0 + e < a.rows) {
+            float M, S;
+            float2 O;
+            if (p[e].n > 0) {
+                join_parts<false>(p[e], 0, 32, lane, M, S, O);
+                if (lane == 0) rowms[2 * warp + e] = make_float2(M, inverse(S));
+            } else if (lane == 0) {
+                rowms[2 * warp + e] = p[e].n == 0 ? stats[prow + (long)(i0 + e) * group] : make_float2(0.f, 0.f);
+            }
+        }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int base = pblk * 256 + warp * 64 + j * 16;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int p = base + place(g) + 8 * (e >> 1), i = r0 + 2 * t + (e & 1);
-            if (p >= a.cap || i >= a.rows) continue;
-            const float x =
-                p < lim[e & 1] ? ex2_approx(s[0][e] * f - (ms[e & 1].x - PSHIFT)) * ms[e & 1].y : 0.f;
-            a.probs[((b * a.slots + slot) * a.rows + i) * (long)a.cap + p] = __float2half_rn(x);
+            const int pos = base + place(g) + 8 * (e >> 1), i = r0 + 2 * t + (e & 1);
+            if (pos >= a.cap || i >= a.rows) continue;
+            const float2 ms = rowms[2 * t + (e & 1)];
+            const int lim = a.causal ? max(0, L - a.rows + i + 1) : L;
+            const float v = pos < lim ? ex2_approx(s[j][0][e] - (ms.x - PSHIFT)) * ms.y : 0.f;
+            a.probs[((b * a.slots + slot) * a.rows + i) * (long)a.cap + pos] = __float2half_rn(v);
         }
     }
 }
 
-// How a call is laid out, from its sizes alone (lens is on the device): rows of a tile, tiles, CTAs of a cluster and
-// clusters along the sequence, and the scratch.
+// The layout of a call, from its sizes alone (lens is on the device), and its scratch.
 namespace {
+constexpr long SLOTS = 148 * 3;  // CTAs that a B200 holds at once (shared memory: 3 to an SM)
 struct Plan {
-    int ntl, tiles, cs, nclus;
-    size_t part, stats;
+    int mode;   // Rows' MODE
+    bool flat;
+    Lay lay;
+    size_t smem, part, stats;
 };
 Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     Plan p;
-    const long R = (long)rows * (q_heads / kv_heads);
-    p.ntl = R <= 8 ? 1 : 4;
-    p.tiles = (int)((R + 8 * p.ntl - 1) / (8 * p.ntl));
-    const long units = (long)batch * kv_heads * p.tiles, chunks = ((long)cap + CH - 1) / CH;
-    // CTAs for every SM several times over (148 SMs x 3 resident x 2), and a chunk at least to each warp
-    long s = (888 + units - 1) / units;
-    const long top = (chunks + WARPS - 1) / WARPS;
+    const long R = (long)rows * (q_heads / kv_heads), pairs = (long)batch * kv_heads, chunks = ((long)cap + CH - 1) / CH;
+    const long rt = R <= 8 ? 8 : 32;
+    p.mode = R <= 4 ? 0 : R <= 8 ? 1 : 4;
+    p.stats = slots > 0 ? (size_t)pairs * R * 8 : 0;
+    p.flat = R <= 8 && pairs * chunks >= FLAT_FROM * SLOTS * WARPS && pairs * chunks < 0x7fffffffl;
+    if (p.flat) {
+        p.lay = {1, 1, 0, 0, 1};
+        p.smem = sizeof(Smem);
+        p.part = (size_t)SLOTS * WARPS * 2 * RECF * 4;
+        return p;
+    }
+    p.lay.wrows = R > 32;
+    const long block = p.lay.wrows ? WARPS * rt : rt;
+    p.lay.block = (int)(R < block ? R : block);
+    p.lay.tiles = (int)((R + block - 1) / block);
+    // CTAs for every SM, and a chunk at least to each warp
+    const long units = pairs * p.lay.tiles, top = p.lay.wrows ? chunks : (chunks + WARPS - 1) / WARPS;
+    long s = (SLOTS + units - 1) / units;
     if (s > top) s = top;
-    p.cs = s <= 1 ? 1 : s <= 2 ? 2 : s <= 4 ? 4 : 8;
-    p.nclus = (int)((s + p.cs - 1) / p.cs);
-    const size_t rr = (size_t)units * 8 * p.ntl;
-    p.part = p.nclus > 1 ? ((rr * p.nclus * REC * 4 + 15) & ~(size_t)15) : 0;
-    p.stats = slots > 0 ? rr * 8 : 0;
+    const int cs = s <= 1 ? 1 : s <= 2 ? 2 : s <= 4 ? 4 : 8;
+    p.lay.cs = cs;
+    p.lay.nclus = (int)((s + cs - 1) / cs);
+    const size_t n = (size_t)p.lay.block * cs * (p.lay.wrows ? 1 : WARPS);  // (row, source) pairs
+    p.smem = sizeof(Smem) + (n + (n & 1)) * 8 + n * (HD / cs) * 4;
+    p.part = p.lay.nclus > 1 ? ((size_t)pairs * R * p.lay.nclus * REC * 4 + 15) & ~(size_t)15 : 0;
     return p;
 }
 
-template <int KIND, int NTL>
+template <int KIND, int MODE>
 int launch_main(const Attn8& a, const Plan& p, float* part, float2* stats, DevCtx& dc, cudaStream_t st) {
-    const size_t smem = sizeof(Smem<NTL>);
+    if constexpr (MODE != 4) {
+        if (p.flat)
+            return check_pdl(launch_pdl(attn8_flat_kernel<KIND, MODE>, dim3(SLOTS), dim3(NT), p.smem, st, a, part, stats,
+                                        dc.status, dc.limit_ns),
+                             "attn8");
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long)a.batch * a.kv_heads * p.tiles * p.nclus * p.cs));
+    cfg.gridDim = dim3((unsigned)((long)a.batch * a.kv_heads * p.lay.tiles * p.lay.nclus * p.lay.cs));
     cfg.blockDim = dim3(NT);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = p.smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = p.cs;
+    at[1].val.clusterDim.x = p.lay.cs;
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    if (check_pdl(cudaLaunchKernelEx(&cfg, attn8_kernel<KIND, NTL>, a, p.cs, p.nclus, p.tiles, part, stats, dc.status,
-                                     dc.limit_ns),
-                  "attn8"))
-        return -1;
-    if (p.nclus == 1) return 0;
-    return check_pdl(launch_pdl(attn8_join_kernel<NTL>, dim3((unsigned)((long)a.batch * a.kv_heads * p.tiles)), dim3(NT),
-                                0, st, a, p.nclus, p.tiles, (const float*)part, stats),
+    return check_pdl(cudaLaunchKernelEx(&cfg, attn8_kernel<KIND, MODE>, a, p.lay, part, stats, dc.status, dc.limit_ns),
                      "attn8");
+}
+
+template <int KIND>
+int launch_mode(const Attn8& a, const Plan& p, float* part, float2* stats, DevCtx& dc, cudaStream_t st) {
+    return p.mode == 0   ? launch_main<KIND, 0>(a, p, part, stats, dc, st)
+           : p.mode == 1 ? launch_main<KIND, 1>(a, p, part, stats, dc, st)
+                         : launch_main<KIND, 4>(a, p, part, stats, dc, st);
 }
 }  // namespace
 
@@ -569,31 +974,38 @@ int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, 
     const int slots = a.probs ? a.slots : 0;
     if ((long)a.rows * (a.q_heads / a.kv_heads) > 0x7fffff00l) return fail("attn8: too many rows in one call");
     const Plan p = plan(a.batch, a.rows, a.q_heads, a.kv_heads, a.cap, slots);
-    const long grid = (long)a.batch * a.kv_heads * p.tiles * p.nclus * p.cs;
-    const long pgrid = (long)a.batch * slots * ((a.rows + 7) / 8) * ((a.cap + 255) / 256);
-    if (grid > 0x7fffffffl || pgrid > 0x7fffffffl) return fail("attn8: more than 2^31 blocks in one call");
+    const long grid = (long)a.batch * a.kv_heads * p.lay.tiles * p.lay.nclus * p.lay.cs;
+    const long jblocks = p.flat || p.lay.nclus > 1 ? (long)a.batch * a.rows * a.q_heads : 0;  // rows with parts
+    const long post = jblocks + (long)a.batch * slots * ((a.rows + 7) / 8) * ((a.cap + 255) / 256);
+    if (grid > 0x7fffffffl || post > 0x7fffffffl) return fail("attn8: more than 2^31 blocks in one call");
     if (p.part + p.stats && (!scratch || ((uintptr_t)scratch & 15) || scratch_bytes < p.part + p.stats))
         return fail("attn8: scratch too small or not 16-byte aligned");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     float* part = (float*)scratch;
     float2* stats = slots ? (float2*)((char*)scratch + p.part) : nullptr;
-    int r;
-    if (kind == KV8_INT8)
-        r = p.ntl == 1 ? launch_main<KV8_INT8, 1>(a, p, part, stats, dc, st) : launch_main<KV8_INT8, 4>(a, p, part, stats, dc, st);
-    else
-        r = p.ntl == 1 ? launch_main<KV8_E4M3, 1>(a, p, part, stats, dc, st) : launch_main<KV8_E4M3, 4>(a, p, part, stats, dc, st);
-    if (r || !slots) return r;
-    auto* fn = kind == KV8_INT8 ? attn8_probs_kernel<KV8_INT8> : attn8_probs_kernel<KV8_E4M3>;
-    return check_pdl(launch_pdl(fn, dim3((unsigned)pgrid), dim3(NT), 0, st, a, p.tiles, 8 * p.ntl, (const float2*)stats),
+    const int r = kind == KV8_INT8 ? launch_mode<KV8_INT8>(a, p, part, stats, dc, st)
+                                   : launch_mode<KV8_E4M3>(a, p, part, stats, dc, st);
+    if (r || !post) return r;
+    auto* fn = kind == KV8_INT8 ? attn8_post_kernel<KV8_INT8> : attn8_post_kernel<KV8_E4M3>;
+    return check_pdl(launch_pdl(fn, dim3((unsigned)post), dim3(NT), 0, st, a, (unsigned)jblocks, p.lay.nclus,
+                                p.flat ? (unsigned)(SLOTS * WARPS) : 0u, (const float*)part, (const float2*)stats),
                      "attn8");
 }
 
 void init_attn8_attrs() {
-    cudaFuncSetAttribute(attn8_kernel<KV8_INT8, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem<1>));
-    cudaFuncSetAttribute(attn8_kernel<KV8_E4M3, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem<1>));
-    cudaFuncSetAttribute(attn8_kernel<KV8_INT8, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem<4>));
-    cudaFuncSetAttribute(attn8_kernel<KV8_E4M3, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem<4>));
+    const int most = (int)(sizeof(Smem) + WARPS * 32 * (8 * 8 + HD * 4));  // any layout's shared memory
+    auto set = [&](auto* fn) { cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, most); };
+    set(attn8_kernel<KV8_INT8, 0>);
+    set(attn8_kernel<KV8_INT8, 1>);
+    set(attn8_kernel<KV8_INT8, 4>);
+    set(attn8_kernel<KV8_E4M3, 0>);
+    set(attn8_kernel<KV8_E4M3, 1>);
+    set(attn8_kernel<KV8_E4M3, 4>);
+    set(attn8_flat_kernel<KV8_INT8, 0>);
+    set(attn8_flat_kernel<KV8_INT8, 1>);
+    set(attn8_flat_kernel<KV8_E4M3, 0>);
+    set(attn8_flat_kernel<KV8_E4M3, 1>);
 }
 
 }  // namespace mmz

@@ -35,8 +35,8 @@ using namespace kv8;
 
 // grid: items / (4 / W) CTAs, an item = one (sequence, head, k or v, block); W warps to an item
 template <int KIND>
-__global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* __restrict__ k, const h16* __restrict__ v, long x_seq,
-                                                       long x_tok, long x_head, Cache c, const int* __restrict__ pos,
+__global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* k, const h16* v, long x_seq,
+                                                       long x_tok, long x_head, Cache c, const int* pos,
                                                        int heads, int n, int cap, int block, int nblk, long items) {
     __shared__ float wmax[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -129,9 +129,9 @@ __global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* __restrict__ k
 
 // thread = 8 values of one token and head, of k and then of v
 template <int KIND>
-__global__ void __launch_bounds__(256) kv8_read_kernel(Cache c, h16* __restrict__ k, h16* __restrict__ v, long y_seq,
-                                                       long y_tok, long y_head, const int* __restrict__ pos,
-                                                       const int* __restrict__ lens, int heads, int n, int cap,
+__global__ void __launch_bounds__(256) kv8_read_kernel(Cache c, h16* k, h16* v, long y_seq,
+                                                       long y_tok, long y_head, const int* pos,
+                                                       const int* lens, int heads, int n, int cap,
                                                        int block, long items) {
     const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
     griddep_wait();

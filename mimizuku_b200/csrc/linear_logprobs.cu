@@ -9,8 +9,8 @@ constexpr int T = 64;  // tile of the product
 }  // namespace ll
 
 // y[rows][V] = x . emb^T, 64 x 64 tiles, 4 x 4 sums to a thread
-__global__ void __launch_bounds__(256) linear_kernel(const h16* __restrict__ x, long ldx, const h16* __restrict__ emb,
-                                                     int rows, int V, int d, float* __restrict__ y) {
+__global__ void __launch_bounds__(256) linear_kernel(const h16* x, long ldx, const h16* emb,
+                                                     int rows, int V, int d, float* y) {
     __shared__ float xs[16][ll::T + 1], es[16][ll::T + 1];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const long r0 = (long)blockIdx.y * ll::T, v0 = (long)blockIdx.x * ll::T;

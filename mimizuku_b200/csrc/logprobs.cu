@@ -11,8 +11,8 @@ constexpr int NT = 512;
 }  // namespace lp
 
 template <typename T>
-__global__ void __launch_bounds__(lp::NT) token_logprobs_kernel(const T* __restrict__ x, long ldx, int V,
-                                                                const unsigned char* __restrict__ sup, LogpOut o) {
+__global__ void __launch_bounds__(lp::NT) token_logprobs_kernel(const T* x, long ldx, int V,
+                                                                const unsigned char* sup, LogpOut o) {
     __shared__ RowStat st[16];
     __shared__ unsigned long long best[16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

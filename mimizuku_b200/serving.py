@@ -4,63 +4,81 @@ Every call works on the current device and stream (or `stream`), checks its tens
 without waiting; outputs are tensors that the caller gives."""
 import torch
 
-from . import MmzError, _check, _stream, lib
+from . import MmzError, _check, lib
 
 _KIND = {torch.int8: 0, torch.float8_e4m3fn: 1}
-_I32, _F16, _F32 = torch.int32, torch.float16, torch.float32
+_I32, _F16, _F32, _U8 = torch.int32, torch.float16, torch.float32, torch.uint8
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _tensor(what, name, t, dtype, shape=None, last=True):
-    """A CUDA tensor of the current device with that dtype and shape (None: any length), its last dimension dense."""
+def _device():
+    return torch.cuda.current_device() if torch.cuda.is_available() else 0
+
+
+def _stream(stream, dev):
+    if stream is None:
+        return _raw_stream(dev)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _refuse(what, name, t, dtype, shape, dev):
+    """Says what is wrong with a tensor that is no CUDA tensor of that dtype, shape (None: any) and device."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise MmzError(f"{what}: {name} is not a CUDA tensor")
     if t.dtype is not dtype:
         raise MmzError(f"{what}: {name} is {t.dtype}, not {dtype}")
-    if t.get_device() != torch.cuda.current_device():
-        raise MmzError(f"{what}: {name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    if shape is not None:
-        got = t.shape
-        if len(got) != len(shape) or any(n is not None and n != g for n, g in zip(shape, got)):
-            raise MmzError(f"{what}: {name} is {tuple(got)}, not {tuple(shape)}")
-        if last and got and got[-1] > 1 and t.stride(-1) != 1:
-            raise MmzError(f"{what}: the last dimension of {name} is not dense")
+    if t.get_device() != dev:
+        raise MmzError(f"{what}: {name} is on {t.device}, the current device is cuda:{dev}")
+    if shape is not None and t.shape != shape:
+        raise MmzError(f"{what}: {name} is {tuple(t.shape)}, not {tuple(shape)}")
+    raise MmzError(f"{what}: {name} is not contiguous")
+
+
+def _strided(what, name, t, dtype, shape, dev):
+    """The address of a CUDA tensor of the current device with that dtype and shape."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
+        _refuse(what, name, t, dtype, shape, dev)
     return t.data_ptr()
 
 
-def _dense(what, name, t, dtype, shape):
-    p = _tensor(what, name, t, dtype, shape)
-    if not t.is_contiguous():
-        raise MmzError(f"{what}: {name} is not contiguous")
-    return p
+def _dense(what, name, t, dtype, shape, dev):
+    """The same of a contiguous one; None for None."""
+    if t is None:
+        return None
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev
+            or shape is not None and t.shape != shape or not t.is_contiguous()):
+        _refuse(what, name, t, dtype, shape, dev)
+    return t.data_ptr()
 
 
-def _cache(what, k8, v8, ks, vs, block):
-    """(batch, heads, cap, kind, pointers, strides) of a cache."""
+def _cache(what, k8, v8, ks, vs, block, dev):
+    """(batch, heads, cap, kind, pointers and strides) of a cache."""
     if not isinstance(k8, torch.Tensor) or k8.dtype not in _KIND or k8.dim() != 4 or k8.shape[3] != 64:
         raise MmzError(f"{what}: k8 is an int8 or float8_e4m3fn tensor [batch][heads][cap][64]")
-    b, h, cap, _ = k8.shape
     if block not in (16, 32, 64, 128):
         raise MmzError(f"{what}: block is 16, 32, 64 or 128")
-    nb = (cap + block - 1) // block
-    ptrs = (_tensor(what, "k8", k8, k8.dtype, (b, h, cap, 64)), _tensor(what, "v8", v8, k8.dtype, (b, h, cap, 64)),
-            _tensor(what, "ks", ks, _F32, (b, h, nb)), _tensor(what, "vs", vs, _F32, (b, h, nb)))
+    shape, dtype = k8.shape, k8.dtype
+    b, h, cap, _ = shape
+    blocks = (b, h, (cap + block - 1) // block)
+    pk, pv = _strided(what, "k8", k8, dtype, shape, dev), _strided(what, "v8", v8, dtype, shape, dev)
+    qk, qv = _strided(what, "ks", ks, _F32, blocks, dev), _strided(what, "vs", vs, _F32, blocks, dev)
     cs, ss = k8.stride(), ks.stride()
-    if cap > 1 and cs[2] != 64:
-        raise MmzError(f"{what}: a head's rows of the cache lie one after another")
     if v8.stride() != cs or vs.stride() != ss:
         raise MmzError(f"{what}: keys and values of the cache have the same strides")
-    return b, h, cap, _KIND[k8.dtype], ptrs, (cs[0], cs[1], ss[0], ss[1])
+    if cs[3] != 1 or cap > 1 and cs[2] != 64 or blocks[2] > 1 and ss[2] != 1:
+        raise MmzError(f"{what}: a head's rows of the cache, and its scales, lie one after another")
+    return b, h, cap, _KIND[dtype], (pk, pv, qk, qv, cs[0], cs[1], ss[0], ss[1])
 
 
-def _pair(what, k, v, b, h):
+def _pair(what, k, v, b, h, dev):
     """Pointers, token count and shared strides of k and v [batch][n][heads][64] fp16."""
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise MmzError(f"{what}: k is a tensor [batch][n][heads][64]")
     n = k.shape[1]
-    pk, pv = _tensor(what, "k", k, _F16, (b, n, h, 64)), _tensor(what, "v", v, _F16, (b, n, h, 64))
+    pk, pv = _strided(what, "k", k, _F16, (b, n, h, 64), dev), _strided(what, "v", v, _F16, (b, n, h, 64), dev)
     s = k.stride()
-    if v.stride() != s:
-        raise MmzError(f"{what}: k and v have the same strides")
+    if v.stride() != s or s[3] != 1:
+        raise MmzError(f"{what}: k and v have the same strides, the last dimension dense")
     return pk, pv, n, s
 
 
@@ -68,21 +86,22 @@ def kv8_write(k, v, k8, v8, ks, vs, block=64, pos=None, stream=None):
     """Quantises the tokens k, v [b][n][heads][64] fp16 into the cache k8, v8 [b][heads][cap][64] (int8 or
     float8_e4m3fn) with the scales ks, vs [b][heads][ceil(cap / block)] float32, at positions pos[b].. (int32 [b]; None:
     from 0). A block that already has tokens keeps at least its scale; its codes are rounded again when it grows."""
-    b, h, cap, kind, c, cs = _cache("kv8_write", k8, v8, ks, vs, block)
-    pk, pv, n, s = _pair("kv8_write", k, v, b, h)
-    at = _dense("kv8_write", "pos", pos, _I32, (b,)) if pos is not None else None
-    _check(lib.mmz_kv8_write(pk, pv, s[0], s[1], s[2], *c, *cs, at, b, h, n, cap, block, kind, _stream(stream)),
+    dev = _device()
+    b, h, cap, kind, c = _cache("kv8_write", k8, v8, ks, vs, block, dev)
+    pk, pv, n, s = _pair("kv8_write", k, v, b, h, dev)
+    at = _dense("kv8_write", "pos", pos, _I32, (b,), dev)
+    _check(lib.mmz_kv8_write(pk, pv, s[0], s[1], s[2], *c, at, b, h, n, cap, block, kind, _stream(stream, dev)),
            "kv8_write")
 
 
 def kv8_read(k8, v8, ks, vs, k, v, block=64, pos=None, lens=None, stream=None):
     """The cache's values at positions pos[b].. (None: from 0) into k, v [b][n][heads][64] fp16, zeros from position
     min(lens[b], cap) on (lens None: cap)."""
-    b, h, cap, kind, c, cs = _cache("kv8_read", k8, v8, ks, vs, block)
-    pk, pv, n, s = _pair("kv8_read", k, v, b, h)
-    at = _dense("kv8_read", "pos", pos, _I32, (b,)) if pos is not None else None
-    ln = _dense("kv8_read", "lens", lens, _I32, (b,)) if lens is not None else None
-    _check(lib.mmz_kv8_read(*c, *cs, pk, pv, s[0], s[1], s[2], at, ln, b, h, n, cap, block, kind, _stream(stream)),
+    dev = _device()
+    b, h, cap, kind, c = _cache("kv8_read", k8, v8, ks, vs, block, dev)
+    pk, pv, n, s = _pair("kv8_read", k, v, b, h, dev)
+    at, ln = _dense("kv8_read", "pos", pos, _I32, (b,), dev), _dense("kv8_read", "lens", lens, _I32, (b,), dev)
+    _check(lib.mmz_kv8_read(*c, pk, pv, s[0], s[1], s[2], at, ln, b, h, n, cap, block, kind, _stream(stream, dev)),
            "kv8_read")
 
 
@@ -98,48 +117,51 @@ def attn8(q, k8, v8, ks, vs, out, block=64, lens=None, causal=False, scale=0.125
     positions. A row that sees nothing gives zeros. probs [b][slots][rows][cap] fp16 receives the probabilities of the
     heads with pslot[head] >= 0 (int32 [q_heads]). scratch: a uint8 tensor of attn8_scratch_bytes(...) (allocated here
     when None and needed)."""
-    b, h, cap, kind, c, cs = _cache("attn8", k8, v8, ks, vs, block)
+    dev = _device()
+    b, h, cap, kind, c = _cache("attn8", k8, v8, ks, vs, block, dev)
     if not isinstance(q, torch.Tensor) or q.dim() != 4:
         raise MmzError("attn8: q is a tensor [batch][rows][q_heads][64]")
-    rows, hq = q.shape[1], q.shape[2]
-    pq = _tensor("attn8", "q", q, _F16, (b, rows, hq, 64))
-    po = _tensor("attn8", "out", out, _F16, (b, rows, hq, 64))
-    ln = _dense("attn8", "lens", lens, _I32, (b,)) if lens is not None else None
+    shape = q.shape
+    rows, hq = shape[1], shape[2]
+    if shape[0] != b or shape[3] != 64:
+        raise MmzError(f"attn8: q is {tuple(shape)}, not {(b, rows, hq, 64)}")
+    pq, po = _strided("attn8", "q", q, _F16, shape, dev), _strided("attn8", "out", out, _F16, shape, dev)
+    s, o = q.stride(), out.stride()
+    if s[3] != 1 or o[3] != 1:
+        raise MmzError("attn8: the last dimension of q and out is dense")
+    ln = _dense("attn8", "lens", lens, _I32, (b,), dev)
     pp = ps = None
     slots = 0
     if probs is not None:
-        slots = probs.shape[1] if isinstance(probs, torch.Tensor) and probs.dim() == 4 else None
-        pp = _dense("attn8", "probs", probs, _F16, (b, slots, rows, cap))
-        ps = _dense("attn8", "pslot", pslot, _I32, (hq,))
-    need = lib.mmz_attn8_scratch_bytes(b, rows, hq, h, cap, slots)
-    if need and scratch is None:
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    sp, sb = _scratch("attn8", scratch)
-    s, o = q.stride(), out.stride()
-    _check(lib.mmz_attn8(pq, s[0], s[1], s[2], *c, *cs, ln, po, o[0], o[1], o[2], b, rows, hq, h, cap, block, kind,
-                         int(causal), scale, pp, ps, slots, sp, sb, _stream(stream)), "attn8")
+        slots = probs.shape[1] if isinstance(probs, torch.Tensor) and probs.dim() == 4 else 1
+        pp = _dense("attn8", "probs", probs, _F16, (b, slots, rows, cap), dev)
+        ps = _dense("attn8", "pslot", pslot, _I32, (hq,), dev)
+    if scratch is None:
+        need = lib.mmz_attn8_scratch_bytes(b, rows, hq, h, cap, slots)
+        if need:
+            scratch = torch.empty(need, dtype=_U8, device=q.device)
+    sp, sb = _scratch("attn8", scratch, dev)
+    _check(lib.mmz_attn8(pq, s[0], s[1], s[2], *c, ln, po, o[0], o[1], o[2], b, rows, hq, h, cap, block, kind, causal,
+                         scale, pp, ps, slots, sp, sb, _stream(stream, dev)), "attn8")
 
 
-def _scratch(what, t):
-    return (None, 0) if t is None else (_dense(what, "scratch", t, torch.uint8, None), t.numel())
+def _scratch(what, t, dev):
+    return (None, 0) if t is None else (_dense(what, "scratch", t, _U8, None, dev), t.numel())
 
 
-def _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col):
-    """The pointers of the outputs, alternatives and their stride: [rows], or [rows][steps] with a column counter."""
+def _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col, dev):
+    """The arguments from sup to col: [rows] outputs, or [rows][steps] with a column counter."""
     if not isinstance(logp, torch.Tensor) or logp.dim() != (1 if col is None else 2):
         raise MmzError(f"{what}: logp is a tensor [rows], or [rows][steps] with col")
-    shape = (rows,) if col is None else (rows, logp.shape[1])
     ld = 1 if col is None else logp.shape[1]
-    got = [_dense(what, "target", target, _I32, shape), _dense(what, "logp", logp, _F32, shape)]
-    for name, t in (("entropy", entropy), ("lse", lse)):
-        got.append(None if t is None else _dense(what, name, t, _F32, shape))
+    shape = (rows,) if col is None else (rows, ld)
     one = top_id if top_id is not None else top_logp
     top = one.shape[-1] if isinstance(one, torch.Tensor) and one.dim() else 0
-    got.append(None if top_id is None else _dense(what, "top_id", top_id, _I32, shape + (top,)))
-    got.append(None if top_logp is None else _dense(what, "top_logp", top_logp, _F32, shape + (top,)))
-    ps = None if sup is None else _dense(what, "sup", sup, torch.uint8, (vocab,))
-    pc = None if col is None else _dense(what, "col", col, _I32, None)
-    return ps, got + [top, ld, pc]
+    return (_dense(what, "sup", sup, _U8, (vocab,), dev), _dense(what, "target", target, _I32, shape, dev),
+            _dense(what, "logp", logp, _F32, shape, dev), _dense(what, "entropy", entropy, _F32, shape, dev),
+            _dense(what, "lse", lse, _F32, shape, dev), _dense(what, "top_id", top_id, _I32, shape + (top,), dev),
+            _dense(what, "top_logp", top_logp, _F32, shape + (top,), dev), top, ld,
+            _dense(what, "col", col, _I32, None, dev))
 
 
 def token_logprobs(logits, target, logp, entropy=None, lse=None, top_id=None, top_logp=None, sup=None, col=None,
@@ -150,12 +172,15 @@ def token_logprobs(logits, target, logp, entropy=None, lse=None, top_id=None, to
     column col[0] is read and written. A target outside the vocabulary has logp 0."""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in (_F16, _F32) or logits.dim() != 2:
         raise MmzError("token_logprobs: logits is an fp16 or fp32 tensor [rows][vocab]")
+    dev = _device()
     rows, vocab = logits.shape
-    px = _tensor("token_logprobs", "logits", logits, logits.dtype, (rows, vocab))
-    ps, o = _outputs("token_logprobs", rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col)
-    ldx = logits.stride(0) if rows > 1 else vocab
-    _check(lib.mmz_token_logprobs(px, ldx, int(logits.dtype is _F32), rows, vocab, ps, *o, _stream(stream)),
-           "token_logprobs")
+    px = _strided("token_logprobs", "logits", logits, logits.dtype, logits.shape, dev)
+    s = logits.stride()
+    if s[1] != 1 and vocab > 1:
+        raise MmzError("token_logprobs: the last dimension of logits is dense")
+    o = _outputs("token_logprobs", rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col, dev)
+    _check(lib.mmz_token_logprobs(px, s[0] if rows > 1 else vocab, logits.dtype is _F32, rows, vocab, *o,
+                                  _stream(stream, dev)), "token_logprobs")
 
 
 def linear_logprobs_scratch_bytes(rows, vocab, d):
@@ -170,11 +195,15 @@ def linear_logprobs(x, emb, target, logp, entropy=None, lse=None, top_id=None, t
     what = "linear_logprobs"
     if not isinstance(x, torch.Tensor) or not isinstance(emb, torch.Tensor) or x.dim() != 2 or emb.dim() != 2:
         raise MmzError("linear_logprobs: x [rows][d] and emb [vocab][d] are tensors")
+    dev = _device()
     (rows, d), vocab = x.shape, emb.shape[0]
-    px, pe = _tensor(what, "x", x, _F16, (rows, d)), _dense(what, "emb", emb, _F16, (vocab, d))
-    ps, o = _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col)
+    px, pe = _strided(what, "x", x, _F16, x.shape, dev), _dense(what, "emb", emb, _F16, (vocab, d), dev)
+    s = x.stride()
+    if s[1] != 1:
+        raise MmzError("linear_logprobs: the last dimension of x is dense")
+    o = _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col, dev)
     if scratch is None:
-        scratch = torch.empty(lib.mmz_linear_logprobs_scratch_bytes(rows, vocab, d), dtype=torch.uint8, device=x.device)
-    sp, sb = _scratch(what, scratch)
-    ldx = x.stride(0) if rows > 1 else d
-    _check(lib.mmz_linear_logprobs(px, ldx, pe, rows, vocab, d, ps, *o, sp, sb, _stream(stream)), what)
+        scratch = torch.empty(lib.mmz_linear_logprobs_scratch_bytes(rows, vocab, d), dtype=_U8, device=x.device)
+    sp, sb = _scratch(what, scratch, dev)
+    _check(lib.mmz_linear_logprobs(px, s[0] if rows > 1 else d, pe, rows, vocab, d, *o, sp, sb, _stream(stream, dev)),
+           what)

@@ -218,12 +218,17 @@ ATTENDS = [  # b, rows, kv heads, group, cap, lens (None: cap), causal
     (2, 1, 1, 4, 200, [199, 65], False), (1, 5, 3, 1, 1500, None, False), (2, 7, 2, 2, 97, [97, 33], True),
     (3, 40, 2, 1, 70, [70, 40, 11], True), (1, 223, 1, 1, 448, None, True), (1, 33, 1, 3, 130, [129], False),
     (2, 3, 1, 1, 2, [1, 2], True), (1, 1, 1, 1, 20000, None, False), (4, 1, 20, 1, 448, [17, 448, 15, 16], False),
-    (2, 1, 3, 1, 33, [-5, 1000000], False), (1, 9, 1, 8, 300, [300], True), (150, 1, 8, 1, 100, None, False)]
+    (2, 1, 3, 1, 33, [-5, 1000000], False), (1, 9, 1, 8, 300, [300], True), (150, 1, 8, 1, 100, None, False),
+    # many chunks: an equal share of them to each warp, whatever the lengths
+    (32, 1, 20, 1, 448, [14 * i for i in range(32)], False), (2, 1, 4, 2, 30000, [30000, 17], False),
+    (40, 3, 16, 1, 400, [(37 * i) % 401 for i in range(40)], True), (4, 2, 8, 4, 8000, [8000, 1, 0, 7999], True),
+    (64, 1, 16, 1, 300, [i % 3 * 32 for i in range(64)], False), (60, 1, 20, 1, 200, [0] * 60, False),
+    (100, 1, 12, 1, 257, [200 + i % 58 for i in range(100)], False), (1, 8, 1, 1, 230000, None, True)]
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("block", [16, 32, 64, 128])
-@pytest.mark.parametrize("case", ATTENDS)
+@pytest.mark.parametrize("case", ATTENDS, ids=lambda c: "x".join(map(str, c[:5])))
 def test_attention(cuda, kind, block, case):
     b, rows, h, group, cap, lens, causal = case
     gen = torch.Generator().manual_seed(cap + block)

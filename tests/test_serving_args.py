@@ -51,7 +51,7 @@ def attend(q=A, qs=(64, 64, 64), k8=A, cs=(6400, 6400), ks=A, out=A, os=(64, 64,
     (dict(probs=A + 8, pslot=A, slots=1), b"aligned"), (dict(qs=(64, 64, 63)), b"strides"),
     (dict(os=(64, 4, 64)), b"strides"), (dict(cs=(6401, 6400)), b"strides"), (dict(cap=0x7fffffff), b"cap"),
     (dict(probs=A, pslot=A, slots=1), b"scratch"), (dict(probs=A, pslot=A, slots=1, scratch=A + 8, sb=1 << 20), b"scratch"),
-    (dict(probs=A, pslot=A, slots=1, scratch=A, sb=8), b"scratch"), (dict(cap=100000), b"scratch"),
+    (dict(probs=A, pslot=A, slots=1, scratch=A, sb=4), b"scratch"), (dict(cap=100000), b"scratch"),
     (dict(batch=1 << 20, hq=1 << 12, hkv=1 << 12), b"2^31"), (dict(rows=0x7fffffff), b"rows")])
 def test_attention_refuses(bad, word):
     assert attend(**bad) == -1
