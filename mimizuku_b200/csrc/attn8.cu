@@ -5,7 +5,7 @@
 // and the probabilities of chosen heads as fp16. Sums and softmax statistics in fp32; only the outputs are rounded.
 //
 // The query heads and rows that share a key head are one block of rows: up to 8 (a decoding step, hypotheses of one
-// clip, grouped heads) or tiles of 32 (prompts). A warp takes chunks of 64 positions, keys and values by bulk copies
+// clip, grouped heads) or tiles of 16 (prompts). A warp takes chunks of 64 positions, keys and values by bulk copies
 // into a ring of its own, and works in registers from there:
 //   * every code (int8 or e4m3) is a number of fp16, so the products run exactly on the tensor cores (m16n8k16, fp32
 //     sums): S^T = K q^T with the 16 positions as M and the 8 rows as N, then O^T = V^T P^T. The contraction indices are
@@ -19,7 +19,7 @@
 // Two ways through the cache (plan() chooses):
 //   flat     many chunks, up to 8 rows: a fixed number of warps, each with an equal share of all sequences' and heads'
 //            chunks in a row, whatever the lengths; a pair's parts on several warps join in a second kernel
-//   cluster  few chunks, or more rows: a CTA to a (pair, row block), its warps along the positions (up to 32 rows) or
+//   cluster  few chunks, or more rows: a CTA to a (pair, row block), its warps along the positions (up to 16 rows) or
 //            along the rows; CTAs of a cluster split the sequence and join through distributed shared memory, and where
 //            one cluster is too little, clusters through scratch and a second kernel
 #include "attn8.h"
@@ -36,7 +36,7 @@ constexpr int KB = CH * HD;     // bytes of a chunk's keys (and of its values)
 constexpr int REC = HD + 2;     // a row's partial result: 64 sums, maximum, sum of p
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float PSHIFT = 10.f;  // p <= 2^10
-constexpr long FLAT_FROM = 2;   // chunks to a warp from which on the flat way is taken
+constexpr long FLAT_FROM = 4;   // chunks to a warp from which on the flat way is taken
 
 struct Smem {
     uint8_t ring[WARPS][STG][2][KB];
@@ -69,12 +69,10 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w, bool hi) {
 // quad are positions t, t + 4, t + 8, t + 12
 __device__ __forceinline__ int place(int r) { return (r & 8) | ((r & 1) << 2) | ((r & 6) >> 1); }
 
-// scores of 16 positions (keys at k, 64 bytes a row) against 8 rows per column tile; lane (g, t) receives position
-// place(g) (and + 8) for rows 2t and 2t + 1
+// scores of 16 positions against 8 rows per column tile, from 16 bytes of the keys place(g) and place(g) + 8 (those from
+// byte 16 t on); lane (g, t) receives these positions for rows 2t and 2t + 1
 template <int KIND, int NTL>
-__device__ __forceinline__ void scores16(const uint8_t* k, int lane, const uint32_t (&q)[NTL][8], float (&s)[NTL][4]) {
-    const uint8_t* p = k + place(lane >> 2) * HD + (lane & 3) * 16;
-    const uint4 lo = *reinterpret_cast<const uint4*>(p), hi = *reinterpret_cast<const uint4*>(p + 8 * HD);
+__device__ __forceinline__ void scores16(const uint4& lo, const uint4& hi, const uint32_t (&q)[NTL][8], float (&s)[NTL][4]) {
     const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
     for (int n = 0; n < NTL; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -106,15 +104,17 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) {  // 0x80 in the byte
     return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
-// A warp's rows and their running results. MODE 0: up to 4 rows, columns 4-7 repeat columns 0-3; 1: up to 8; 4: up to 32.
+// A warp's rows and their running results. MODE 0: up to 4 rows, columns 4-7 repeat columns 0-3; 1: up to 8; 2: up to 16.
 // Lane (g, t) of the warp (g = lane / 4, t = lane % 4) holds columns 8 n + 2 t + e of dimensions 8 g .. 8 g + 7.
 template <int KIND, int MODE>
 struct Rows {
-    static constexpr int NTL = MODE == 4 ? 4 : 1;        // column tiles of 8
+    static constexpr int NTL = MODE == 2 ? 2 : 1;        // column tiles of 8
     static constexpr int SUB = NTL == 1 ? 64 : 32;       // positions whose scores are in registers at a time
     static constexpr int NJ = SUB / 16;
     uint32_t q[NTL][8];
     float m[NTL][2], l[NTL][2], o[4][NTL][4];  // o[i][n][e + 2 k]: dimension 8 g + 2 i + k, column 8 n + 2 t + e
+    float* raw[NTL][2];                        // where the scores of the lane's columns go, null: nowhere
+    bool any;                                  // some lane of the warp has a raw
 
     // the row of column c of tile n
     static __device__ __forceinline__ int row(int n, int c) { return MODE == 0 ? c & 3 : 8 * n + c; }
@@ -127,6 +127,23 @@ struct Rows {
             else
                 for (int i = 0; i < 8; i++) q[n][i] = 0;
         }
+    }
+    // the rows' places in raw scores [batch][slots][rows][cap]
+    __device__ __forceinline__ void record(const Attn8& a, float* to, long b, int hk, int group, int r0, int R, int lane) {
+        bool have_one = false;
+#pragma unroll
+        for (int n = 0; n < NTL; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int r = r0 + 8 * n + 2 * (lane & 3) + e;
+                raw[n][e] = nullptr;
+                if (!to || r >= R || !have(lane & 3)) continue;
+                const int slot = a.pslot[hk * group + r % group];
+                if (slot < 0 || slot >= a.slots) continue;
+                raw[n][e] = to + ((b * a.slots + slot) * a.rows + r / group) * (long)a.cap;
+                have_one = true;
+            }
+        any = to && __any_sync(0xffffffff, have_one);
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -177,11 +194,11 @@ struct Rows {
         }
     }
     // One chunk: codes at ck, cv (shared memory), positions base .. base + 63 of which those below `most` exist. sc:
-    // lanes 0-3 the key scales (times scale log2 e) of the four tiles of 16 positions, lanes 4-7 the value scales. lim:
-    // what the lane's columns see; whole: every row sees the whole chunk.
+    // chunk_scale's; scale: the scores' factor. lim: what the lane's columns see; whole: every row sees the whole chunk.
     __device__ __forceinline__ void chunk(const uint8_t* ck, uint8_t* cv, int base, int most, bool whole, float sc,
-                                          const int (&lim)[NTL][2], int block, int lane) {
+                                          float scale, const int (&lim)[NTL][2], int block, int lane) {
         const int g = lane >> 2, t = lane & 3;
+        if (lane < 4) sc *= scale * LOG2E;
         // the sequence's last chunk: the rows that were not copied hold what the ring held. Their weights are 0, but a
         // NaN times 0 would not be
         if (base + CH > most) {
@@ -196,7 +213,8 @@ struct Rows {
             float s[NJ][NTL][4];
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                scores16<KIND, NTL>(ck + (sub * SUB + 16 * j) * HD, lane, q, s[j]);
+                const uint8_t* k = ck + (sub * SUB + 16 * j + place(g)) * HD + 16 * t;
+                scores16<KIND, NTL>(*reinterpret_cast<const uint4*>(k), *reinterpret_cast<const uint4*>(k + 8 * HD), q, s[j]);
                 const float f = __shfl_sync(0xffffffff, sc, sub * NJ + j);
 #pragma unroll
                 for (int n = 0; n < NTL; n++)
@@ -213,6 +231,17 @@ struct Rows {
                         for (int e = 0; e < 4; e++)
                             if (p + (e >> 1) * 8 >= lim[n][e & 1]) s[j][n][e] = -INFINITY;
                 }
+            }
+            if (any) {
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int n = 0; n < NTL; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int p = sb + 16 * j + place(g) + 8 * (e >> 1);
+                            if (raw[n][e & 1] && p < lim[n][e & 1]) raw[n][e & 1][p] = s[j][n][e];
+                        }
             }
             // running maximum, p and its sum
             uint32_t ph[NJ][NTL][2], pl[NJ][NTL][2];
@@ -342,12 +371,12 @@ struct Rows {
     }
 };
 
-// lanes 0-3: the key scales (times scale log2 e) of a chunk's four tiles of 16 positions, lanes 4-7 the value scales
-__device__ __forceinline__ float chunk_scale(const float* ks, const float* vs, int c, int most, int shift, float scale,
-                                             int lane) {
+// lanes 0-3: the key scales of a chunk's four tiles of 16 positions, lanes 4-7 the value scales. A load whose result is
+// first used with the chunk, so that it is never waited for on the way there
+__device__ __forceinline__ float chunk_scale(const float* ks, const float* vs, int c, int most, int shift, int lane) {
     if (lane >= 8) return 0.f;
     const int j = min(c * CH + 16 * (lane & 3), most - 1) >> shift;
-    return lane < 4 ? ks[j] * (scale * LOG2E) : vs[j];
+    return lane < 4 ? ks[j] : vs[j];
 }
 
 // How a cluster call is laid out along its CTAs (plan() below).
@@ -364,11 +393,11 @@ using namespace a8;
 // grid: cluster rank fastest, then cluster along the sequence, row block, (sequence, key head); cluster of cs CTAs.
 // nclus 1: the cluster's rows go to out (and their statistics to stats, if not null); else to part
 template <int KIND, int MODE>
-__global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part, float2* stats, unsigned* status,
+__global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part, float2* stats, float* raws, unsigned* status,
                                                    unsigned long long limit_ns) {
     constexpr int NTL = Rows<KIND, MODE>::NTL, RT = 8 * NTL;
-    extern __shared__ __align__(128) uint8_t raw[];
-    Smem& sm = *reinterpret_cast<Smem*>(raw);
+    extern __shared__ __align__(128) uint8_t smem[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int cs = lay.cs, wstep = lay.wrows ? 1 : WARPS;
     unsigned x = blockIdx.x;
@@ -394,6 +423,7 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part
 
     Rows<KIND, MODE> w;
     w.queries(a, b, hk, group, r0, R, lane);
+    w.record(a, raws, b, hk, group, r0, R, lane);
     w.clear();
     const int L = a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap;
     // what row r sees; the warp's last row sees the most
@@ -416,7 +446,7 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part
         bulk_g2s(sm.ring[warp][st][0], k8 + (long)c * KB, bytes, &full[st]);
         bulk_g2s(sm.ring[warp][st][1], v8 + (long)c * KB, bytes, &full[st]);
     };
-    auto scale_of = [&](int c) { return c < c1 ? chunk_scale(ks, vs, c, most, shift, a.scale, lane) : 0.f; };
+    auto scale_of = [&](int c) { return c < c1 ? chunk_scale(ks, vs, c, most, shift, lane) : 0.f; };
     int at = cw;
     if (lane == 0)
         for (int i = 0; i < STG && cw + i * wstep < c1; i++) issue(cw + i * wstep, i);
@@ -435,7 +465,8 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part
         if (!ok) break;
         const float sc = sc_next;
         sc_next = scale_of(c + wstep);
-        w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], c * CH, most, c * CH + CH <= least, sc, lim, a.block, lane);
+        w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], c * CH, most, c * CH + CH <= least, sc, a.scale, lim,
+                a.block, lane);
         __syncwarp();
         if (lane == 0 && c + STG * wstep < c1) issue(c + STG * wstep, st);
         at = c + wstep;
@@ -455,7 +486,7 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part
     // Each warp sends its rows' statistics to every CTA of the cluster and its sums to the CTA that joins those
     // dimensions (the lane's 8 have one owner): stores, and one barrier, instead of loads that are waited for.
     const int src = rank * wstep + (lay.wrows ? 0 : warp), share = HD / cs;
-    float2* ms = reinterpret_cast<float2*>(raw + sizeof(Smem));
+    float2* ms = reinterpret_cast<float2*>(smem + sizeof(Smem));
     float* sums = reinterpret_cast<float*>(ms + lay.block * nsrc + (lay.block * nsrc & 1));
     if (cs > 1) cluster_wait();
 #pragma unroll
@@ -539,30 +570,47 @@ struct Flat {
         all = __reduce_add_sync(0xffffffff, all) * kv_heads;
         upto = __reduce_add_sync(0xffffffff, upto) * kv_heads;
     }
-    // whole warp: the sequence that chunk f of the whole row lies in; f becomes its place among that sequence's
-    __device__ __forceinline__ int find(unsigned& f, int lane) const {
+    // whole warp: the chunks that warp w of W has, and where they start: sequence b, and f its place among that
+    // sequence's. One load per lane for up to 32 sequences
+    __device__ __forceinline__ unsigned find(unsigned w, unsigned W, int lane, int& b, int& len, unsigned& f) const {
+        unsigned upto, all, n;
         if (!lens) {
-            const unsigned per = chunks(0) * kv_heads, b = f / per;
+            before(0, lane, upto, all);
+            const Share share(all, W);
+            const unsigned per = chunks(0) * kv_heads;
+            f = share.first(w);
+            b = f / per, len = cap;
             f -= b * per;
-            return (int)b;
+            return share.count(w);
         }
-        for (int i = 0; i < batch; i += 32) {
-            const unsigned mine = chunks(i + lane) * kv_heads;
+        all = 0;
+        if (batch > 32) before(0, lane, upto, all);
+        for (int i = 0;; i += 32) {
+            const int l = i + lane < batch ? this->len(i + lane) : 0;
+            const unsigned mine = (unsigned)(l + CH - 1) / CH * kv_heads;
             unsigned up = mine;  // through this lane's sequence
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const unsigned x = __shfl_up_sync(0xffffffff, up, o);
                 if (lane >= o) up += x;
             }
+            if (i == 0) {
+                if (batch <= 32) all = __shfl_sync(0xffffffff, up, 31);
+                const Share share(all, W);
+                n = share.count(w);
+                if (n == 0) return 0;
+                f = share.first(w);
+            }
             const unsigned hit = __ballot_sync(0xffffffff, up > f);
             if (hit) {
                 const int k = __ffs(hit) - 1;
                 f -= __shfl_sync(0xffffffff, up - mine, k);
-                return i + k;
+                b = i + k, len = __shfl_sync(0xffffffff, l, k);
+                return n;
             }
             f -= __shfl_sync(0xffffffff, up, 31);
+            if (i + 32 >= batch) return 0;  // not reached: f is below the total
         }
-        return batch - 1;  // not reached: f is below the total
     }
 };
 // where a warp stands in the row of chunks
@@ -579,11 +627,12 @@ struct Place {
 };
 }  // namespace a8
 
+// (at most 128 registers, so that the next kernel's blocks find room beside three CTAs)
 template <int KIND, int MODE>
-__global__ void __launch_bounds__(NT) attn8_flat_kernel(Attn8 a, float* rec, float2* stats, unsigned* status,
+__global__ void __launch_bounds__(NT, 4) attn8_flat_kernel(Attn8 a, float* rec, float2* stats, float* raws, unsigned* status,
                                                         unsigned long long limit_ns) {
-    extern __shared__ __align__(128) uint8_t raw[];
-    Smem& sm = *reinterpret_cast<Smem*>(raw);
+    extern __shared__ __align__(128) uint8_t smem[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = a.q_heads / a.kv_heads, R = a.rows * group;
     const Flat flat{a.lens, a.cap, a.batch, a.kv_heads};
@@ -596,20 +645,13 @@ __global__ void __launch_bounds__(NT) attn8_flat_kernel(Attn8 a, float* rec, flo
     griddep_wait();
     griddep_launch_dependents();
     const unsigned me = blockIdx.x * WARPS + warp;
-    unsigned upto, all;
-    flat.before(0, lane, upto, all);
-    const Share share(all, gridDim.x * WARPS);
-    const unsigned n = share.count(me);
-    if (n == 0) return;
     Place cur;
-    {
-        unsigned f = share.first(me);
-        cur.b = flat.find(f, lane);
-        cur.len = flat.len(cur.b);
-        cur.nch = (cur.len + CH - 1) / CH;
-        cur.hk = f / (unsigned)cur.nch;
-        cur.c = f % (unsigned)cur.nch;
-    }
+    unsigned f;
+    const unsigned n = flat.find(me, gridDim.x * WARPS, lane, cur.b, cur.len, f);
+    if (n == 0) return;
+    cur.nch = (cur.len + CH - 1) / CH;
+    cur.hk = f / (unsigned)cur.nch;
+    cur.c = f % (unsigned)cur.nch;
     Place ahead = cur;
     const int shift = 31 - __clz(a.block);
     float sc[STG];  // the scales of the chunks in the ring, the next one first
@@ -623,7 +665,7 @@ __global__ void __launch_bounds__(NT) attn8_flat_kernel(Attn8 a, float* rec, flo
             bulk_g2s(sm.ring[warp][st][1], a.v8 + at, bytes, &full[st]);
         }
         const long sat = (long)ahead.b * a.s_seq + ahead.hk * a.s_head;
-        const float x = chunk_scale(a.ks + sat, a.vs + sat, ahead.c, ahead.len, shift, a.scale, lane);
+        const float x = chunk_scale(a.ks + sat, a.vs + sat, ahead.c, ahead.len, shift, lane);
         sent++;
         if (sent < n) ahead.next(flat);
         return x;
@@ -635,6 +677,7 @@ __global__ void __launch_bounds__(NT) attn8_flat_kernel(Attn8 a, float* rec, flo
     int lim[1][2], from = cur.c;  // the segment's first chunk
     auto begin = [&]() {
         w.queries(a, cur.b, cur.hk, group, 0, R, lane);
+        w.record(a, raws, cur.b, cur.hk, group, 0, R, lane);
         w.clear();
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -651,7 +694,8 @@ __global__ void __launch_bounds__(NT) attn8_flat_kernel(Attn8 a, float* rec, flo
         ok = __all_sync(0xffffffff, mbar_wait(&full[st], (it / STG) & 1, &sm.abort, limit_ns, status, K_ATTN8, 2));
         if (!ok) break;
         const int base = cur.c * CH, least = a.causal ? max(0, cur.len - a.rows + 1) : cur.len;
-        w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], base, cur.len, base + CH <= least, sc[0], lim, a.block, lane);
+        w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], base, cur.len, base + CH <= least, sc[0], a.scale, lim,
+                a.block, lane);
         if (base + CH > cur.len) fence_proxy_async_smem();  // zeros written behind the end, before the next copy
         __syncwarp();
 #pragma unroll
@@ -743,55 +787,64 @@ __device__ __forceinline__ void join_parts(const Parts& p, int first, int stride
         S = S * f + s;
         if constexpr (SUMS) {
             O.x *= f, O.y *= f;
+            const unsigned have = __ballot_sync(0xffffffff, y.x != -INFINITY);  // a part whose row saw something
             const int n = min(32, p.n - k0);
-#pragma unroll 8
-            for (int j = 0; j < n; j++) {
-                const float gj = __shfl_sync(0xffffffff, g, j);
-                const bool have = __shfl_sync(0xffffffff, y.x, j) != -INFINITY;
-                const float2 x = have ? *reinterpret_cast<const float2*>(p.at(k0 + j) + p.so + 2 * lane) : make_float2(0.f, 0.f);
-                O.x += gj * x.x;
-                O.y += gj * x.y;
+            for (int j0 = 0; j0 < n; j0 += 16) {  // 16 loads at once
+                float2 x[16];
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    x[j] = make_float2(0.f, 0.f);
+                    if (have >> (j0 + j) & 1) x[j] = *reinterpret_cast<const float2*>(p.at(k0 + j0 + j) + p.so + 2 * lane);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const float gj = __shfl_sync(0xffffffff, g, j0 + j);
+                    O.x += gj * x[j].x;
+                    O.y += gj * x[j].y;
+                }
             }
         }
     }
 }
 }  // namespace a8
 
-// Blocks 0 .. jblocks - 1: a row each, its parts joined (the warps share them) and written; the others: the
-// probabilities of 8 rows and 256 positions of a (sequence, slot), p = 2^(s - M) / S with the scores computed again (the
-// same products in the same order). All but the parts and statistics is read before the wait for the main kernel, which
-// lets this one start once it has waited for what came before.
-template <int KIND>
-__global__ void __launch_bounds__(NT) attn8_post_kernel(Attn8 a, unsigned jblocks, int nclus, unsigned W,
-                                                        const float* part, const float2* stats) {
-    __shared__ float red[WARPS][REC];
-    __shared__ float2 rowms[8];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// Blocks 0 .. jblocks - 1: rows whose parts are joined and written, one to a block (jrows 1: the warps share its parts)
+// or one to a warp (where a row has a few parts). The others: the probabilities of a (sequence, slot, row),
+// p = 2^(s - M) / S from the scores that the main kernel left. This kernel starts once the main one has waited for what
+// came before, and finds out where the parts lie meanwhile.
+__global__ void __launch_bounds__(512) attn8_post_kernel(Attn8 a, unsigned jblocks, int jrows, int nclus, unsigned W,
+                                                         const float* part, const float2* stats, const float* raws) {
+    __shared__ float red[16][REC];
+    __shared__ float2 rowms;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
     const int group = a.q_heads / a.kv_heads, R = a.rows * group;
+    Parts p;
+    p.n = 0;
     if (blockIdx.x < jblocks) {
-        const int r = blockIdx.x % R;
-        const unsigned pair = blockIdx.x / R;
-        const int hk = pair % a.kv_heads, b = pair / a.kv_heads;
-        const Parts p = parts_of(a, part, nclus, W, b, hk, r, R, lane);
+        const unsigned row = jrows == 1 ? blockIdx.x : blockIdx.x * nw + warp, pair = row / R;
+        const int r = row % R, hk = pair % a.kv_heads, b = pair / a.kv_heads;
+        if (b < a.batch) p = parts_of(a, part, nclus, W, b, hk, r, R, lane);
         griddep_wait();
         griddep_launch_dependents();
         if (p.n == 0) return;
         float M, S;
         float2 O;
-        join_parts<true>(p, 32 * warp, 32 * WARPS, lane, M, S, O);
-        red[warp][2 * lane] = O.x;
-        red[warp][2 * lane + 1] = O.y;
-        if (lane == 0) red[warp][HD] = M, red[warp][HD + 1] = S;
-        __syncthreads();
-        if (warp) return;
-        float m = M;
-        for (int w = 1; w < WARPS; w++) m = fmaxf(m, red[w][HD]);
-        S = 0.f, O = make_float2(0.f, 0.f);
-        for (int w = 0; w < WARPS; w++) {
-            const float f = weight(red[w][HD], m);
-            S += f * red[w][HD + 1];
-            O.x += f * red[w][2 * lane];
-            O.y += f * red[w][2 * lane + 1];
+        join_parts<true>(p, jrows == 1 ? 32 * warp : 0, jrows == 1 ? 32 * nw : 32, lane, M, S, O);
+        if (jrows == 1) {
+            red[warp][2 * lane] = O.x;
+            red[warp][2 * lane + 1] = O.y;
+            if (lane == 0) red[warp][HD] = M, red[warp][HD + 1] = S;
+            __syncthreads();
+            if (warp) return;
+            float m = M;
+            for (int w = 1; w < nw; w++) m = fmaxf(m, red[w][HD]);
+            S = 0.f, O = make_float2(0.f, 0.f);
+            for (int w = 0; w < nw; w++) {
+                const float f = weight(red[w][HD], m);
+                S += f * red[w][HD + 1];
+                O.x += f * red[w][2 * lane];
+                O.y += f * red[w][2 * lane + 1];
+            }
         }
         const float inv = inverse(S);
         const int h = hk * group + r % group;
@@ -799,82 +852,42 @@ __global__ void __launch_bounds__(NT) attn8_post_kernel(Attn8 a, unsigned jblock
             __floats2half2_rn(O.x * inv, O.y * inv);
         return;
     }
-    const int pt = (a.cap + 255) / 256, nrt = (a.rows + 7) / 8;
     unsigned x = blockIdx.x - jblocks;
-    const int pblk = x % pt;
-    x /= pt;
-    const int rtile = x % nrt;
-    x /= nrt;
-    const int slot = x % a.slots;
-    const long b = x / a.slots;
+    const int i = x % a.rows;
+    x /= a.rows;
+    const int slot = x % a.slots, b = x / a.slots;
     int h = 0x7fffffff;
-    for (int i = lane; i < a.q_heads; i += 32)
-        if (h == 0x7fffffff && a.pslot[i] == slot) h = i;
+    for (int k = lane; k < a.q_heads; k += 32)
+        if (h == 0x7fffffff && a.pslot[k] == slot) h = k;
     h = __reduce_min_sync(0xffffffff, h);
     const bool live = h < a.q_heads;  // a slot that no head has is left as it is
-    const int hk = live ? h / group : 0, r0 = rtile * 8;
-    const int L = a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap;
-    const uint8_t* k8 = a.k8 + b * a.c_seq + hk * a.c_head;
-    const float* ks = a.ks + b * a.s_seq + hk * a.s_head;
-    uint32_t q[1][8];
-    if (live && r0 + g < a.rows) load_q(a.q + b * a.q_seq + (r0 + g) * a.q_row + h * a.q_head, t, q[0]);
-    else
-        for (int i = 0; i < 8; i++) q[0][i] = 0;
-    const int last = a.causal ? max(0, L - a.rows + min(r0 + 8, a.rows)) : L;  // positions that some row sees
-    float s[4][1][4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int base = pblk * 256 + warp * 64 + j * 16;
-        s[j][0][0] = s[j][0][1] = s[j][0][2] = s[j][0][3] = 0.f;
-        if (live && base + 16 <= last) {
-            scores16<KIND, 1>(k8 + (long)base * HD, lane, q, s[j]);
-        } else if (live && base < last) {  // rows past the sequence's end are not read: its last one instead
-            const int p0 = min(base + place(g), last - 1), p1 = min(base + place(g) + 8, last - 1);
-            const uint4 lo = *reinterpret_cast<const uint4*>(k8 + (long)p0 * HD + 16 * t);
-            const uint4 hi = *reinterpret_cast<const uint4*>(k8 + (long)p1 * HD + 16 * t);
-            const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t f[4] = {codes2<KIND>(wl[e], false), codes2<KIND>(wh[e], false), codes2<KIND>(wl[e], true),
-                                       codes2<KIND>(wh[e], true)};
-                mma(s[j][0], f, q[0][2 * e], q[0][2 * e + 1]);
-            }
-        }
-        const float f = live && base < last ? ks[base / a.block] * (a.scale * LOG2E) : 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[j][0][e] *= f;
-    }
-    const long prow = (b * a.kv_heads + hk) * R + h % group;  // the head's row 0; row i lies i * group on
-    const int i0 = r0 + 2 * warp;                             // the warp's two rows
-    Parts p[2];
-    for (int e = 0; e < 2; e++)
-        if (live && i0 + e < a.rows) p[e] = parts_of(a, part, nclus, W, (int)b, hk, (i0 + e) * group + h % group, R, lane);
+    const int hk = live ? h / group : 0, r = i * group + (live ? h % group : 0);
+    if (live && warp == 0) p = parts_of(a, part, nclus, W, b, hk, r, R, lane);
+    const int L = a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap, lim = a.causal ? max(0, L - a.rows + i + 1) : L;
     griddep_wait();
     griddep_launch_dependents();
     if (!live) return;
-    for (int e = 0; e < 2; e++)
-        if (i0 + e < a.rows) {
-            float M, S;
-            float2 O;
-            if (p[e].n > 0) {
-                join_parts<false>(p[e], 0, 32, lane, M, S, O);
-                if (lane == 0) rowms[2 * warp + e] = make_float2(M, inverse(S));
-            } else if (lane == 0) {
-                rowms[2 * warp + e] = p[e].n == 0 ? stats[prow + (long)(i0 + e) * group] : make_float2(0.f, 0.f);
-            }
-        }
+    if (warp == 0) {
+        float M = 0.f, S = 0.f;
+        float2 O;
+        if (p.n > 0) join_parts<false>(p, 0, 32, lane, M, S, O);
+        if (lane == 0)
+            rowms = p.n == 0 ? stats[((long)b * a.kv_heads + hk) * R + r] : make_float2(M, inverse(S));
+    }
     __syncthreads();
+    const float off = rowms.x - PSHIFT, inv = rowms.y;
+    const long at = (((long)b * a.slots + slot) * a.rows + i) * a.cap;
+    for (int j0 = threadIdx.x; j0 < a.cap; j0 += 8 * blockDim.x) {  // 8 loads at once
+        float v[8];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int base = pblk * 256 + warp * 64 + j * 16;
+        for (int k = 0; k < 8; k++) {
+            const int j = j0 + k * blockDim.x;
+            v[k] = j < lim ? raws[at + j] : -INFINITY;
+        }
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int pos = base + place(g) + 8 * (e >> 1), i = r0 + 2 * t + (e & 1);
-            if (pos >= a.cap || i >= a.rows) continue;
-            const float2 ms = rowms[2 * t + (e & 1)];
-            const int lim = a.causal ? max(0, L - a.rows + i + 1) : L;
-            const float v = pos < lim ? ex2_approx(s[j][0][e] - (ms.x - PSHIFT)) * ms.y : 0.f;
-            a.probs[((b * a.slots + slot) * a.rows + i) * (long)a.cap + pos] = __float2half_rn(v);
+        for (int k = 0; k < 8; k++) {
+            const int j = j0 + k * blockDim.x;
+            if (j < a.cap) a.probs[at + j] = __float2half_rn(j < lim ? ex2_approx(v[k] - off) * inv : 0.f);
         }
     }
 }
@@ -886,14 +899,15 @@ struct Plan {
     int mode;   // Rows' MODE
     bool flat;
     Lay lay;
-    size_t smem, part, stats;
+    size_t smem, part, stats, raws;
 };
 Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     Plan p;
     const long R = (long)rows * (q_heads / kv_heads), pairs = (long)batch * kv_heads, chunks = ((long)cap + CH - 1) / CH;
-    const long rt = R <= 8 ? 8 : 32;
-    p.mode = R <= 4 ? 0 : R <= 8 ? 1 : 4;
-    p.stats = slots > 0 ? (size_t)pairs * R * 8 : 0;
+    const long rt = R <= 8 ? 8 : 16;
+    p.mode = R <= 4 ? 0 : R <= 8 ? 1 : 2;
+    p.stats = slots > 0 ? ((size_t)pairs * R * 8 + 15) & ~(size_t)15 : 0;
+    p.raws = (size_t)batch * slots * rows * cap * 4;
     p.flat = R <= 8 && pairs * chunks >= FLAT_FROM * SLOTS * WARPS && pairs * chunks < 0x7fffffffl;
     if (p.flat) {
         p.lay = {1, 1, 0, 0, 1};
@@ -901,17 +915,17 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
         p.part = (size_t)SLOTS * WARPS * 2 * RECF * 4;
         return p;
     }
-    p.lay.wrows = R > 32;
+    p.lay.wrows = R > 16;
     const long block = p.lay.wrows ? WARPS * rt : rt;
     p.lay.block = (int)(R < block ? R : block);
     p.lay.tiles = (int)((R + block - 1) / block);
-    // CTAs for every SM, and a chunk at least to each warp
+    // splits of the sequence: no more CTAs than the GPU holds at once, and a chunk at least to each warp
     const long units = pairs * p.lay.tiles, top = p.lay.wrows ? chunks : (chunks + WARPS - 1) / WARPS;
-    long s = (SLOTS + units - 1) / units;
-    if (s > top) s = top;
-    const int cs = s <= 1 ? 1 : s <= 2 ? 2 : s <= 4 ? 4 : 8;
+    long s = SLOTS / units;
+    s = s < 1 ? 1 : s > top ? top : s;
+    const int cs = s < 2 ? 1 : s < 4 ? 2 : s < 8 ? 4 : 8;
     p.lay.cs = cs;
-    p.lay.nclus = (int)((s + cs - 1) / cs);
+    p.lay.nclus = (int)(s / cs);
     const size_t n = (size_t)p.lay.block * cs * (p.lay.wrows ? 1 : WARPS);  // (row, source) pairs
     p.smem = sizeof(Smem) + (n + (n & 1)) * 8 + n * (HD / cs) * 4;
     p.part = p.lay.nclus > 1 ? ((size_t)pairs * R * p.lay.nclus * REC * 4 + 15) & ~(size_t)15 : 0;
@@ -919,10 +933,10 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
 }
 
 template <int KIND, int MODE>
-int launch_main(const Attn8& a, const Plan& p, float* part, float2* stats, DevCtx& dc, cudaStream_t st) {
-    if constexpr (MODE != 4) {
+int launch_main(const Attn8& a, const Plan& p, float* part, float2* stats, float* raws, DevCtx& dc, cudaStream_t st) {
+    if constexpr (MODE != 2) {
         if (p.flat)
-            return check_pdl(launch_pdl(attn8_flat_kernel<KIND, MODE>, dim3(SLOTS), dim3(NT), p.smem, st, a, part, stats,
+            return check_pdl(launch_pdl(attn8_flat_kernel<KIND, MODE>, dim3(SLOTS), dim3(NT), p.smem, st, a, part, stats, raws,
                                         dc.status, dc.limit_ns),
                              "attn8");
     }
@@ -939,21 +953,21 @@ int launch_main(const Attn8& a, const Plan& p, float* part, float2* stats, DevCt
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return check_pdl(cudaLaunchKernelEx(&cfg, attn8_kernel<KIND, MODE>, a, p.lay, part, stats, dc.status, dc.limit_ns),
+    return check_pdl(cudaLaunchKernelEx(&cfg, attn8_kernel<KIND, MODE>, a, p.lay, part, stats, raws, dc.status, dc.limit_ns),
                      "attn8");
 }
 
 template <int KIND>
-int launch_mode(const Attn8& a, const Plan& p, float* part, float2* stats, DevCtx& dc, cudaStream_t st) {
-    return p.mode == 0   ? launch_main<KIND, 0>(a, p, part, stats, dc, st)
-           : p.mode == 1 ? launch_main<KIND, 1>(a, p, part, stats, dc, st)
-                         : launch_main<KIND, 4>(a, p, part, stats, dc, st);
+int launch_mode(const Attn8& a, const Plan& p, float* part, float2* stats, float* raws, DevCtx& dc, cudaStream_t st) {
+    return p.mode == 0   ? launch_main<KIND, 0>(a, p, part, stats, raws, dc, st)
+           : p.mode == 1 ? launch_main<KIND, 1>(a, p, part, stats, raws, dc, st)
+                         : launch_main<KIND, 2>(a, p, part, stats, raws, dc, st);
 }
 }  // namespace
 
 size_t attn8_scratch_bytes(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     const Plan p = plan(batch, rows, q_heads, kv_heads, cap, slots);
-    return p.part + p.stats;
+    return p.part + p.stats + p.raws;
 }
 
 int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, cudaStream_t st) {
@@ -975,33 +989,47 @@ int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, 
     if ((long)a.rows * (a.q_heads / a.kv_heads) > 0x7fffff00l) return fail("attn8: too many rows in one call");
     const Plan p = plan(a.batch, a.rows, a.q_heads, a.kv_heads, a.cap, slots);
     const long grid = (long)a.batch * a.kv_heads * p.lay.tiles * p.lay.nclus * p.lay.cs;
-    const long jblocks = p.flat || p.lay.nclus > 1 ? (long)a.batch * a.rows * a.q_heads : 0;  // rows with parts
-    const long post = jblocks + (long)a.batch * slots * ((a.rows + 7) / 8) * ((a.cap + 255) / 256);
+    // rows with parts: one to a warp, or where a row has more than 32 parts or so one to a block
+    const long jall = p.flat || p.lay.nclus > 1 ? (long)a.batch * a.rows * a.q_heads : 0;
+    const int jrows = (p.flat ? SLOTS * WARPS / ((long)a.batch * a.kv_heads) : p.lay.nclus) > 32 ? 1 : 8;
+    const long jblocks = (jall + jrows - 1) / jrows;
+    const long post = jblocks + (long)a.batch * slots * a.rows;
     if (grid > 0x7fffffffl || post > 0x7fffffffl) return fail("attn8: more than 2^31 blocks in one call");
-    if (p.part + p.stats && (!scratch || ((uintptr_t)scratch & 15) || scratch_bytes < p.part + p.stats))
+    const size_t need = p.part + p.stats + p.raws;
+    if (need && (!scratch || ((uintptr_t)scratch & 15) || scratch_bytes < need))
         return fail("attn8: scratch too small or not 16-byte aligned");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     float* part = (float*)scratch;
     float2* stats = slots ? (float2*)((char*)scratch + p.part) : nullptr;
-    const int r = kind == KV8_INT8 ? launch_mode<KV8_INT8>(a, p, part, stats, dc, st)
-                                   : launch_mode<KV8_E4M3>(a, p, part, stats, dc, st);
+    float* raws = slots ? (float*)((char*)scratch + p.part + p.stats) : nullptr;
+    const int r = kind == KV8_INT8 ? launch_mode<KV8_INT8>(a, p, part, stats, raws, dc, st)
+                                   : launch_mode<KV8_E4M3>(a, p, part, stats, raws, dc, st);
     if (r || !post) return r;
-    auto* fn = kind == KV8_INT8 ? attn8_post_kernel<KV8_INT8> : attn8_post_kernel<KV8_E4M3>;
-    return check_pdl(launch_pdl(fn, dim3((unsigned)post), dim3(NT), 0, st, a, (unsigned)jblocks, p.lay.nclus,
-                                p.flat ? (unsigned)(SLOTS * WARPS) : 0u, (const float*)part, (const float2*)stats),
+    return check_pdl(launch_pdl(attn8_post_kernel, dim3((unsigned)post), dim3(jrows == 1 ? 512 : 256), 0, st, a,
+                                (unsigned)jblocks, jrows, p.lay.nclus, p.flat ? (unsigned)(SLOTS * WARPS) : 0u,
+                                (const float*)part, (const float2*)stats, (const float*)raws),
                      "attn8");
 }
 
 void init_attn8_attrs() {
-    const int most = (int)(sizeof(Smem) + WARPS * 32 * (8 * 8 + HD * 4));  // any layout's shared memory
-    auto set = [&](auto* fn) { cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, most); };
+    const int most = (int)(sizeof(Smem) + WARPS * 16 * (8 * 8 + HD * 4));  // any layout's shared memory
+    // every kernel asks for the largest shared memory of an SM: the split from the L1 cache changes only on an idle SM,
+    // and a CTA of the main kernel that finds too little beside the last call's blocks starts when the others end
+    auto carve = [&](auto* fn) {
+        cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    };
+    auto set = [&](auto* fn) {
+        cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        carve(fn);
+    };
+    carve(attn8_post_kernel);
     set(attn8_kernel<KV8_INT8, 0>);
     set(attn8_kernel<KV8_INT8, 1>);
-    set(attn8_kernel<KV8_INT8, 4>);
+    set(attn8_kernel<KV8_INT8, 2>);
     set(attn8_kernel<KV8_E4M3, 0>);
     set(attn8_kernel<KV8_E4M3, 1>);
-    set(attn8_kernel<KV8_E4M3, 4>);
+    set(attn8_kernel<KV8_E4M3, 2>);
     set(attn8_flat_kernel<KV8_INT8, 0>);
     set(attn8_flat_kernel<KV8_INT8, 1>);
     set(attn8_flat_kernel<KV8_E4M3, 0>);
