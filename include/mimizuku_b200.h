@@ -29,7 +29,8 @@ int mmz_init(int device);
 const char* mmz_last_error(void);
 /* Reads and clears the device status word of the current device: code[0] error (0 none, 1 wait timed out,
  * 2 misaligned shared memory, 3 bad argument), code[1] kernel (1 enc_flash, 2 self_attn, 3 cross_attn, 4 layernorm,
- * 5 dec_linear, 6 the wait self-test, 7 logits_argmax, 8 gemm_bias, 10 attn8), code[2] site.
+ * 5 dec_linear, 6 the wait self-test, 7 logits_argmax, 8 gemm_bias, 10 attn8, 11 token_logprobs and
+ * linear_logprobs), code[2] site.
  * Synchronises the device. No reference counterpart (the reference has no in-kernel failure detection). */
 int mmz_status(int code[3]);
 /* Sets the bound on every in-kernel wait, in milliseconds (default 1000). */

@@ -3,29 +3,37 @@
 //     lse = m + log sum e^(x - m),   logp = x_t - lse,   entropy = log sum e^(x - m) - sum e^(x - m) (x - m) / sum e^(x - m)
 // and the `top` largest logits, equal ones by the lower id, each with its log probability. Sums in fp32.
 //
-// Bound by reading the logits, once: a cluster of 1 to 8 CTAs takes a row, a thread 8 logits at a time (16-byte loads
-// from the row's first aligned address on, 64 bytes of a thread in flight), with a running maximum and the two sums in
-// packed fp32. The alternatives cost no work per logit: a thread's running maximum is its largest logit, so after the
-// pass the top-th largest of the warps' maxima is a bound below which no alternative lies, and only threads whose own
-// maximum reaches it (about as many as there are alternatives) have their logits read again, by their whole warp. What
-// reaches the bound is ranked by counting. Where more than LIST logits do (rows of equal logits), the alternatives are
-// found one after another in `top` passes instead.
+// Bound by reading the logits, once: a producer warp streams the row in 16 KB bulk copies through a ring in shared
+// memory (96 KB, two CTAs to an SM), so that memory keeps reading while a row is being finished; 8 warps keep a running
+// maximum and the two sums in packed fp32, 64 bytes of a thread's logits at a time. CTAs go from row to row; few rows are
+// shared by clusters of up to 8 CTAs. The alternatives cost next to no work per logit: a thread keeps the 64 bytes with
+// its largest logit, and the largest logit of its others. After the pass the top-th largest of 16 groups' maxima is a
+// bound below which no alternative lies: about as many threads as there are alternatives reach it, nearly always with
+// the bytes they kept alone; the others' logits are read again, by their whole warp. What reaches the bound is ranked by
+// counting. Where more than LIST logits do (rows of equal logits), the alternatives are found one after another in `top`
+// passes instead.
 #include "launch.h"
 #include "logprobs.cuh"
 
 namespace mmz {
 namespace lp {
-constexpr int NT = 512, NW = NT / 32;
-constexpr int LIST = 1024;  // candidates of a CTA
+constexpr int NT = 256, NW = NT / 32, NG = 16;  // threads that sum, their warps, groups of 16 of them
+constexpr int NS = 6, CB = 16384;               // stages and bytes of the ring
+constexpr int PIECES = CB / 16;                 // 16-byte pieces of a stage: 4 to a thread
+constexpr int LIST = 1024;                      // candidates of a CTA
 constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.4426950408889634f;
 
 struct Smem {
-    unsigned long long list[LIST], best[TOP_MAX], all[8][TOP_MAX];  // all: every CTA's, in the cluster's first
-    float wm[NW], ws[NW], wu[NW];
+    uint8_t ring[NS][CB];
+    unsigned long long list[LIST], best[TOP_MAX], all[8 * TOP_MAX];  // all: every CTA's, in the cluster's first
+    uint64_t full[NS], empty[NS];
+    float gm[NG], ws[NW], wu[NW];
     RowStat stat[8];
     float tau;
-    int n;
+    int n, abort;
 };
+
+__device__ __forceinline__ void sync_sums() { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -33,36 +41,42 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// 8 logits from a 16-byte aligned address
-__device__ __forceinline__ void load8(const h16* p, uint4 (&r)[1]) { r[0] = *reinterpret_cast<const uint4*>(p); }
-__device__ __forceinline__ void load8(const float* p, uint4 (&r)[2]) {
-    r[0] = reinterpret_cast<const uint4*>(p)[0];
-    r[1] = reinterpret_cast<const uint4*>(p)[1];
-}
-__device__ __forceinline__ void floats(const uint4 (&r)[1], float (&x)[8]) {
-    const __half2* h = reinterpret_cast<const __half2*>(&r[0]);
+// the logits of a 16-byte piece: 8 of fp16, 4 of fp32
+template <typename T>
+struct Piece;
+template <>
+struct Piece<h16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void floats(const uint4& r, float (&x)[N]) {
+        const __half2* h = reinterpret_cast<const __half2*>(&r);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(h[i]);
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(h[i]);
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
     }
-}
-__device__ __forceinline__ void floats(const uint4 (&r)[2], float (&x)[8]) {
-    const float* f = reinterpret_cast<const float*>(&r[0]);
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = f[i];
-}
+};
+template <>
+struct Piece<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void floats(const uint4& r, float (&x)[N]) {
+        x[0] = __uint_as_float(r.x), x[1] = __uint_as_float(r.y), x[2] = __uint_as_float(r.z), x[3] = __uint_as_float(r.w);
+    }
+};
 
-// the mask bytes of ids i .. i + 7: two aligned words where both lie inside the mask, else byte by byte
-__device__ __forceinline__ unsigned long long mask8(const unsigned char* sup, int i, int V) {
+// the mask bytes of ids i .. i + N - 1: two aligned words where both lie inside the mask, else byte by byte
+template <int N>
+__device__ __forceinline__ unsigned long long mask_of(const unsigned char* sup, int i, int V) {
     const uintptr_t a = (uintptr_t)(sup + i), w = a & ~(uintptr_t)7;
     const int sh = 8 * (int)(a & 7);
-    if (w >= (uintptr_t)sup && w + 16 <= (uintptr_t)(sup + V)) {
-        const unsigned long long lo = *(const unsigned long long*)w;
-        return sh ? (lo >> sh) | (*(const unsigned long long*)(w + 8) << (64 - sh)) : lo;
-    }
     unsigned long long m = 0;
-    for (int k = 0; k < 8; k++) m |= (unsigned long long)(sup[i + k] != 0) << (8 * k);
+    if (w >= (uintptr_t)sup && w + 16 <= (uintptr_t)(sup + V)) {
+        m = *(const unsigned long long*)w >> sh;
+        if (sh > 64 - 8 * N) m |= *(const unsigned long long*)(w + 8) << (64 - sh);
+        if (N == 4) m &= 0xffffffffull;
+    } else {
+        for (int k = 0; k < N; k++) m |= (unsigned long long)(sup[i + k] != 0) << (8 * k);
+    }
     return m;
 }
 
@@ -86,193 +100,312 @@ struct Run {
         s = fadd2(s, e);
         u = ffma2(e, d, u);
     }
-    __device__ __forceinline__ void add8(const float (&x)[8]) {
-        raise(fmax3(fmax3(x[0], x[1], x[2]), fmax3(x[3], x[4], x[5]), fmaxf(x[6], x[7])));
+    // K pieces of N logits: one look at the maximum, two sets of sums
+    template <int K, int N>
+    __device__ __forceinline__ void add(const float (&x)[K][N], float h) {  // h: the largest of x
+        raise(h);
+        Run other{m, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) add2(x[i], x[i + 1]);
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                add2(x[k][i], x[k][i + 1]);
+                other.add2(x[k][i + 2], x[k][i + 3]);
+            }
+        s = fadd2(s, other.s);
+        u = fadd2(u, other.u);
     }
 };
 }  // namespace lp
 using namespace lp;
 
+// grid: rows in turn over gridDim / cl clusters of cl = 2^lg CTAs (cl > 1: one row to a cluster); dynamic shared memory
+// sizeof(Smem)
 template <typename T>
-__global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const T* x, long ldx, int V, const unsigned char* sup,
-                                                               LogpOut o, int lg) {
-    constexpr int NL = sizeof(T) / 2;        // 16-byte loads of 8 logits
-    constexpr int UN = NL == 1 ? 4 : 2;      // vectors of a thread in flight
-    __shared__ Smem sm;
+__global__ void __launch_bounds__(NT + 32, 2)
+    token_logprobs_kernel(const T* x, long ldx, int rows, int V, const unsigned char* sup, LogpOut o, int lg,
+                          unsigned* status, unsigned long long limit_ns) {
+    constexpr int N = Piece<T>::N;
+    extern __shared__ __align__(128) uint8_t smem[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cl = 1 << lg, rank = blockIdx.x & (cl - 1);
-    const long row = blockIdx.x >> lg;
-    if (threadIdx.x == 0) sm.n = 0;
+    const int row0 = blockIdx.x >> lg, step = gridDim.x >> lg;
+    if (threadIdx.x == 0) {
+        sm.abort = 0;
+        for (int i = 0; i < NS; i++) {
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.empty[i], NW);
+        }
+        fence_mbar_init();
+    }
+    __syncthreads();
+    if (cl > 1) cluster_arrive_relaxed();  // the first CTA has started before anything is sent to it
     griddep_wait();
     griddep_launch_dependents();
-    const long at = row_at(o, row);
-    if (at < 0) return;  // the whole cluster
-    if (cl > 1) cluster_arrive_relaxed();  // the first CTA has started before anything is sent to it
-    const T* xr = x + row * ldx;
-    // ids before the first aligned address, vectors of 8, ids after the last vector; this CTA's share
-    const int head = min(V, (int)((16 - ((uintptr_t)xr & 15)) & 15) / (int)sizeof(T));
-    const int nv = (V - head) / 8, tail = head + nv * 8;
-    const int v0 = (int)((long)nv * rank >> lg), v1 = (int)((long)nv * (rank + 1) >> lg);
-    const int t = o.target ? o.target[at] : -1;
-    auto logit = [&](int i) { return sup && sup[i] ? -INFINITY : (float)xr[i]; };
-    const bool has = t >= 0 && t < V;
-    float tgt = 0.f;
-    if (rank == 0 && threadIdx.x == 0 && has) tgt = logit(t);
-
-    auto vec = [&](int v, const uint4 (&r)[NL], float (&f)[8]) {  // vector v's logits, -inf for what is left out
-        floats(r, f);
-        if (sup) {
-            const unsigned long long m = mask8(sup, head + 8 * v, V);
-            if (m)
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (m >> (8 * k) & 0xff) f[k] = -INFINITY;
-        }
+    const int col = (int)row_at(o, 0);  // the outputs' column, -1: outside them (nothing is read then either)
+    // ids before a row's first aligned address, its pieces, ids after the last piece; this CTA's share of the pieces
+    struct Row {
+        const T* x;
+        int head, np, p0, p1;
     };
-    // the ids outside the vectors: at most 7 before, with the first CTA, and 7 after, with the last
-    const int edge = threadIdx.x < 8 ? (rank == 0 && threadIdx.x < head ? threadIdx.x : -1)
-                     : threadIdx.x < 16 && rank == cl - 1 && tail + threadIdx.x - 8 < V ? tail + (int)threadIdx.x - 8 : -1;
-    Run run{LOWEST, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-    if (edge >= 0) {
-        const float e = logit(edge);
-        run.raise(e);
-        run.add2(e, -INFINITY);
-    }
-    for (int v = v0 + threadIdx.x; v < v1; v += UN * NT) {
-        uint4 r[UN][NL];
-#pragma unroll
-        for (int k = 0; k < UN; k++)
-            if (v + k * NT < v1) load8(xr + head + 8l * (v + k * NT), r[k]);
-#pragma unroll
-        for (int k = 0; k < UN; k++)
-            if (v + k * NT < v1) {
-                float f[8];
-                vec(v + k * NT, r[k], f);
-                run.add8(f);
+    auto row_of = [&](int r) {
+        Row w;
+        w.x = x + r * ldx;
+        w.head = min(V, (int)((16 - ((uintptr_t)w.x & 15)) & 15) / (int)sizeof(T));
+        w.np = (V - w.head) / N;
+        w.p0 = (int)((long)w.np * rank >> lg), w.p1 = (int)((long)w.np * (rank + 1) >> lg);
+        return w;
+    };
+    if (warp == NW) {
+        // ---------------------------------------------------------------- producer
+        if (lane == 0) {
+            unsigned q = 0;
+            bool ok = true;
+            for (int r = row0; r < rows && col >= 0 && ok; r += step) {
+                const Row w = row_of(r);
+                for (int p = w.p0; p < w.p1; p += PIECES, q++) {
+                    const int st = q % NS;
+                    if (q >= NS && !mbar_wait(&sm.empty[st], (q / NS - 1) & 1, &sm.abort, limit_ns, status, K_LOGP, 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bytes = (uint32_t)min(PIECES, w.p1 - p) * 16;
+                    mbar_expect_tx(&sm.full[st], bytes);
+                    bulk_g2s(sm.ring[st], (const uint8_t*)(w.x + w.head) + 16l * p, bytes, &sm.full[st]);
+                }
             }
-    }
-    // ---------------------------------------------------------------- the CTA's statistics
-    const float mine = run.m;
-    float wm = mine;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffff, wm, w));
-    if (lane == 0) sm.wm[warp] = wm;
-    __syncthreads();
-    float M = LOWEST;
-#pragma unroll
-    for (int w = 0; w < NW; w++) M = fmaxf(M, sm.wm[w]);
-    run.raise(M);
-    float S = run.s.x + run.s.y, U = run.u.x + run.u.y;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) {
-        S += __shfl_xor_sync(0xffffffff, S, w);
-        U += __shfl_xor_sync(0xffffffff, U, w);
-    }
-    if (lane == 0) sm.ws[warp] = S, sm.wu[warp] = U;
-    // ---------------------------------------------------------------- its alternatives
-    if (o.top > 0) {
-        if (warp == 0 && lane < NW) {  // the top-th largest of the warps' maxima
-            const float a = sm.wm[lane];
-            int above = 0;
-#pragma unroll
-            for (int w = 0; w < NW; w++) above += sm.wm[w] > a || (sm.wm[w] == a && w < lane);
-            if (above == o.top - 1) sm.tau = a;
+            if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
+                for (unsigned i = q > NS ? q - NS : 0; i < q; i++)
+                    mbar_wait(&sm.full[i % NS], (i / NS) & 1, nullptr, limit_ns, nullptr, 0, 0);
         }
-        __syncthreads();
-        const float tau = sm.tau;
-        auto take = [&](float f, int id) {
-            const unsigned long long key = f >= tau ? top_key(f, id) : 0ull;
-            if (key) {
-                const int k = atomicAdd(&sm.n, 1);
-                if (k < LIST) sm.list[k] = key;
+        __syncwarp();
+        if (cl > 1) {
+            cluster_wait();
+            if (col >= 0) cluster_sync();
+        }
+        return;
+    }
+    if (cl > 1) cluster_wait();
+    if (col < 0) return;
+    unsigned q = 0;
+    bool ok = true;
+    for (int r = row0; r < rows; r += step) {
+        const Row w = row_of(r);
+        const T* xr = w.x;
+        const int head = w.head, tail = head + w.np * N;
+        const long at = row_at(o, r);
+        const int t = o.target ? o.target[at] : -1;
+        auto logit = [&](int i) { return sup && sup[i] ? -INFINITY : (float)xr[i]; };
+        const bool has = t >= 0 && t < V;
+        float tgt = 0.f;
+        if (rank == 0 && threadIdx.x == 0 && has) tgt = logit(t);
+        auto piece = [&](int p, const uint4& v, float (&f)[N]) {  // piece p's logits, -inf for what is left out
+            Piece<T>::floats(v, f);
+            if (sup) {
+                const unsigned long long m = mask_of<N>(sup, head + N * p, V);
+                if (m)
+#pragma unroll
+                    for (int k = 0; k < N; k++)
+                        if (m >> (8 * k) & 0xff) f[k] = -INFINITY;
             }
         };
-        if (edge >= 0) take(logit(edge), edge);
-        for (unsigned who = __ballot_sync(0xffffffff, mine >= tau); who; who &= who - 1) {
-            const int first = v0 + warp * 32 + __ffs(who) - 1;  // the thread's vectors: every NT-th from here
-            for (int v = first + lane * NT; v < v1; v += 32 * NT) {
-                uint4 r[NL];
-                float f[8];
-                load8(xr + head + 8l * v, r);
-                vec(v, r, f);
+        // the ids outside the pieces: at most 7 before, with the first CTA, and 7 after, with the last
+        const int edge = threadIdx.x < 8 ? (rank == 0 && threadIdx.x < head ? (int)threadIdx.x : -1)
+                         : threadIdx.x < 16 && rank == cl - 1 && tail + (int)threadIdx.x - 8 < V ? tail + (int)threadIdx.x - 8 : -1;
+        Run run{LOWEST, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if (edge >= 0) {
+            const float e = logit(edge);
+            run.raise(e);
+            run.add2(e, -INFINITY);
+        }
+        uint4 kept[PIECES / NT] = {};            // the stage's pieces with the thread's largest logit,
+        int kept_p = -1;                         // the first of them (-1: none),
+        float most = LOWEST, others = -INFINITY;  // that logit, and the largest in the thread's other pieces
+        for (int p = w.p0; p < w.p1; p += PIECES, q++) {
+            const int st = q % NS, n = min(PIECES, w.p1 - p);
+            ok = ok && __all_sync(0xffffffff, mbar_wait(&sm.full[st], (q / NS) & 1, &sm.abort, limit_ns, status, K_LOGP, 2));
+            if (!ok) continue;
+            uint4 v[PIECES / NT];
 #pragma unroll
-                for (int k = 0; k < 8; k++) take(f[k], head + 8 * v + k);
+            for (int k = 0; k < PIECES / NT; k++) v[k] = reinterpret_cast<const uint4*>(sm.ring[st])[k * NT + threadIdx.x];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.empty[st]);
+            float f[PIECES / NT][N];
+#pragma unroll
+            for (int k = 0; k < PIECES / NT; k++) {
+                if (k * NT + (int)threadIdx.x < n) {
+                    piece(p + k * NT + threadIdx.x, v[k], f[k]);
+                } else {  // past the row's last piece
+#pragma unroll
+                    for (int e = 0; e < N; e++) f[k][e] = -INFINITY;
+                }
+            }
+            float h = f[0][0];
+#pragma unroll
+            for (int k = 0; k < PIECES / NT; k++)
+#pragma unroll
+                for (int i = 0; i < N; i += 2) h = fmax3(h, f[k][i], f[k][i + 1]);
+            run.add(f, h);
+            if (h > most) {
+                others = most, most = h, kept_p = p;
+#pragma unroll
+                for (int k = 0; k < PIECES / NT; k++) kept[k] = v[k];
+            } else {
+                others = fmaxf(others, h);
             }
         }
+        // ---------------------------------------------------------------- the CTA's statistics
+        float gm = run.m;
+#pragma unroll
+        for (int d = 8; d; d >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffff, gm, d));
+        if ((lane & 15) == 0) sm.gm[threadIdx.x >> 4] = gm;
+        if (threadIdx.x == 0) sm.n = 0;
         if (threadIdx.x < TOP_MAX) sm.best[threadIdx.x] = 0ull;
-        __syncthreads();
-        const int n = sm.n;
-        if (n <= LIST) {
-            for (int i = threadIdx.x; i < n; i += NT) {  // a key's rank is the number of larger ones: no two are equal
-                const unsigned long long key = sm.list[i];
+        sync_sums();
+        float M = LOWEST;
+#pragma unroll
+        for (int g = 0; g < NG; g++) M = fmaxf(M, sm.gm[g]);
+        run.raise(M);
+        float S = run.s.x + run.s.y, U = run.u.x + run.u.y;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            S += __shfl_xor_sync(0xffffffff, S, d);
+            U += __shfl_xor_sync(0xffffffff, U, d);
+        }
+        if (lane == 0) sm.ws[warp] = S, sm.wu[warp] = U;
+        // ---------------------------------------------------------------- its alternatives
+        if (o.top > 0) {
+            // every warp finds the top-th largest of the groups' maxima
+            const float a = sm.gm[lane & 15];
+            int above = 0;
+#pragma unroll
+            for (int g = 0; g < NG; g++) above += sm.gm[g] > a || (sm.gm[g] == a && g < (lane & 15));
+            const float tau = __shfl_sync(0xffffffff, a, __ffs(__ballot_sync(0xffffffff, above == o.top - 1)) - 1);
+            auto take = [&](float f, int id) {
+                const unsigned long long key = f >= tau ? top_key(f, id) : 0ull;
+                if (key) {
+                    const int k = atomicAdd(&sm.n, 1);
+                    if (k < LIST) sm.list[k] = key;
+                }
+            };
+            if (edge >= 0) take(logit(edge), edge);
+            if (kept_p >= 0 && most >= tau && !(others >= tau)) {
+#pragma unroll
+                for (int k = 0; k < PIECES / NT; k++) {
+                    const int p = kept_p + k * NT + threadIdx.x;
+                    if (p < w.p1) {
+                        float f[N];
+                        piece(p, kept[k], f);
+#pragma unroll
+                        for (int e = 0; e < N; e++) take(f[e], head + N * p + e);
+                    }
+                }
+            }
+            // two threads' pieces (every NT-th from the thread's first) at a time, two loads of each in flight
+            for (unsigned who = __ballot_sync(0xffffffff, others >= tau); who;) {
+                int first[2];
+                first[0] = first[1] = w.p0 + warp * 32 + __ffs(who) - 1;
+                who &= who - 1;
+                if (who) first[1] = w.p0 + warp * 32 + __ffs(who) - 1;
+                who &= who - 1;
+                const int sets = first[1] == first[0] ? 1 : 2;
+                for (int d = lane * NT; first[0] + d - lane * NT < w.p1; d += 64 * NT) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int p = first[k >> 1] + d + (k & 1) * 32 * NT;
+                        if ((k >> 1) < sets && p < w.p1) v[k] = reinterpret_cast<const uint4*>(xr + head)[p];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int p = first[k >> 1] + d + (k & 1) * 32 * NT;
+                        if ((k >> 1) < sets && p < w.p1) {
+                            float f[N];
+                            piece(p, v[k], f);
+#pragma unroll
+                            for (int e = 0; e < N; e++) take(f[e], head + N * p + e);
+                        }
+                    }
+                }
+            }
+            sync_sums();
+            const int n = sm.n;
+            if (n <= LIST) {
+                for (int i = threadIdx.x; i < n; i += NT) {  // a key's rank is the number of larger ones: no two are equal
+                    const unsigned long long key = sm.list[i];
+                    int more = 0;
+                    for (int k = 0; k < n && more < o.top; k++) more += sm.list[k] > key;
+                    if (more < o.top) sm.best[more] = key;
+                }
+            } else {
+                unsigned long long last = ~0ull;
+                for (int k = 0; k < o.top; k++) {
+                    unsigned long long b = 0;
+                    auto see = [&](float f, int id) {
+                        const unsigned long long key = top_key(f, id);
+                        if (key < last && key > b) b = key;
+                    };
+                    if (edge >= 0) see(logit(edge), edge);
+                    for (int p = w.p0 + threadIdx.x; p < w.p1; p += NT) {
+                        float f[N];
+                        piece(p, reinterpret_cast<const uint4*>(xr + head)[p], f);
+#pragma unroll
+                        for (int e = 0; e < N; e++) see(f[e], head + N * p + e);
+                    }
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) {
+                        const unsigned long long c = __shfl_xor_sync(0xffffffff, b, d);
+                        b = c > b ? c : b;
+                    }
+                    sync_sums();
+                    if (lane == 0) sm.list[warp] = b;
+                    sync_sums();
+                    for (int g = 0; g < NW; g++) b = sm.list[g] > b ? sm.list[g] : b;
+                    if (threadIdx.x == 0) sm.best[k] = b;
+                    last = b;
+                }
+            }
+        }
+        sync_sums();
+        // ---------------------------------------------------------------- the cluster's CTAs joined in its first
+        if (warp == 0) {
+            S = lane < NW ? sm.ws[lane] : 0.f, U = lane < NW ? sm.wu[lane] : 0.f;
+#pragma unroll
+            for (int d = NW / 2; d; d >>= 1) {
+                S += __shfl_xor_sync(0xffffffff, S, d);
+                U += __shfl_xor_sync(0xffffffff, U, d);
+            }
+            if (lane == 0) {
+                const uint32_t to = dsmem_addr(&sm.stat[rank], 0);
+                st_dsmem_f32(to, S == 0.f ? -INFINITY : M);  // nothing above -inf: the empty set
+                st_dsmem_f32(to + 4, S);
+                st_dsmem_f32(to + 8, U);
+            }
+            if (lane < TOP_MAX && lane < o.top)
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dsmem_addr(&sm.all[rank * o.top + lane], 0)),
+                             "l"(sm.best[lane])
+                             : "memory");
+            __syncwarp();
+        }
+        if (cl > 1) cluster_sync();
+        if (rank == 0 && warp == 0) {
+            RowStat a = lane < cl ? sm.stat[lane] : stat_none();
+            for (int d = 1; d < cl; d *= 2)
+                a = stat_join(a, {__shfl_xor_sync(0xffffffff, a.m, d), __shfl_xor_sync(0xffffffff, a.s, d),
+                                  __shfl_xor_sync(0xffffffff, a.u, d)});
+            float lse = 0.f;
+            if (lane == 0) lse = store_row(o, at, a, has, tgt);
+            lse = __shfl_sync(0xffffffff, lse, 0);
+            const int n = cl * o.top;
+            for (int i = lane; i < n; i += 32) {
+                const unsigned long long key = sm.all[i];
                 int above = 0;
-                for (int k = 0; k < n && above < o.top; k++) above += sm.list[k] > key;
-                if (above < o.top) sm.best[above] = key;
+#pragma unroll 8
+                for (int k = 0; k < n; k++) above += sm.all[k] > key || (sm.all[k] == key && k < i);  // only empty ones are equal
+                if (above < o.top) store_top(o, at, above, key, lse);
             }
-        } else {
-            unsigned long long last = ~0ull;
-            for (int k = 0; k < o.top; k++) {
-                unsigned long long b = 0;
-                auto see = [&](float f, int id) {
-                    const unsigned long long key = top_key(f, id);
-                    if (key < last && key > b) b = key;
-                };
-                if (edge >= 0) see(logit(edge), edge);
-                for (int v = v0 + threadIdx.x; v < v1; v += NT) {
-                    uint4 r[NL];
-                    float f[8];
-                    load8(xr + head + 8l * v, r);
-                    vec(v, r, f);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) see(f[e], head + 8 * v + e);
-                }
-#pragma unroll
-                for (int w = 16; w; w >>= 1) {
-                    const unsigned long long c = __shfl_xor_sync(0xffffffff, b, w);
-                    b = c > b ? c : b;
-                }
-                if (lane == 0) sm.list[warp] = b;
-                __syncthreads();
-                for (int w = 0; w < NW; w++) b = sm.list[w] > b ? sm.list[w] : b;
-                __syncthreads();
-                if (threadIdx.x == 0) sm.best[k] = b;
-                last = b;
-            }
+            __syncwarp();
         }
-    }
-    __syncthreads();
-    if (cl > 1) cluster_wait();
-    // ---------------------------------------------------------------- the cluster's CTAs joined in its first
-    if (warp == 0) {
-        if (lane == 0) {
-            S = U = 0.f;
-            for (int w = 0; w < NW; w++) S += sm.ws[w], U += sm.wu[w];
-            const uint32_t to = dsmem_addr(&sm.stat[rank], 0);
-            st_dsmem_f32(to, S == 0.f ? -INFINITY : M);  // nothing above -inf: the empty set
-            st_dsmem_f32(to + 4, S);
-            st_dsmem_f32(to + 8, U);
-        }
-        if (lane < TOP_MAX && lane < o.top)
-            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dsmem_addr(&sm.all[rank][lane], 0)), "l"(sm.best[lane])
-                         : "memory");
-    }
-    if (cl > 1) cluster_sync();
-    else __syncthreads();
-    if (rank || warp) return;
-    RowStat a = sm.stat[0];
-    for (int c = 1; c < cl; c++) a = stat_join(a, sm.stat[c]);
-    float lse = 0.f;
-    if (lane == 0) lse = store_row(o, at, a, has, tgt);
-    lse = __shfl_sync(0xffffffff, lse, 0);
-    for (int i = lane; i < cl * o.top; i += 32) {
-        const unsigned long long key = sm.all[i / o.top][i % o.top];
-        int above = 0;
-        for (int k = 0; k < cl * o.top; k++) {
-            const unsigned long long other = sm.all[k / o.top][k % o.top];
-            above += other > key || (other == key && k < i);  // only the empty ones are equal
-        }
-        if (above < o.top) store_top(o, at, above, key, lse);
     }
 }
 
@@ -292,17 +425,18 @@ int launch_token_logprobs(const void* x, long long ldx, int type, int rows, int 
     if (logp_check("token_logprobs", o)) return -1;
     if (rows == 0) return 0;
     if (!x || ((uintptr_t)x & (type ? 3 : 1))) return fail("token_logprobs: logits null or not aligned to their type");
-    // CTAs of a row: shares of at most 64 KB, and as many CTAs as fit at once (2 to an SM) while a share is above 8 KB
+    // a CTA to a row, two to an SM, each going from row to row; fewer than 148 rows: clusters, while the CTAs fit at once
+    // and a CTA's share is above 8 KB (32 rows of 104 KB: 8 CTAs each)
     const long bytes = (long)V * (type ? 4 : 2);
     int lg = 0;
-    while (lg < 3 && (bytes >> lg > 65536 || ((long)rows << lg <= 148 && bytes >> lg > 8192))) lg++;
-    const int cl = 1 << lg;
-    if ((long)rows * cl > 0x7fffffffl) return fail("token_logprobs: too many rows in one call");
+    while (lg < 3 && (long)rows << lg <= 148 && bytes >> lg > 8192) lg++;
+    const int cl = 1 << lg, grid = lg ? rows << lg : rows < 296 ? rows : 296;
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * cl));
-    cfg.blockDim = dim3(NT);
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(NT + 32);
+    cfg.dynamicSmemBytes = sizeof(Smem);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -312,9 +446,16 @@ int launch_token_logprobs(const void* x, long long ldx, int type, int rows, int 
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return check_pdl(type ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<float>, (const float*)x, (long)ldx, V, sup, o, lg)
-                          : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<h16>, (const h16*)x, (long)ldx, V, sup, o, lg),
+    return check_pdl(type ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<float>, (const float*)x, (long)ldx, rows, V, sup,
+                                               o, lg, dc.status, dc.limit_ns)
+                          : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<h16>, (const h16*)x, (long)ldx, rows, V, sup, o,
+                                               lg, dc.status, dc.limit_ns),
                      "token_logprobs");
+}
+
+void init_logprobs_attrs() {
+    cudaFuncSetAttribute(token_logprobs_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem));
+    cudaFuncSetAttribute(token_logprobs_kernel<h16>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem));
 }
 
 }  // namespace mmz

@@ -76,6 +76,7 @@ static void init_ctx(DevCtx& c, int dev) {
     init_gemv_attrs();
     init_align_attrs();
     init_attn8_attrs();
+    init_logprobs_attrs();
     cudaGetLastError();
     c.ok = true;
     c.err = "";
