@@ -71,6 +71,7 @@ void init_gemm_attrs(DevCtx& c);
 void init_align_attrs();
 void init_attn8_attrs();
 void init_logprobs_attrs();
+void init_linear_logprobs_attrs();
 
 // launchers (device pointers, asynchronous on `st`); 0 on success, -1 with the last error set
 size_t cross_attn_scratch_bytes(int batch, int d);

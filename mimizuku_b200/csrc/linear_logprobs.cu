@@ -1,65 +1,554 @@
-// Log probabilities from hidden states, for sm_100a: token_logprobs (logprobs.cu) of the logits x . emb^T, which keep
-// the product's fp32 sums (no rounding between the product and the softmax).
+// Log probabilities from hidden states, for sm_100a: token_logprobs (logprobs.cu) of the logits x . emb^T, without the
+// logits in memory. A product on the 5th-generation tensor cores whose epilogue, instead of storing a tile, takes it into
+// its rows' running maximum, sums and alternatives; the fp32 sums are used as they are.
+//
+// D[rows][vocabulary ids], so that a thread of the epilogue has a row: one TMEM lane, 32 ids at a time. Per id it does
+// what token_logprobs does (packed fp32, one exponential); where a chunk of 32 has a logit above the row's last
+// alternative, or the target, the warp puts the chunk into shared memory and each lane picks its own out. Each CTA (or
+// pair) has an equal share of the (row tile, vocabulary tile) sequence, vocabulary innermost, and leaves one record per
+// row tile it worked on; a second kernel joins the records of a row.
+//   up to 128 rows   linear_one_kernel: tiles of 128 rows x 128 ids, a CTA to an SM. Bound by reading the embedding once
+//                    (the rows are zero-padded to 128 in the product, but only loaded to the next 8)
+//   more             linear_pair_kernel: tiles of 256 x 256 on pairs of CTAs (cta_group::2). Bound by the tensor cores
+//                    (at a width of 1280 a tile's products take about five times its epilogue)
+// Both: a TMA producer and an MMA issuer (one warp each) feed two TMEM accumulators in turn, the epilogue works on one
+// while the other fills. Every wait is bounded; a CTA that gives up lets its copies land, waits for its MMAs and frees its
+// TMEM.
 #include "launch.h"
 #include "logprobs.cuh"
 
 namespace mmz {
 namespace ll {
-constexpr int T = 64;  // tile of the product
-}  // namespace ll
 
-// y[rows][V] = x . emb^T, 64 x 64 tiles, 4 x 4 sums to a thread
-__global__ void __launch_bounds__(256) linear_kernel(const h16* x, long ldx, const h16* emb,
-                                                     int rows, int V, int d, float* y) {
-    __shared__ float xs[16][ll::T + 1], es[16][ll::T + 1];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const long r0 = (long)blockIdx.y * ll::T, v0 = (long)blockIdx.x * ll::T;
-    griddep_wait();
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < d; k0 += 16) {
-        for (int i = threadIdx.x; i < 16 * ll::T; i += 256) {
-            const int k = i & 15, r = i >> 4;
-            xs[k][r] = r0 + r < rows ? f(x[(r0 + r) * ldx + k0 + k]) : 0.f;
-            es[k][r] = v0 + r < V ? f(emb[(v0 + r) * d + k0 + k]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] += xs[k][ty + 16 * i] * es[k][tx + 16 * j];
-        __syncthreads();
+constexpr int BK = 64;              // K per stage (one 128-byte swizzle atom)
+constexpr int FIELDS = 4 + 2 * TOP_MAX;  // a record's fields: m, s, u, the target's logit, alternatives' logits and ids
+constexpr int PAIRS = 74;           // pairs of SMs of a B200
+
+// equal contiguous shares of T tiles for W workers, the first T % W have one more
+struct Share {
+    int T, W, per, more;
+    __host__ __device__ Share(int T, int W) : T(T), W(W), per(T / W), more(T % W) {}
+    __host__ __device__ int first(int w) const { return w * per + (w < more ? w : more); }
+    __host__ __device__ int count(int w) const { return per + (w < more ? 1 : 0); }
+    __host__ __device__ int owner(int f) const {
+        const int big = more * (per + 1);
+        return f < big ? f / (per + 1) : more + (f - big) / per;
     }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const long r = r0 + ty + 16 * i, v = v0 + tx + 16 * j;
-            if (r < rows && v < V) y[r * V + v] = acc[i][j];
+};
+
+// One row's running state in a thread of the epilogue.
+struct RowState {
+    Run run;
+    float v[TOP_MAX], tgt, kth;
+    int id[TOP_MAX];
+    __device__ __forceinline__ void clear() {
+        run = {LOWEST, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        tgt = kth = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < TOP_MAX; i++) v[i] = -INFINITY, id[i] = -1;
+    }
+    // x among the largest, behind equal ones (ids come in order)
+    __device__ __forceinline__ void insert(float x, int n, int top) {
+#pragma unroll
+        for (int i = TOP_MAX - 1; i >= 0; i--) {
+            const bool here = x > v[i], up = i > 0 && x > v[i > 0 ? i - 1 : 0];
+            v[i] = up ? v[i > 0 ? i - 1 : 0] : here ? x : v[i];
+            id[i] = up ? id[i > 0 ? i - 1 : 0] : here ? n : id[i];
         }
+        kth = v[0];
+#pragma unroll
+        for (int i = 1; i < TOP_MAX; i++)
+            if (i < top) kth = v[i];
+    }
+    // 32 logits of ids c0 .. c0 + 31, those with a bit in `out` left out; box: the warp's [32 ids][32 lanes] floats
+    __device__ __forceinline__ void take(const uint32_t (&acc)[32], int c0, uint32_t out, int target, int top, float* box,
+                                         int lane) {
+        float x[1][32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) x[0][i] = __uint_as_float(acc[i]);
+        if (out) {
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+                if (out >> i & 1) x[0][i] = -INFINITY;
+        }
+        float h = fmax3(x[0][0], x[0][1], x[0][2]);
+#pragma unroll
+        for (int i = 3; i < 31; i += 2) h = fmax3(h, x[0][i], x[0][i + 1]);
+        h = fmaxf(h, x[0][31]);
+        run.add(x, h);
+        const bool mine = target >= c0 && target < c0 + 32, more = top > 0 && h > kth;
+        if (!__any_sync(0xffffffff, mine || more)) return;
+        uint32_t cand = 0;
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            box[i * 32 + lane] = x[0][i];  // read by the same lane only
+            if (x[0][i] > kth) cand |= 1u << i;
+        }
+        if (mine) tgt = box[(target - c0) * 32 + lane];
+        if (top == 0) return;
+        for (; cand; cand &= cand - 1) {
+            const int i = __ffs(cand) - 1;
+            const float f = box[i * 32 + lane];
+            if (f > kth) insert(f, c0 + i, top);
+        }
+    }
+    // field k of the row's record at rec[k * rows]
+    __device__ __forceinline__ void store(float* rec, int rows, int top) const {
+        const float s = run.s.x + run.s.y;
+        rec[0] = s == 0.f ? -INFINITY : run.m;  // nothing above -inf: the empty set
+        rec[rows] = s;
+        rec[2l * rows] = run.u.x + run.u.y;
+        rec[3l * rows] = tgt;
+#pragma unroll
+        for (int i = 0; i < TOP_MAX; i++)
+            if (i < top) rec[(4l + i) * rows] = v[i], rec[(4l + TOP_MAX + i) * rows] = __int_as_float(id[i]);
+    }
+};
+
+// the ids c0 .. c0 + 31 that are left out: suppressed, or past the vocabulary
+__device__ __forceinline__ uint32_t left_out(const unsigned char* sup, int c0, int V, int lane) {
+    const int id = c0 + lane;
+    return __ballot_sync(0xffffffff, id >= V || (sup && sup[id]));
 }
 
-size_t linear_logprobs_scratch_bytes(int rows, int V, int) { return ((size_t)rows * V * 4 + 15) & ~(size_t)15; }
+namespace one {
+constexpr int BM = 128, BN = 128, NS = 6, NTHREADS = 192;  // warps 0-3 epilogue, 4 TMA, 5 MMA
+constexpr int AT = BM * BK * 2, BT = BN * BK * 2;          // 16 KB each
+constexpr uint32_t IDESC = idesc_f16_f32(BM, BN, false);
+struct Smem {
+    uint8_t a[NS][AT], b[NS][BT];
+    float box[4][32 * 32];
+    uint64_t full[NS], empty[NS], accf[2], acce[2], fin;
+    uint32_t tmem;
+    int abort;
+};
+}  // namespace one
+
+namespace pair {
+constexpr int BMC = 128, BN = 256, NS = 5, EPW = 8, NTHREADS = 64 + 32 * EPW;  // warp 0 TMA, 1 MMA, 2-9 epilogue
+constexpr int AT = BMC * BK * 2, BT = BN / 2 * BK * 2;                         // 16 KB each, in each CTA
+constexpr uint32_t IDESC = idesc_f16_f32(2 * BMC, BN, false);
+struct Smem {
+    uint8_t a[NS][AT], b[NS][BT];
+    float box[EPW][32 * 32];
+    uint64_t full[NS], empty[NS], accf[2], acce[2], fin;
+    uint32_t tmem;
+    int abort;
+};
+}  // namespace pair
+}  // namespace ll
+using namespace ll;
+
+// grid min(SMs, tiles), block NTHREADS, dynamic shared memory sizeof(Smem) + 1024 (alignment slack). xbox: rows that a
+// load of x brings (a multiple of 8). rec [CTAs][FIELDS][128]
+__global__ void __launch_bounds__(one::NTHREADS, 1)
+    linear_one_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap emap, int rows, int V,
+                      int d, int xbox, const unsigned char* sup, LogpOut o, float* rec, unsigned* status,
+                      unsigned long long limit_ns) {
+    using namespace one;
+    extern __shared__ uint8_t smem_raw[];
+    Smem& s = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+    const Share share((V + BN - 1) / BN, gridDim.x);
+    const int t0 = share.first(cta), my = share.count(cta), nch = d / BK, nq = my * nch;
+    volatile int* abort = &s.abort;
+    if (warp == 4 && lane == 0) {
+        s.abort = 0;
+        for (int i = 0; i < NS; i++) {
+            mbar_init(&s.full[i], 1);
+            mbar_init(&s.empty[i], 1);
+        }
+        for (int a = 0; a < 2; a++) {
+            mbar_init(&s.accf[a], 1);
+            mbar_init(&s.acce[a], 4);
+        }
+        mbar_init(&s.fin, 1);
+        fence_mbar_init();
+        prefetch_tmap(&xmap);
+        prefetch_tmap(&emap);
+    }
+    if (warp == 5) {
+        tmem_alloc(&s.tmem, 2 * BN);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint32_t tb = s.tmem;
+    if (warp == 4) {
+        // ---------------------------------------------------------------- producer
+        if (lane == 0) {
+            int issued = 0;
+            for (int q = 0; q < nq; q++) {
+                const int st = q % NS, i = q / nch, kc = q % nch;
+                if (q >= NS && !mbar_wait_spin(&s.empty[st], ((q / NS) - 1) & 1, abort, limit_ns, status, K_LOGP, 3)) break;
+                mbar_expect_tx(&s.full[st], BT + xbox * BK * 2);
+                tma_load_2d(s.b[st], &emap, kc * BK, (t0 + i) * BN, &s.full[st]);
+                tma_load_2d(s.a[st], &xmap, kc * BK, 0, &s.full[st]);
+                issued = q + 1;
+            }
+            if (*abort)  // let every issued copy land before the shared memory is released
+                for (int q = issued > NS ? issued - NS : 0; q < issued; q++)
+                    mbar_wait(&s.full[q % NS], (q / NS) & 1, nullptr, limit_ns, nullptr, 0, 0);
+        }
+    } else if (warp == 5) {
+        // ---------------------------------------------------------------- MMA issuer
+        if (lane == 0) {
+            const uint64_t ad0 = sdesc_sw128(smem_u32(s.a[0]), 16, 1024), bd0 = sdesc_sw128(smem_u32(s.b[0]), 16, 1024);
+            constexpr uint64_t ASTAGE = AT >> 4, BSTAGE = BT >> 4, KSTEP = 32 >> 4;
+            bool ok = true;
+            for (int i = 0, q = 0; ok && i < my; i++) {
+                const int a = i & 1;
+                if (i >= 2 && !mbar_wait_spin(&s.acce[a], ((i >> 1) - 1) & 1, abort, limit_ns, status, K_LOGP, 4)) break;
+                tc_fence_after();
+                for (int kc = 0; kc < nch; kc++, q++) {
+                    const int st = q % NS;
+                    if (!mbar_wait_spin(&s.full[st], (q / NS) & 1, abort, limit_ns, status, K_LOGP, 5)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; kk++)
+                        umma_f16_ss(tb + a * BN, ad0 + st * ASTAGE + kk * KSTEP, bd0 + st * BSTAGE + kk * KSTEP, IDESC,
+                                    (kc > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit(&s.empty[st]);
+                }
+                if (ok) umma_commit(&s.accf[a]);
+            }
+            umma_commit(&s.fin);  // completes once every MMA issued above has finished
+        }
+    } else {
+        // ---------------------------------------------------------------- epilogue: thread = row
+        const int row = warp * 32 + lane, col = (int)row_at(o, 0);
+        const bool live = warp * 32 < rows && col >= 0;
+        const int target = live && row < rows && o.target ? o.target[row_at(o, row)] : -1;
+        const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);
+        RowState r;
+        r.clear();
+        for (int i = 0; i < my; i++) {
+            const int a = i & 1, n0 = (t0 + i) * BN;
+            const bool ok =
+                __all_sync(0xffffffff, mbar_wait_spin(&s.accf[a], (i >> 1) & 1, abort, limit_ns, status, K_LOGP, 6));
+            if (ok && live) {
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < BN / 32; c++) {
+                    const uint32_t out = left_out(sup, n0 + 32 * c, V, lane);
+                    uint32_t acc[32];
+                    __syncwarp();
+                    tmem_ld32(tl + a * BN + 32 * c, acc);
+                    if (out != 0xffffffffu) r.take(acc, n0 + 32 * c, out, target, o.top, s.box[warp], lane);
+                }
+                tc_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.acce[a]);
+        }
+        if (live && row < rows) r.store(rec + (long)cta * FIELDS * BM + row, BM, o.top);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 5) {  // the MMA pipe must drain before the TMEM is released
+        mbar_wait(&s.fin, 0, nullptr, limit_ns, status, K_LOGP, 7);
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tb, 2 * BN);
+    }
+}
+
+// grid 2 x pairs, cluster (2, 1, 1), block NTHREADS, dynamic shared memory sizeof(Smem) + 1024. emap: a box of 128 ids
+// (half of a tile's). rec [row tiles][parts][2 halves of a tile's ids][FIELDS][256]
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap emap, int rows, int V,
+                       int d, int parts, const unsigned char* sup, LogpOut o, float* rec, unsigned* status,
+                       unsigned long long limit_ns) {
+    using namespace pair;
+    extern __shared__ uint8_t smem_raw[];
+    Smem& s = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();  // 0: the CTA that issues the MMAs
+    const bool lead = rank == 0;
+    const int pid = blockIdx.x / 2, nt = (V + BN - 1) / BN, mt = (rows + 2 * BMC - 1) / (2 * BMC);
+    const Share share(mt * nt, gridDim.x / 2);
+    const int t0 = share.first(pid), my = share.count(pid), nch = d / BK, nq = my * nch;
+    volatile int* abort = &s.abort;
+    if (warp == 0 && lane == 0) {
+        s.abort = 0;
+        for (int i = 0; i < NS; i++) {
+            mbar_init(&s.full[i], 1);  // the even CTA's producer (expected bytes of both CTAs)
+            mbar_init(&s.empty[i], 1);
+        }
+        for (int a = 0; a < 2; a++) {
+            mbar_init(&s.accf[a], 1);
+            mbar_init(&s.acce[a], 2 * EPW);  // both CTAs' epilogue warps (used in the even CTA)
+        }
+        mbar_init(&s.fin, 1);
+        fence_mbar_init();
+        prefetch_tmap(&xmap);
+        prefetch_tmap(&emap);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(&s.tmem, 2 * BN);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();  // both CTAs' barriers initialised and TMEM allocated before either touches the other's
+    tc_fence_after();
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint32_t tb = s.tmem;
+    if (warp == 0) {
+        // ---------------------------------------------------------------- producer (each CTA, its own halves)
+        if (lane == 0) {
+            const uint32_t full0 = dsmem_addr(&s.full[0], 0);
+            int issued = 0, st = 0, ph = 0;  // ring slot and its use count
+            for (int i = 0; i < my; i++) {
+                const int arow = (t0 + i) / nt * 2 * BMC + (int)rank * BMC, brow = (t0 + i) % nt * BN + (int)rank * (BN / 2);
+                bool ok = true;
+                for (int kc = 0; kc < nch; kc++) {
+                    if (issued >= NS && !mbar_wait_spin(&s.empty[st], (ph - 1) & 1, abort, limit_ns, status, K_LOGP, 8)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lead) mbar_expect_tx(&s.full[st], 2 * (AT + BT));
+                    tma_load_2d_pair(s.b[st], &emap, kc * BK, brow, full0 + 8 * st);
+                    tma_load_2d_pair(s.a[st], &xmap, kc * BK, arow, full0 + 8 * st);
+                    issued++;
+                    if (++st == NS) st = 0, ph++;
+                }
+                if (!ok) break;
+            }
+            // let the copies counted on this CTA's barriers land before shared memory is released (the odd CTA's land on
+            // the even CTA's barriers, which the even CTA waits for here; the pair leaves together)
+            if (*abort && lead)
+                for (int q = issued > NS ? issued - NS : 0; q < issued; q++)
+                    mbar_wait(&s.full[q % NS], (q / NS) & 1, nullptr, limit_ns, nullptr, 0, 0);
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer (even CTA)
+        if (lead && lane == 0) {
+            const uint64_t ad0 = sdesc_sw128(smem_u32(s.a[0]), 16, 1024), bd0 = sdesc_sw128(smem_u32(s.b[0]), 16, 1024);
+            constexpr uint64_t ASTAGE = AT >> 4, BSTAGE = BT >> 4, KSTEP = 32 >> 4;
+            const uint32_t empty0[2] = {dsmem_addr(&s.empty[0], 0), dsmem_addr(&s.empty[0], 1)};
+            const uint32_t accf0[2] = {dsmem_addr(&s.accf[0], 0), dsmem_addr(&s.accf[0], 1)};
+            bool ok = true;
+            int st = 0, ph = 0;
+            for (int i = 0; ok && i < my; i++) {
+                const int a = i & 1;
+                if (i >= 2 && !mbar_wait_cluster(&s.acce[a], ((i >> 1) - 1) & 1, abort, limit_ns, status, K_LOGP, 9)) break;
+                tc_fence_after();
+                for (int kc = 0; kc < nch; kc++) {
+                    if (!mbar_wait_spin(&s.full[st], ph & 1, abort, limit_ns, status, K_LOGP, 10)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t ad = ad0 + st * ASTAGE, bd = bd0 + st * BSTAGE;
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; kk++)
+                        umma_f16_ss_pair(tb + a * BN, ad + kk * KSTEP, bd + kk * KSTEP, IDESC, (kc > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit_pair(empty0[0] + 8 * st);
+                    umma_commit_pair(empty0[1] + 8 * st);
+                    if (++st == NS) st = 0, ph++;
+                }
+                if (ok) {
+                    umma_commit_pair(accf0[0] + 8 * a);
+                    umma_commit_pair(accf0[1] + 8 * a);
+                }
+            }
+            umma_commit_pair(dsmem_addr(&s.fin, 0));  // both CTAs: every MMA issued above has finished
+            umma_commit_pair(dsmem_addr(&s.fin, 1));
+        }
+    } else {
+        // ---------------------------------------------------------------- epilogue: thread = row, half of a tile's ids
+        const int qd = warp & 3, half = (warp - 2) >> 2;  // the TMEM lane quarter this warp may read
+        const int col = (int)row_at(o, 0), lrow = (int)rank * BMC + qd * 32 + lane;  // row of the tile
+        const uint32_t tl = tb + ((uint32_t)(qd * 32) << 16) + half * (BN / 2);
+        const uint32_t acce0 = dsmem_addr(&s.acce[0], 0);
+        RowState r;
+        r.clear();
+        int m = -1, target = -1;  // row tile
+        auto finish = [&]() {
+            if (m < 0 || m * 2 * BMC + lrow >= rows || col < 0) return;
+            const int k = pid - share.owner(m * nt);  // this pair's part of the row tile
+            r.store(rec + ((((long)m * parts + k) * 2 + half) * FIELDS) * 2 * BMC + lrow, 2 * BMC, o.top);
+        };
+        for (int i = 0; i < my; i++) {
+            const int a = i & 1, n0 = (t0 + i) % nt * BN + half * (BN / 2);
+            if ((t0 + i) / nt != m) {
+                finish();
+                m = (t0 + i) / nt;
+                r.clear();
+                const int row = m * 2 * BMC + lrow;
+                target = row < rows && o.target && col >= 0 ? o.target[row_at(o, row)] : -1;
+            }
+            const bool ok =
+                __all_sync(0xffffffff, mbar_wait_spin(&s.accf[a], (i >> 1) & 1, abort, limit_ns, status, K_LOGP, 11));
+            if (ok && m * 2 * BMC + (int)rank * BMC + qd * 32 < rows) {
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < BN / 64; c++) {
+                    const uint32_t out = left_out(sup, n0 + 32 * c, V, lane);
+                    uint32_t acc[32];
+                    __syncwarp();
+                    tmem_ld32(tl + a * BN + 32 * c, acc);
+                    if (out != 0xffffffffu) r.take(acc, n0 + 32 * c, out, target, o.top, s.box[warp - 2], lane);
+                }
+                tc_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) {
+                if (lead) mbar_arrive(&s.acce[a]);
+                else mbar_arrive_remote(acce0 + 8 * a);
+            }
+        }
+        finish();
+    }
+    // teardown: every MMA into either CTA's TMEM has finished before the pair releases it, and neither CTA leaves while
+    // the other may still signal its barriers
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        mbar_wait(&s.fin, 0, nullptr, limit_ns, status, K_LOGP, 12);
+        __syncwarp();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tb, 2 * BN);
+}
+
+// A warp to a row: its records joined, the outputs written. Row r has records at rec + part(r)'s; tile rows `tr` (128 or
+// 256), `bn` ids to a vocabulary tile, `halves` records to a worker and row tile
+__global__ void __launch_bounds__(128) linear_join_kernel(const float* rec, int rows, int V, int tr, int bn, int halves,
+                                                          int workers, int parts, LogpOut o) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5);
+    griddep_wait();
+    griddep_launch_dependents();
+    if (row >= rows) return;
+    const long at = row_at(o, row);
+    if (at < 0) return;
+    const int mt = (rows + tr - 1) / tr, nt = (V + bn - 1) / bn, m = row / tr;
+    const Share share(mt * nt, workers);
+    const int w0 = share.owner(m * nt), n = (share.owner((m + 1) * nt - 1) - w0 + 1) * halves;
+    const float* base = rec + (long)m * parts * halves * FIELDS * tr + row % tr;
+    const int t = o.target ? o.target[at] : -1;
+    const bool has = t >= 0 && t < V;
+    float tgt = 0.f;
+    if (has) {
+        const int k = (share.owner(m * nt + t / bn) - w0) * halves + t % bn / (bn / halves);
+        tgt = base[((long)k * FIELDS + 3) * tr];
+    }
+    RowStat a = stat_none();
+    unsigned long long best[TOP_MAX] = {};
+    for (int k = lane; k < n; k += 32) {
+        const float* f = base + (long)k * FIELDS * tr;
+        a = stat_join(a, {f[0], f[tr], f[2l * tr]});
+        for (int i = 0; i < o.top; i++) {
+            unsigned long long key = top_key(f[(4l + i) * tr], __float_as_int(f[(4l + TOP_MAX + i) * tr]));
+            if (key <= best[TOP_MAX - 1]) break;  // a record's come in order
+#pragma unroll
+            for (int j = 0; j < TOP_MAX; j++)
+                if (key > best[j]) {
+                    const unsigned long long x = best[j];
+                    best[j] = key;
+                    key = x;
+                }
+        }
+    }
+#pragma unroll
+    for (int w = 16; w; w >>= 1)
+        a = stat_join(a, {__shfl_xor_sync(0xffffffff, a.m, w), __shfl_xor_sync(0xffffffff, a.s, w),
+                          __shfl_xor_sync(0xffffffff, a.u, w)});
+    float lse = 0.f;
+    if (lane == 0) lse = store_row(o, at, a, has, tgt);
+    lse = __shfl_sync(0xffffffff, lse, 0);
+    for (int i = 0; i < o.top; i++) {
+        unsigned long long x = best[0];
+#pragma unroll
+        for (int w = 16; w; w >>= 1) {
+            const unsigned long long y = __shfl_xor_sync(0xffffffff, x, w);
+            x = y > x ? y : x;
+        }
+        if (lane == 0) store_top(o, at, i, x, lse);
+        if (best[0] == x && x) {  // one lane's: the next of its own
+#pragma unroll
+            for (int j = 0; j + 1 < TOP_MAX; j++) best[j] = best[j + 1];
+            best[TOP_MAX - 1] = 0ull;
+        }
+    }
+}
+
+// the layout of a call, from its sizes
+namespace {
+struct Plan {
+    bool pairs;
+    int tr, bn, halves, workers, parts;
+    size_t bytes;
+};
+Plan plan(int rows, int V) {
+    Plan p;
+    p.pairs = rows > 128;
+    p.tr = p.pairs ? 256 : 128, p.bn = p.pairs ? pair::BN : one::BN, p.halves = p.pairs ? 2 : 1;
+    const int mt = (rows + p.tr - 1) / p.tr, nt = (V + p.bn - 1) / p.bn, most = p.pairs ? PAIRS : 2 * PAIRS;
+    const long T = (long)mt * nt;
+    p.workers = (int)(T < most ? T : most);
+    const int per = (int)(T / p.workers);
+    p.parts = (nt + per - 1) / per + 1;  // workers that a row tile's vocabulary can lie on
+    if (p.parts > p.workers) p.parts = p.workers;
+    p.bytes = (size_t)mt * p.parts * p.halves * FIELDS * p.tr * 4;
+    return p;
+}
+}  // namespace
+
+size_t linear_logprobs_scratch_bytes(int rows, int V, int) { return plan(rows, V).bytes; }
 
 int launch_linear_logprobs(const void* x, long long ldx, const void* emb, int rows, int V, int d,
                            const unsigned char* sup, const LogpOut& o, void* scratch, size_t scratch_bytes,
                            cudaStream_t st) {
     if (rows < 0 || V < 1 || d < 64 || d % 64) return fail("linear_logprobs: rows >= 0, vocab >= 1, width a multiple of 64");
+    if (V > 0x7ffffc00 || rows > 0x7ffffc00) return fail("linear_logprobs: vocab and rows up to 2^31 - 1024");
     if (logp_check("linear_logprobs", o)) return -1;
     if (rows == 0) return 0;
     if (!x || !emb || (((uintptr_t)x | (uintptr_t)emb) & 15) || (ldx & 7) || ldx < d)
         return fail("linear_logprobs: x and emb 16-byte aligned, ldx >= width with a 16-byte row pitch");
-    const size_t need = linear_logprobs_scratch_bytes(rows, V, d);
-    if (need && (!scratch || ((uintptr_t)scratch & 15) || scratch_bytes < need))
+    const long tiles = ((long)rows + 127) / 128 * (((long)V + 127) / 128);
+    if (tiles > 0x7fffffffl) return fail("linear_logprobs: more than 2^31 tiles in one call");
+    const Plan p = plan(rows, V);
+    if (!scratch || ((uintptr_t)scratch & 15) || scratch_bytes < p.bytes)
         return fail("linear_logprobs: scratch too small or not 16-byte aligned");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
-    const dim3 grid((V + ll::T - 1) / ll::T, (rows + ll::T - 1) / ll::T);
-    if (grid.y > 65535) return fail("linear_logprobs: too many rows in one call");
-    if (check_pdl(launch_pdl(linear_kernel, grid, dim3(256), 0, st, (const h16*)x, (long)ldx, (const h16*)emb, rows, V, d,
-                             (float*)scratch),
-                  "linear_logprobs"))
-        return -1;
-    return launch_token_logprobs(scratch, V, 1, rows, V, sup, o, st);
+    CUtensorMap xm, em;
+    const int xbox = p.pairs ? 128 : (rows + 7) / 8 * 8;
+    const uint64_t xd[2] = {(uint64_t)d, (uint64_t)rows}, xs[1] = {(uint64_t)ldx * 2};
+    const uint32_t xb[2] = {BK, (uint32_t)xbox};
+    const uint64_t ed[2] = {(uint64_t)d, (uint64_t)V}, es[1] = {(uint64_t)d * 2};
+    const uint32_t eb[2] = {BK, 128};
+    if (make_tmap_2d(&xm, x, xd, xs, xb, 128) || make_tmap_2d(&em, emb, ed, es, eb, 128))
+        return fail("linear_logprobs: cuTensorMapEncodeTiled failed");
+    float* rec = (float*)scratch;
+    const int e = p.pairs
+                      ? check_pdl(launch_pdl(linear_pair_kernel, dim3(2 * p.workers), dim3(pair::NTHREADS),
+                                             sizeof(pair::Smem) + 1024, st, xm, em, rows, V, d, p.parts, sup, o, rec,
+                                             dc.status, dc.limit_ns),
+                                  "linear_logprobs")
+                      : check_pdl(launch_pdl(linear_one_kernel, dim3(p.workers), dim3(one::NTHREADS),
+                                             sizeof(one::Smem) + 1024, st, xm, em, rows, V, d, xbox, sup, o, rec,
+                                             dc.status, dc.limit_ns),
+                                  "linear_logprobs");
+    if (e) return e;
+    return check_pdl(launch_pdl(linear_join_kernel, dim3((rows + 3) / 4), dim3(128), 0, st, (const float*)rec, rows, V, p.tr,
+                                p.bn, p.halves, p.workers, p.parts, o),
+                     "linear_logprobs");
+}
+
+void init_linear_logprobs_attrs() {
+    cudaFuncSetAttribute(linear_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(one::Smem) + 1024);
+    cudaFuncSetAttribute(linear_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(pair::Smem) + 1024);
 }
 
 }  // namespace mmz

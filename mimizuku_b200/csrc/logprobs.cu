@@ -21,7 +21,6 @@ constexpr int NT = 256, NW = NT / 32, NG = 16;  // threads that sum, their warps
 constexpr int NS = 6, CB = 16384;               // stages and bytes of the ring
 constexpr int PIECES = CB / 16;                 // 16-byte pieces of a stage: 4 to a thread
 constexpr int LIST = 1024;                      // candidates of a CTA
-constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.4426950408889634f;
 
 struct Smem {
     uint8_t ring[NS][CB];
@@ -34,12 +33,6 @@ struct Smem {
 };
 
 __device__ __forceinline__ void sync_sums() { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); }
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 
 // the logits of a 16-byte piece: 8 of fp16, 4 of fp32
 template <typename T>
@@ -80,42 +73,6 @@ __device__ __forceinline__ unsigned long long mask_of(const unsigned char* sup, 
     return m;
 }
 
-// a thread's running maximum and sums; m starts at the lowest finite number, so that -inf adds e^(-inf) = 0 to every sum
-struct Run {
-    float m;
-    float2 s, u;
-    __device__ __forceinline__ void raise(float to) {
-        if (to > m) {
-            const float d = fmaxf(m - to, -200.f), e = ex2_approx(d * LOG2E);  // below e^-200 nothing is left
-            u = ffma2(make_float2(d, d), s, u);
-            u = make_float2(u.x * e, u.y * e);
-            s = make_float2(s.x * e, s.y * e);
-            m = to;
-        }
-    }
-    __device__ __forceinline__ void add2(float a, float b) {
-        float2 d = fadd2(make_float2(a, b), make_float2(-m, -m));
-        d.x = max_nan(d.x, -200.f), d.y = max_nan(d.y, -200.f);  // a NaN stays; e = 0 for all that is cut
-        const float2 e = make_float2(ex2_approx(d.x * LOG2E), ex2_approx(d.y * LOG2E));
-        s = fadd2(s, e);
-        u = ffma2(e, d, u);
-    }
-    // K pieces of N logits: one look at the maximum, two sets of sums
-    template <int K, int N>
-    __device__ __forceinline__ void add(const float (&x)[K][N], float h) {  // h: the largest of x
-        raise(h);
-        Run other{m, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int k = 0; k < K; k++)
-#pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                add2(x[k][i], x[k][i + 1]);
-                other.add2(x[k][i + 2], x[k][i + 3]);
-            }
-        s = fadd2(s, other.s);
-        u = fadd2(u, other.u);
-    }
-};
 }  // namespace lp
 using namespace lp;
 

@@ -37,6 +37,50 @@ __device__ __forceinline__ void stat_add(RowStat& a, float x) {
     }
 }
 
+constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// a thread's running maximum and sums; m starts at the lowest finite number, so that -inf adds e^(-inf) = 0 to every sum
+struct Run {
+    float m;
+    float2 s, u;
+    __device__ __forceinline__ void raise(float to) {
+        if (to > m) {
+            const float d = fmaxf(m - to, -200.f), e = ex2_approx(d * LOG2E);  // below e^-200 nothing is left
+            u = ffma2(make_float2(d, d), s, u);
+            u = make_float2(u.x * e, u.y * e);
+            s = make_float2(s.x * e, s.y * e);
+            m = to;
+        }
+    }
+    __device__ __forceinline__ void add2(float a, float b) {
+        float2 d = fadd2(make_float2(a, b), make_float2(-m, -m));
+        d.x = max_nan(d.x, -200.f), d.y = max_nan(d.y, -200.f);  // a NaN stays; e = 0 for all that is cut
+        const float2 e = make_float2(ex2_approx(d.x * LOG2E), ex2_approx(d.y * LOG2E));
+        s = fadd2(s, e);
+        u = ffma2(e, d, u);
+    }
+    // K pieces of N logits: one look at the maximum, two sets of sums
+    template <int K, int N>
+    __device__ __forceinline__ void add(const float (&x)[K][N], float h) {  // h: the largest of x
+        raise(h);
+        Run other{m, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                add2(x[k][i], x[k][i + 1]);
+                other.add2(x[k][i + 2], x[k][i + 3]);
+            }
+        s = fadd2(s, other.s);
+        u = fadd2(u, other.u);
+    }
+};
 // (value, lower id first) as one unsigned comparison; 0 stands for no candidate. -0 counts as +0. A NaN and -inf are no
 // candidates.
 __device__ __forceinline__ unsigned long long top_key(float v, int id) {

@@ -77,6 +77,7 @@ static void init_ctx(DevCtx& c, int dev) {
     init_align_attrs();
     init_attn8_attrs();
     init_logprobs_attrs();
+    init_linear_logprobs_attrs();
     cudaGetLastError();
     c.ok = true;
     c.err = "";

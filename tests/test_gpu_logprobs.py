@@ -223,7 +223,8 @@ def grid_states(gen, rows, V, d):
 
 HIDDEN = [(1, 1, 64, 1), (2, 5, 64, 8), (1, 51865, 384, 5), (3, 1000, 128, 5), (32, 3001, 1280, 8), (33, 2000, 192, 0),
           (31, 131, 64, 3), (64, 700, 64, 2), (100, 5000, 384, 5), (128, 257, 64, 8), (129, 1024, 256, 5),
-          (257, 777, 64, 5), (1000, 2049, 128, 4), (300, 20000, 64, 5), (8, 60000, 64, 5), (513, 256, 1280, 5)]
+          (257, 777, 64, 5), (1000, 2049, 128, 4), (300, 20000, 64, 5), (8, 60000, 64, 5), (513, 256, 1280, 5),
+          (20000, 600, 64, 3), (3000, 3001, 64, 8), (130, 51866, 384, 5)]
 
 
 @pytest.mark.parametrize("shape", HIDDEN)
