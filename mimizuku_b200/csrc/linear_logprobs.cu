@@ -5,13 +5,16 @@
 // D[rows][vocabulary ids], so that a thread of the epilogue has a row: one TMEM lane, 32 ids at a time. Per id it does
 // what token_logprobs does (packed fp32, one exponential); where a chunk of 32 has a logit above the row's last
 // alternative, or the target, the warp puts the chunk into shared memory and each lane picks its own out. Each CTA (or
-// pair) has an equal share of the (row tile, vocabulary tile) sequence, vocabulary innermost, and leaves one record per
-// row tile it worked on; a second kernel joins the records of a row.
-//   up to 128 rows   linear_one_kernel: tiles of 128 rows x 128 ids, a CTA to an SM. Bound by reading the embedding once
-//                    (the rows are zero-padded to 128 in the product, but only loaded to the next 8)
+// pair) has an equal share of the (row tile, vocabulary) sequence, vocabulary innermost, and leaves one record per row
+// tile it worked on; a second kernel joins the records of a row.
+//   up to 32 rows    linear_one_kernel<true>: 128 rows (32 loaded, the rest of the product is not looked at) x up to 128
+//                    ids, a CTA to an SM, shares in units of 32 ids. One warp can read the 32 rows' TMEM lanes: it
+//                    hands the chunks to the four warps of the epilogue through shared memory
+//   up to 128        linear_one_kernel<false>: the same, each of the four warps with its 32 rows
+//                    Both are bound by reading the embedding once
 //   more             linear_pair_kernel: tiles of 256 x 256 on pairs of CTAs (cta_group::2). Bound by the tensor cores
 //                    (at a width of 1280 a tile's products take about five times its epilogue)
-// Both: a TMA producer and an MMA issuer (one warp each) feed two TMEM accumulators in turn, the epilogue works on one
+// All: a TMA producer and an MMA issuer (one warp each) feed two TMEM accumulators in turn, the epilogue works on one
 // while the other fills. Every wait is bounded; a CTA that gives up lets its copies land, waits for its MMAs and frees its
 // TMEM.
 #include "launch.h"
@@ -21,7 +24,7 @@ namespace mmz {
 namespace ll {
 
 constexpr int BK = 64;              // K per stage (one 128-byte swizzle atom)
-constexpr int FIELDS = 4 + 2 * TOP_MAX;  // a record's fields: m, s, u, the target's logit, alternatives' logits and ids
+constexpr int FIELDS = 4 + 2 * TOP_MAX;  // a record: m, s, u, the target's logit, (logit, id) of the alternatives
 constexpr int PAIRS = 74;           // pairs of SMs of a B200
 
 // equal contiguous shares of T tiles for W workers, the first T % W have one more
@@ -60,31 +63,41 @@ struct RowState {
         for (int i = 1; i < TOP_MAX; i++)
             if (i < top) kth = v[i];
     }
-    // 32 logits of ids c0 .. c0 + 31, those with a bit in `out` left out; box: the warp's [32 ids][32 lanes] floats
-    __device__ __forceinline__ void take(const uint32_t (&acc)[32], int c0, uint32_t out, int target, int top, float* box,
-                                         int lane) {
-        float x[1][32];
-#pragma unroll
-        for (int i = 0; i < 32; i++) x[0][i] = __uint_as_float(acc[i]);
+    // 32 logits of ids c0 .. c0 + 31, those with a bit in `out` left out; box: [32 ids][32 lanes] floats of the warp, which
+    // hold the logits already where STORED
+    template <bool STORED>
+    __device__ __forceinline__ void take(float (&x)[1][32], int c0, uint32_t out, int target, int top, float* box, int lane) {
         if (out) {
 #pragma unroll
             for (int i = 0; i < 32; i++)
                 if (out >> i & 1) x[0][i] = -INFINITY;
         }
-        float h = fmax3(x[0][0], x[0][1], x[0][2]);
+        float g[8];  // the largest of each four
 #pragma unroll
-        for (int i = 3; i < 31; i += 2) h = fmax3(h, x[0][i], x[0][i + 1]);
-        h = fmaxf(h, x[0][31]);
+        for (int i = 0; i < 8; i++) g[i] = fmaxf(fmax3(x[0][4 * i], x[0][4 * i + 1], x[0][4 * i + 2]), x[0][4 * i + 3]);
+        const float h = fmaxf(fmax3(fmax3(g[0], g[1], g[2]), g[3], g[4]), fmax3(g[5], g[6], g[7]));
         run.add(x, h);
         const bool mine = target >= c0 && target < c0 + 32, more = top > 0 && h > kth;
         if (!__any_sync(0xffffffff, mine || more)) return;
+        // an empty list: only what reaches the top-th largest of the fours' maxima can end up in it
+        float least = -INFINITY;
+        if (__any_sync(0xffffffff, more && kth == -INFINITY)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                int above = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (j != i) above += g[j] > g[i] || (j < i && g[j] == g[i]);
+                if (above == top - 1 && g[i] == g[i]) least = g[i];
+            }
+        }
         uint32_t cand = 0;
 #pragma unroll
         for (int i = 0; i < 32; i++) {
-            box[i * 32 + lane] = x[0][i];  // read by the same lane only
-            if (x[0][i] > kth) cand |= 1u << i;
+            if (!STORED) box[i * 32 + lane] = x[0][i];  // read by the same lane only
+            if (x[0][i] > kth && x[0][i] >= least) cand |= 1u << i;
         }
-        if (mine) tgt = box[(target - c0) * 32 + lane];
+        if (mine) tgt = out >> (target - c0) & 1 ? -INFINITY : box[(target - c0) * 32 + lane];
         if (top == 0) return;
         for (; cand; cand &= cand - 1) {
             const int i = __ffs(cand) - 1;
@@ -92,18 +105,30 @@ struct RowState {
             if (f > kth) insert(f, c0 + i, top);
         }
     }
-    // field k of the row's record at rec[k * rows]
-    __device__ __forceinline__ void store(float* rec, int rows, int top) const {
+    __device__ __forceinline__ RowStat stat() const {  // nothing above -inf: the empty set
         const float s = run.s.x + run.s.y;
-        rec[0] = s == 0.f ? -INFINITY : run.m;  // nothing above -inf: the empty set
-        rec[rows] = s;
-        rec[2l * rows] = run.u.x + run.u.y;
-        rec[3l * rows] = tgt;
+        return {s == 0.f ? -INFINITY : run.m, s, run.u.x + run.u.y};
+    }
+    __device__ __forceinline__ void store(float* rec, int top) const {
+        const RowStat a = stat();
+        float4* to = reinterpret_cast<float4*>(rec);
+        to[0] = make_float4(a.m, a.s, a.u, tgt);
 #pragma unroll
-        for (int i = 0; i < TOP_MAX; i++)
-            if (i < top) rec[(4l + i) * rows] = v[i], rec[(4l + TOP_MAX + i) * rows] = __int_as_float(id[i]);
+        for (int i = 0; i < TOP_MAX; i += 2)
+            if (i < top) to[1 + i / 2] = make_float4(v[i], __int_as_float(id[i]), v[i + 1], __int_as_float(id[i + 1]));
     }
 };
+
+// key among the eight largest in order
+__device__ __forceinline__ void put(unsigned long long (&best)[TOP_MAX], unsigned long long key) {
+#pragma unroll
+    for (int j = 0; j < TOP_MAX; j++)
+        if (key > best[j]) {
+            const unsigned long long x = best[j];
+            best[j] = key;
+            key = x;
+        }
+}
 
 // the ids c0 .. c0 + 31 that are left out: suppressed, or past the vocabulary
 __device__ __forceinline__ uint32_t left_out(const unsigned char* sup, int c0, int V, int lane) {
@@ -112,12 +137,14 @@ __device__ __forceinline__ uint32_t left_out(const unsigned char* sup, int c0, i
 }
 
 namespace one {
-constexpr int BM = 128, BN = 128, NS = 6, NTHREADS = 192;  // warps 0-3 epilogue, 4 TMA, 5 MMA
-constexpr int AT = BM * BK * 2, BT = BN * BK * 2;          // 16 KB each
-constexpr uint32_t IDESC = idesc_f16_f32(BM, BN, false);
+constexpr int BM = 128, NTHREADS = 192;   // warps 0-3 epilogue, 4 TMA, 5 MMA
+constexpr int UNIT = 32, UB = UNIT * BK * 2;  // ids and bytes (4 KB) of a unit; up to 4 units to a tile
+template <bool NARROW>
 struct Smem {
-    uint8_t a[NS][AT], b[NS][BT];
-    float box[4][32 * 32];
+    static constexpr int NS = NARROW ? 8 : 6, AT = NARROW ? 32 * BK * 2 : BM * BK * 2;
+    uint8_t a[NS][AT];  // NARROW: the product reads 128 rows from a stage's 32 on, what they hold is not looked at
+    uint8_t b[NS][4 * UB];
+    float box[NARROW ? 2 : 1][4][32 * 32];
     uint64_t full[NS], empty[NS], accf[2], acce[2], fin;
     uint32_t tmem;
     int abort;
@@ -139,18 +166,21 @@ struct Smem {
 }  // namespace ll
 using namespace ll;
 
-// grid min(SMs, tiles), block NTHREADS, dynamic shared memory sizeof(Smem) + 1024 (alignment slack). xbox: rows that a
-// load of x brings (a multiple of 8). rec [CTAs][FIELDS][128]
+// grid min(SMs, units of 32 ids), block NTHREADS, dynamic shared memory sizeof(Smem) + 1024 (alignment slack). xbox: rows
+// that a load of x brings (a multiple of 8); emap: a box of 32 ids. rec [CTAs][128][FIELDS]
+template <bool NARROW>
 __global__ void __launch_bounds__(one::NTHREADS, 1)
     linear_one_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap emap, int rows, int V,
                       int d, int xbox, const unsigned char* sup, LogpOut o, float* rec, unsigned* status,
                       unsigned long long limit_ns) {
     using namespace one;
+    using SM = Smem<NARROW>;
+    constexpr int NS = SM::NS;
     extern __shared__ uint8_t smem_raw[];
-    Smem& s = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
+    SM& s = *reinterpret_cast<SM*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
-    const Share share((V + BN - 1) / BN, gridDim.x);
-    const int t0 = share.first(cta), my = share.count(cta), nch = d / BK, nq = my * nch;
+    const Share share((V + UNIT - 1) / UNIT, gridDim.x);
+    const int u0 = share.first(cta), units = share.count(cta), my = (units + 3) / 4, nch = d / BK;
     volatile int* abort = &s.abort;
     if (warp == 4 && lane == 0) {
         s.abort = 0;
@@ -160,7 +190,7 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(&s.accf[a], 1);
-            mbar_init(&s.acce[a], 4);
+            mbar_init(&s.acce[a], NARROW ? 1 : 4);
         }
         mbar_init(&s.fin, 1);
         fence_mbar_init();
@@ -168,7 +198,7 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
         prefetch_tmap(&emap);
     }
     if (warp == 5) {
-        tmem_alloc(&s.tmem, 2 * BN);
+        tmem_alloc(&s.tmem, 256);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -180,14 +210,21 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
     if (warp == 4) {
         // ---------------------------------------------------------------- producer
         if (lane == 0) {
-            int issued = 0;
-            for (int q = 0; q < nq; q++) {
-                const int st = q % NS, i = q / nch, kc = q % nch;
-                if (q >= NS && !mbar_wait_spin(&s.empty[st], ((q / NS) - 1) & 1, abort, limit_ns, status, K_LOGP, 3)) break;
-                mbar_expect_tx(&s.full[st], BT + xbox * BK * 2);
-                tma_load_2d(s.b[st], &emap, kc * BK, (t0 + i) * BN, &s.full[st]);
-                tma_load_2d(s.a[st], &xmap, kc * BK, 0, &s.full[st]);
-                issued = q + 1;
+            int issued = 0, st = 0, ph = 0;  // ring slot and its use count
+            bool ok = true;
+            for (int i = 0; ok && i < my; i++) {
+                const int n = min(4, units - 4 * i), id0 = (u0 + 4 * i) * UNIT;
+                for (int kc = 0; kc < nch; kc++) {
+                    if (issued >= NS && !mbar_wait_spin(&s.empty[st], (ph - 1) & 1, abort, limit_ns, status, K_LOGP, 3)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_expect_tx(&s.full[st], n * UB + xbox * BK * 2);
+                    for (int u = 0; u < n; u++) tma_load_2d(s.b[st] + u * UB, &emap, kc * BK, id0 + u * UNIT, &s.full[st]);
+                    tma_load_2d(s.a[st], &xmap, kc * BK, 0, &s.full[st]);
+                    issued++;
+                    if (++st == NS) st = 0, ph++;
+                }
             }
             if (*abort)  // let every issued copy land before the shared memory is released
                 for (int q = issued > NS ? issued - NS : 0; q < issued; q++)
@@ -197,24 +234,26 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
         // ---------------------------------------------------------------- MMA issuer
         if (lane == 0) {
             const uint64_t ad0 = sdesc_sw128(smem_u32(s.a[0]), 16, 1024), bd0 = sdesc_sw128(smem_u32(s.b[0]), 16, 1024);
-            constexpr uint64_t ASTAGE = AT >> 4, BSTAGE = BT >> 4, KSTEP = 32 >> 4;
+            constexpr uint64_t ASTAGE = SM::AT >> 4, BSTAGE = 4 * UB >> 4, KSTEP = 32 >> 4;
             bool ok = true;
-            for (int i = 0, q = 0; ok && i < my; i++) {
+            int st = 0, ph = 0;
+            for (int i = 0; ok && i < my; i++) {
                 const int a = i & 1;
+                const uint32_t idesc = idesc_f16_f32(BM, UNIT * min(4, units - 4 * i), false);
                 if (i >= 2 && !mbar_wait_spin(&s.acce[a], ((i >> 1) - 1) & 1, abort, limit_ns, status, K_LOGP, 4)) break;
                 tc_fence_after();
-                for (int kc = 0; kc < nch; kc++, q++) {
-                    const int st = q % NS;
-                    if (!mbar_wait_spin(&s.full[st], (q / NS) & 1, abort, limit_ns, status, K_LOGP, 5)) {
+                for (int kc = 0; kc < nch; kc++) {
+                    if (!mbar_wait_spin(&s.full[st], ph & 1, abort, limit_ns, status, K_LOGP, 5)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; kk++)
-                        umma_f16_ss(tb + a * BN, ad0 + st * ASTAGE + kk * KSTEP, bd0 + st * BSTAGE + kk * KSTEP, IDESC,
+                        umma_f16_ss(tb + a * 128, ad0 + st * ASTAGE + kk * KSTEP, bd0 + st * BSTAGE + kk * KSTEP, idesc,
                                     (kc > 0 || kk > 0) ? 1u : 0u);
                     umma_commit(&s.empty[st]);
+                    if (++st == NS) st = 0, ph++;
                 }
                 if (ok) umma_commit(&s.accf[a]);
             }
@@ -222,32 +261,102 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
         }
     } else {
         // ---------------------------------------------------------------- epilogue: thread = row
-        const int row = warp * 32 + lane, col = (int)row_at(o, 0);
-        const bool live = warp * 32 < rows && col >= 0;
+        const int row = NARROW ? lane : warp * 32 + lane, col = (int)row_at(o, 0);
+        const bool live = (NARROW || warp * 32 < rows) && col >= 0;
         const int target = live && row < rows && o.target ? o.target[row_at(o, row)] : -1;
-        const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);
+        const uint32_t tl = tb + ((uint32_t)(NARROW ? 0 : warp * 32) << 16);
         RowState r;
         r.clear();
         for (int i = 0; i < my; i++) {
-            const int a = i & 1, n0 = (t0 + i) * BN;
-            const bool ok =
-                __all_sync(0xffffffff, mbar_wait_spin(&s.accf[a], (i >> 1) & 1, abort, limit_ns, status, K_LOGP, 6));
-            if (ok && live) {
-                tc_fence_after();
+            const int a = i & 1, n = min(4, units - 4 * i), id0 = (u0 + 4 * i) * UNIT;
+            if (NARROW) {
+                // warp 0 hands the tile's chunks round, one to a warp; every warp reaches the barrier of every tile
+                float(*box)[32 * 32] = s.box[a];
+                if (warp == 0) {
+                    const bool ok = __all_sync(
+                        0xffffffff, mbar_wait_spin(&s.accf[a], (i >> 1) & 1, abort, limit_ns, status, K_LOGP, 6));
+                    if (ok) {
+                        tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < BN / 32; c++) {
-                    const uint32_t out = left_out(sup, n0 + 32 * c, V, lane);
-                    uint32_t acc[32];
+                        for (int u = 0; u < n; u++) {
+                            uint32_t acc[32];
+                            __syncwarp();
+                            tmem_ld32(tl + a * 128 + 32 * u, acc);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) box[u][k * 32 + lane] = __uint_as_float(acc[k]);
+                        }
+                        tc_fence_before();
+                    }
                     __syncwarp();
-                    tmem_ld32(tl + a * BN + 32 * c, acc);
-                    if (out != 0xffffffffu) r.take(acc, n0 + 32 * c, out, target, o.top, s.box[warp], lane);
+                    if (lane == 0) mbar_arrive(&s.acce[a]);
                 }
-                tc_fence_before();
+                asm volatile("bar.sync 1, 128;" ::: "memory");  // the boxes of two tiles: written again after the next one's
+                if (live && warp < n) {
+                    const uint32_t out = left_out(sup, id0 + UNIT * warp, V, lane);
+                    float x[1][32];
+#pragma unroll
+                    for (int k = 0; k < 32; k++) x[0][k] = box[warp][k * 32 + lane];
+                    if (out != 0xffffffffu) r.take<true>(x, id0 + UNIT * warp, out, target, o.top, box[warp], lane);
+                }
+            } else {
+                const bool ok =
+                    __all_sync(0xffffffff, mbar_wait_spin(&s.accf[a], (i >> 1) & 1, abort, limit_ns, status, K_LOGP, 6));
+                if (ok && live) {
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int u = 0; u < n; u++) {
+                        const uint32_t out = left_out(sup, id0 + UNIT * u, V, lane);
+                        uint32_t acc[32];
+                        __syncwarp();
+                        tmem_ld32(tl + a * 128 + 32 * u, acc);
+                        float x[1][32];
+#pragma unroll
+                        for (int k = 0; k < 32; k++) x[0][k] = __uint_as_float(acc[k]);
+                        if (out != 0xffffffffu) r.take<false>(x, id0 + UNIT * u, out, target, o.top, s.box[0][warp], lane);
+                    }
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.acce[a]);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.acce[a]);
         }
-        if (live && row < rows) r.store(rec + (long)cta * FIELDS * BM + row, BM, o.top);
+        float* to = rec + ((long)cta * BM + row) * FIELDS;
+        if (!NARROW) {
+            if (live && row < rows) r.store(to, o.top);
+        } else {
+            // the four warps' parts of a row joined by warp 0
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            float* mine = &s.box[0][0][0] + (warp * 32 + lane) * FIELDS;  // 16-byte aligned
+            r.store(mine, o.top);
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (warp == 0 && live && row < rows) {
+                RowStat a = r.stat();
+                float tgt = r.tgt;
+                unsigned long long best[TOP_MAX] = {};
+                for (int w = 0; w < 4; w++) {
+                    const float* f = mine + w * 32 * FIELDS;
+                    const float4 y = *reinterpret_cast<const float4*>(f);
+                    if (w) {
+                        a = stat_join(a, {y.x, y.y, y.z});
+                        if (tgt == -INFINITY) tgt = y.w;  // the warp that had the target has it
+                    }
+                    for (int i = 0; i < o.top; i++) {
+                        const unsigned long long key = top_key(f[4 + 2 * i], __float_as_int(f[5 + 2 * i]));
+                        if (key <= best[TOP_MAX - 1]) break;  // a warp's come in order
+                        put(best, key);
+                    }
+                }
+                float4* z = reinterpret_cast<float4*>(to);
+                z[0] = make_float4(a.m, a.s, a.u, tgt);
+#pragma unroll
+                for (int i = 0; i < TOP_MAX; i += 2)
+                    if (i < o.top) {
+                        const unsigned long long p = best[i], q = best[i + 1];
+                        z[1 + i / 2] = make_float4(p ? key_value(p) : -INFINITY, __int_as_float(key_id(p)),
+                                                   q ? key_value(q) : -INFINITY, __int_as_float(key_id(q)));
+                    }
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -255,12 +364,12 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
         mbar_wait(&s.fin, 0, nullptr, limit_ns, status, K_LOGP, 7);
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tb, 2 * BN);
+        tmem_dealloc(tb, 256);
     }
 }
 
 // grid 2 x pairs, cluster (2, 1, 1), block NTHREADS, dynamic shared memory sizeof(Smem) + 1024. emap: a box of 128 ids
-// (half of a tile's). rec [row tiles][parts][2 halves of a tile's ids][FIELDS][256]
+// (half of a tile's). rec [row tiles][parts][2 halves of a tile's ids][256][FIELDS]
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap emap, int rows, int V,
                        int d, int parts, const unsigned char* sup, LogpOut o, float* rec, unsigned* status,
@@ -273,7 +382,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
     const bool lead = rank == 0;
     const int pid = blockIdx.x / 2, nt = (V + BN - 1) / BN, mt = (rows + 2 * BMC - 1) / (2 * BMC);
     const Share share(mt * nt, gridDim.x / 2);
-    const int t0 = share.first(pid), my = share.count(pid), nch = d / BK, nq = my * nch;
+    const int t0 = share.first(pid), my = share.count(pid), nch = d / BK;
     volatile int* abort = &s.abort;
     if (warp == 0 && lane == 0) {
         s.abort = 0;
@@ -374,7 +483,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
         auto finish = [&]() {
             if (m < 0 || m * 2 * BMC + lrow >= rows || col < 0) return;
             const int k = pid - share.owner(m * nt);  // this pair's part of the row tile
-            r.store(rec + ((((long)m * parts + k) * 2 + half) * FIELDS) * 2 * BMC + lrow, 2 * BMC, o.top);
+            r.store(rec + ((((long)m * parts + k) * 2 + half) * 2 * BMC + lrow) * FIELDS, o.top);
         };
         for (int i = 0; i < my; i++) {
             const int a = i & 1, n0 = (t0 + i) % nt * BN + half * (BN / 2);
@@ -395,7 +504,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
                     uint32_t acc[32];
                     __syncwarp();
                     tmem_ld32(tl + a * BN + 32 * c, acc);
-                    if (out != 0xffffffffu) r.take(acc, n0 + 32 * c, out, target, o.top, s.box[warp - 2], lane);
+                    float x[1][32];
+#pragma unroll
+                    for (int k = 0; k < 32; k++) x[0][k] = __uint_as_float(acc[k]);
+                    if (out != 0xffffffffu) r.take<false>(x, n0 + 32 * c, out, target, o.top, s.box[warp - 2], lane);
                 }
                 tc_fence_before();
             }
@@ -434,30 +546,31 @@ __global__ void __launch_bounds__(128) linear_join_kernel(const float* rec, int 
     const int mt = (rows + tr - 1) / tr, nt = (V + bn - 1) / bn, m = row / tr;
     const Share share(mt * nt, workers);
     const int w0 = share.owner(m * nt), n = (share.owner((m + 1) * nt - 1) - w0 + 1) * halves;
-    const float* base = rec + (long)m * parts * halves * FIELDS * tr + row % tr;
+    const float* base = rec + ((long)m * parts * halves * tr + row % tr) * FIELDS;
     const int t = o.target ? o.target[at] : -1;
     const bool has = t >= 0 && t < V;
     float tgt = 0.f;
     if (has) {
         const int k = (share.owner(m * nt + t / bn) - w0) * halves + t % bn / (bn / halves);
-        tgt = base[((long)k * FIELDS + 3) * tr];
+        tgt = base[(long)k * tr * FIELDS + 3];
     }
     RowStat a = stat_none();
     unsigned long long best[TOP_MAX] = {};
     for (int k = lane; k < n; k += 32) {
-        const float* f = base + (long)k * FIELDS * tr;
-        a = stat_join(a, {f[0], f[tr], f[2l * tr]});
-        for (int i = 0; i < o.top; i++) {
-            unsigned long long key = top_key(f[(4l + i) * tr], __float_as_int(f[(4l + TOP_MAX + i) * tr]));
-            if (key <= best[TOP_MAX - 1]) break;  // a record's come in order
+        const float4* f = reinterpret_cast<const float4*>(base + (long)k * tr * FIELDS);
+        const float4 y = f[0];
+        float4 z[TOP_MAX / 2];
 #pragma unroll
-            for (int j = 0; j < TOP_MAX; j++)
-                if (key > best[j]) {
-                    const unsigned long long x = best[j];
-                    best[j] = key;
-                    key = x;
-                }
-        }
+        for (int i = 0; i < TOP_MAX / 2; i++)
+            if (2 * i < o.top) z[i] = f[1 + i];
+        a = stat_join(a, {y.x, y.y, y.z});
+#pragma unroll
+        for (int i = 0; i < TOP_MAX; i++)
+            if (i < o.top) {
+                const float4 q = z[i / 2];
+                const unsigned long long key = i & 1 ? top_key(q.z, __float_as_int(q.w)) : top_key(q.x, __float_as_int(q.y));
+                if (key > best[TOP_MAX - 1]) put(best, key);
+            }
     }
 #pragma unroll
     for (int w = 16; w; w >>= 1)
@@ -486,13 +599,13 @@ __global__ void __launch_bounds__(128) linear_join_kernel(const float* rec, int 
 namespace {
 struct Plan {
     bool pairs;
-    int tr, bn, halves, workers, parts;
+    int tr, bn, halves, workers, parts;  // rows of a tile, ids of a unit of work, records to a worker and row tile
     size_t bytes;
 };
 Plan plan(int rows, int V) {
     Plan p;
     p.pairs = rows > 128;
-    p.tr = p.pairs ? 256 : 128, p.bn = p.pairs ? pair::BN : one::BN, p.halves = p.pairs ? 2 : 1;
+    p.tr = p.pairs ? 256 : 128, p.bn = p.pairs ? pair::BN : one::UNIT, p.halves = p.pairs ? 2 : 1;
     const int mt = (rows + p.tr - 1) / p.tr, nt = (V + p.bn - 1) / p.bn, most = p.pairs ? PAIRS : 2 * PAIRS;
     const long T = (long)mt * nt;
     p.workers = (int)(T < most ? T : most);
@@ -523,23 +636,29 @@ int launch_linear_logprobs(const void* x, long long ldx, const void* emb, int ro
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     CUtensorMap xm, em;
-    const int xbox = p.pairs ? 128 : (rows + 7) / 8 * 8;
+    const int xbox = p.pairs ? 128 : rows <= 32 ? 32 : (rows + 7) / 8 * 8;
     const uint64_t xd[2] = {(uint64_t)d, (uint64_t)rows}, xs[1] = {(uint64_t)ldx * 2};
     const uint32_t xb[2] = {BK, (uint32_t)xbox};
     const uint64_t ed[2] = {(uint64_t)d, (uint64_t)V}, es[1] = {(uint64_t)d * 2};
-    const uint32_t eb[2] = {BK, 128};
+    const uint32_t eb[2] = {BK, p.pairs ? 128u : (uint32_t)one::UNIT};
     if (make_tmap_2d(&xm, x, xd, xs, xb, 128) || make_tmap_2d(&em, emb, ed, es, eb, 128))
         return fail("linear_logprobs: cuTensorMapEncodeTiled failed");
     float* rec = (float*)scratch;
-    const int e = p.pairs
-                      ? check_pdl(launch_pdl(linear_pair_kernel, dim3(2 * p.workers), dim3(pair::NTHREADS),
-                                             sizeof(pair::Smem) + 1024, st, xm, em, rows, V, d, p.parts, sup, o, rec,
-                                             dc.status, dc.limit_ns),
-                                  "linear_logprobs")
-                      : check_pdl(launch_pdl(linear_one_kernel, dim3(p.workers), dim3(one::NTHREADS),
-                                             sizeof(one::Smem) + 1024, st, xm, em, rows, V, d, xbox, sup, o, rec,
-                                             dc.status, dc.limit_ns),
-                                  "linear_logprobs");
+    int e;
+    if (p.pairs)
+        e = check_pdl(launch_pdl(linear_pair_kernel, dim3(2 * p.workers), dim3(pair::NTHREADS), sizeof(pair::Smem) + 1024, st,
+                                 xm, em, rows, V, d, p.parts, sup, o, rec, dc.status, dc.limit_ns),
+                      "linear_logprobs");
+    else if (rows <= 32)
+        e = check_pdl(launch_pdl(linear_one_kernel<true>, dim3(p.workers), dim3(one::NTHREADS),
+                                 sizeof(one::Smem<true>) + 1024, st, xm, em, rows, V, d, xbox, sup, o, rec, dc.status,
+                                 dc.limit_ns),
+                      "linear_logprobs");
+    else
+        e = check_pdl(launch_pdl(linear_one_kernel<false>, dim3(p.workers), dim3(one::NTHREADS),
+                                 sizeof(one::Smem<false>) + 1024, st, xm, em, rows, V, d, xbox, sup, o, rec, dc.status,
+                                 dc.limit_ns),
+                      "linear_logprobs");
     if (e) return e;
     return check_pdl(launch_pdl(linear_join_kernel, dim3((rows + 3) / 4), dim3(128), 0, st, (const float*)rec, rows, V, p.tr,
                                 p.bn, p.halves, p.workers, p.parts, o),
@@ -547,8 +666,12 @@ int launch_linear_logprobs(const void* x, long long ldx, const void* emb, int ro
 }
 
 void init_linear_logprobs_attrs() {
-    cudaFuncSetAttribute(linear_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(one::Smem) + 1024);
-    cudaFuncSetAttribute(linear_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(pair::Smem) + 1024);
+    auto set = [](auto* fn, size_t bytes) {
+        cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes + 1024);
+    };
+    set(linear_one_kernel<true>, sizeof(one::Smem<true>));
+    set(linear_one_kernel<false>, sizeof(one::Smem<false>));
+    set(linear_pair_kernel, sizeof(pair::Smem));
 }
 
 }  // namespace mmz

@@ -263,6 +263,39 @@ def test_hidden_states_ties_and_rows_that_repeat(cuda):
         assert torch.equal(v[7], v[33])
 
 
+@pytest.mark.parametrize("rows", [3, 40, 200])
+def test_hidden_states_with_nan(cuda, rows):
+    """A NaN in an id's embedding makes every row's sums NaN and is no alternative; in a hidden state, that row's alone;
+    suppressed, it is not read into anything."""
+    gen = torch.Generator().manual_seed(15)
+    x, emb = grid_states(gen, rows, 700, 64)
+    emb[33, 5] = float("nan")
+    target = torch.full((rows,), 3, dtype=torch.int32)
+    logits = x.double().numpy() @ np.nan_to_num(emb.double().numpy()).T
+    logits[:, 33] = -np.inf
+    sup = torch.zeros(700, dtype=torch.uint8)
+    for top in (1, 5):
+        o = buffers(rows, top)
+        m.linear_logprobs(x.cuda(), emb.cuda(), target.cuda(), **o, sup=sup.cuda())
+        assert torch.isnan(torch.cat([o["lse"], o["logp"], o["entropy"]])).all()
+        assert np.array_equal(o["top_id"].cpu().numpy(), reference(logits, target.numpy(), None, top)[0]["top_id"])
+        sup[33] = 1
+        o = buffers(rows, top)
+        m.linear_logprobs(x.cuda(), emb.cuda(), target.cuda(), **o, sup=sup.cuda())
+        compare(o, reference(logits, target.numpy(), None, top), top)
+        sup[33] = 0
+    emb[33, 5] = 0
+    x[1, 7] = float("nan")
+    o = buffers(rows, 5)
+    m.linear_logprobs(x.cuda(), emb.cuda(), target.cuda(), **o)
+    x[1] = 0
+    want, tol, _ = reference(x.double().numpy() @ emb.double().numpy().T, target.numpy(), None, 5)
+    ok = torch.arange(rows) != 1
+    assert torch.isnan(o["lse"][1]) and (o["top_id"][1] == -1).all()
+    near(o["lse"][ok.cuda()], want["lse"][ok.numpy()], tol[ok.numpy()])
+    assert np.array_equal(o["top_id"].cpu().numpy()[ok.numpy()], want["top_id"][ok.numpy()])
+
+
 def test_hidden_states_beside_the_greedy_choice(cuda):
     """The engine's logits_argmax and the first alternative agree where the best two logits are a step of fp16 apart."""
     gen = torch.Generator().manual_seed(13)
