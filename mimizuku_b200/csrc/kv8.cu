@@ -37,17 +37,17 @@ using namespace kv8;
 template <int KIND>
 __global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* k, const h16* v, long x_seq,
                                                        long x_tok, long x_head, Cache c, const int* pos,
-                                                       int heads, int n, int cap, int block, int nblk, long items) {
+                                                       int heads, int n, int cap, int block, int nblk, unsigned items) {
     __shared__ float wmax[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int W = block <= 32 ? 1 : block / 32, tw = block < 32 ? block : 32;  // warps to an item, tokens to a warp
-    const long item = (long)blockIdx.x * (4 / W) + warp / W;
+    const unsigned item = blockIdx.x * (4 / W) + warp / W;
     griddep_wait();
+    griddep_launch_dependents();
     const bool live = item < items;
-    const int ib = (int)(live ? item % nblk : 0);
-    const long rest = live ? item / nblk : 0;
-    const int isv = (int)(rest & 1), hd = (int)((rest >> 1) % heads);
-    const long b = (rest >> 1) / heads;
+    const unsigned rest = live ? item / nblk : 0, pair = rest >> 1;
+    const int ib = live ? (int)(item - rest * nblk) : 0, isv = rest & 1, hd = pair % heads;
+    const long b = pair / heads;
     const int p0 = pos ? pos[b] : 0;
     // the first block with a new token at a position >= 0; blocks past the capacity or the last token have nothing
     const long first = p0 > 0 ? p0 / block : 0;
@@ -127,36 +127,47 @@ __global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* k, const h16* 
     }
 }
 
-// thread = 8 values of one token and head, of k and then of v
+// CTA: 128 tokens of one (sequence, head, k or v); 8 lanes to a token, 4 tokens of a thread in flight
 template <int KIND>
-__global__ void __launch_bounds__(256) kv8_read_kernel(Cache c, h16* k, h16* v, long y_seq,
-                                                       long y_tok, long y_head, const int* pos,
-                                                       const int* lens, int heads, int n, int cap,
-                                                       int block, long items) {
-    const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
+__global__ void __launch_bounds__(256) kv8_read_kernel(Cache c, h16* k, h16* v, long y_seq, long y_tok, long y_head,
+                                                       const int* pos, const int* lens, int heads, int n, int cap,
+                                                       int shift, unsigned tiles) {
+    const unsigned rest = blockIdx.x / tiles, tile = blockIdx.x - rest * tiles, pair = rest >> 1;
+    const int isv = rest & 1, hd = pair % heads, d0 = (threadIdx.x & 7) * 8;
+    const long b = pair / heads;
     griddep_wait();
-    if (i >= items) return;
-    const int d0 = (int)(i & 7) * 8;
-    long rest = i >> 3;
-    const int t = (int)(rest % n);
-    rest /= n;
-    const int isv = (int)(rest & 1), hd = (int)((rest >> 1) % heads);
-    const long b = (rest >> 1) / heads;
-    const long j = (long)(pos ? pos[b] : 0) + t, end = lens ? min(lens[b], cap) : cap;
-    uint4 o = make_uint4(0, 0, 0, 0);
-    if (j >= 0 && j < end) {
-        const uint2 w = *reinterpret_cast<const uint2*>((isv ? c.v : c.k) + b * c.c_seq + hd * c.c_head + j * HD + d0);
-        const float s = ((isv ? c.vs : c.ks) + b * c.s_seq + hd * c.s_head)[j / block];
-        float y[4];
+    griddep_launch_dependents();
+    const long p0 = pos ? pos[b] : 0;
+    const int end = lens ? min(lens[b], cap) : cap;
+    const uint8_t* codes = (isv ? c.v : c.k) + b * c.c_seq + hd * c.c_head + d0;
+    const float* scale = (isv ? c.vs : c.ks) + b * c.s_seq + hd * c.s_head;
+    h16* y = (isv ? v : k) + b * y_seq + hd * y_head + d0;
+    const int t0 = (int)tile * 128 + (threadIdx.x >> 3);
+    uint2 w[4];
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const long j = p0 + t0 + 32 * i;
+        w[i] = make_uint2(0, 0), s[i] = 0.f;
+        if (t0 + 32 * i < n && j >= 0 && j < end) {
+            w[i] = *reinterpret_cast<const uint2*>(codes + j * HD);
+            s[i] = scale[j >> shift];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (t0 + 32 * i >= n) break;
+        uint4 o;
+        float x[4];
         __half2* op = reinterpret_cast<__half2*>(&o);
 #pragma unroll
         for (int q = 0; q < 2; q++) {
-            kv8_load4<KIND>(q ? w.y : w.x, y);
-            op[2 * q] = __floats2half2_rn(__fmul_rn(y[0], s), __fmul_rn(y[1], s));
-            op[2 * q + 1] = __floats2half2_rn(__fmul_rn(y[2], s), __fmul_rn(y[3], s));
+            kv8_load4<KIND>(q ? w[i].y : w[i].x, x);
+            op[2 * q] = __floats2half2_rn(__fmul_rn(x[0], s[i]), __fmul_rn(x[1], s[i]));
+            op[2 * q + 1] = __floats2half2_rn(__fmul_rn(x[2], s[i]), __fmul_rn(x[3], s[i]));
         }
+        *reinterpret_cast<uint4*>(y + (t0 + 32 * i) * y_tok) = o;
     }
-    *reinterpret_cast<uint4*>((isv ? v : k) + b * y_seq + t * y_tok + hd * y_head + d0) = o;
 }
 
 // what both calls ask of their arguments; 0 or the last error set
@@ -190,13 +201,13 @@ int launch_kv8_write(const void* k, const void* v, long long x_seq, long long x_
     const long items = (long)batch * heads * 2 * nblk;
     const int per = block <= 32 ? 4 : 128 / block;
     const long grid = (items + per - 1) / per;
-    if (grid > 0x7fffffffl) return fail("kv8_write: more than 2^31 blocks in one call");
+    if (items > 0xffffff00l || grid > 0x7fffffffl) return fail("kv8_write: more than 2^31 blocks in one call");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     const Cache c{(uint8_t*)k8, (uint8_t*)v8, ks, vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head};
     auto* fn = kind == KV8_INT8 ? kv8_write_kernel<KV8_INT8> : kv8_write_kernel<KV8_E4M3>;
     return check_pdl(launch_pdl(fn, dim3((unsigned)grid), dim3(NT), 0, st, (const h16*)k, (const h16*)v, (long)x_seq,
-                                (long)x_tok, (long)x_head, c, pos, heads, n, cap, block, nblk, items),
+                                (long)x_tok, (long)x_head, c, pos, heads, n, cap, block, nblk, (unsigned)items),
                      "kv8_write");
 }
 
@@ -208,14 +219,15 @@ int launch_kv8_read(const void* k8, const void* v8, const float* ks, const float
                   kind))
         return -1;
     if (batch == 0 || n == 0) return 0;
-    const long items = (long)batch * heads * 2 * n * 8, grid = (items + 255) / 256;
+    const long tiles = ((long)n + 127) / 128, grid = (long)batch * heads * 2 * tiles;
     if (grid > 0x7fffffffl) return fail("kv8_read: more than 2^31 blocks in one call");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     const Cache c{(uint8_t*)k8, (uint8_t*)v8, (float*)ks, (float*)vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head};
     auto* fn = kind == KV8_INT8 ? kv8_read_kernel<KV8_INT8> : kv8_read_kernel<KV8_E4M3>;
     return check_pdl(launch_pdl(fn, dim3((unsigned)grid), dim3(256), 0, st, c, (h16*)k, (h16*)v, (long)y_seq,
-                                (long)y_tok, (long)y_head, pos, lens, heads, n, cap, block, items),
+                                (long)y_tok, (long)y_head, pos, lens, heads, n, cap, 31 - __builtin_clz(block),
+                                (unsigned)tiles),
                      "kv8_read");
 }
 

@@ -119,17 +119,6 @@ struct RowState {
     }
 };
 
-// key among the eight largest in order
-__device__ __forceinline__ void put(unsigned long long (&best)[TOP_MAX], unsigned long long key) {
-#pragma unroll
-    for (int j = 0; j < TOP_MAX; j++)
-        if (key > best[j]) {
-            const unsigned long long x = best[j];
-            best[j] = key;
-            key = x;
-        }
-}
-
 // the ids c0 .. c0 + 31 that are left out: suppressed, or past the vocabulary
 __device__ __forceinline__ uint32_t left_out(const unsigned char* sup, int c0, int V, int lane) {
     const int id = c0 + lane;
@@ -167,7 +156,8 @@ struct Smem {
 using namespace ll;
 
 // grid min(SMs, units of 32 ids), block NTHREADS, dynamic shared memory sizeof(Smem) + 1024 (alignment slack). xbox: rows
-// that a load of x brings (a multiple of 8); emap: a box of 32 ids. rec [CTAs][128][FIELDS]
+// that a load of x brings (a multiple of 8); emap: a box of 32 ids. rec [CTAs][128][FIELDS], NARROW
+// [CTAs][4 warps][32][FIELDS]
 template <bool NARROW>
 __global__ void __launch_bounds__(one::NTHREADS, 1)
     linear_one_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap emap, int rows, int V,
@@ -320,43 +310,7 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
                 if (lane == 0) mbar_arrive(&s.acce[a]);
             }
         }
-        float* to = rec + ((long)cta * BM + row) * FIELDS;
-        if (!NARROW) {
-            if (live && row < rows) r.store(to, o.top);
-        } else {
-            // the four warps' parts of a row joined by warp 0
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            float* mine = &s.box[0][0][0] + (warp * 32 + lane) * FIELDS;  // 16-byte aligned
-            r.store(mine, o.top);
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (warp == 0 && live && row < rows) {
-                RowStat a = r.stat();
-                float tgt = r.tgt;
-                unsigned long long best[TOP_MAX] = {};
-                for (int w = 0; w < 4; w++) {
-                    const float* f = mine + w * 32 * FIELDS;
-                    const float4 y = *reinterpret_cast<const float4*>(f);
-                    if (w) {
-                        a = stat_join(a, {y.x, y.y, y.z});
-                        if (tgt == -INFINITY) tgt = y.w;  // the warp that had the target has it
-                    }
-                    for (int i = 0; i < o.top; i++) {
-                        const unsigned long long key = top_key(f[4 + 2 * i], __float_as_int(f[5 + 2 * i]));
-                        if (key <= best[TOP_MAX - 1]) break;  // a warp's come in order
-                        put(best, key);
-                    }
-                }
-                float4* z = reinterpret_cast<float4*>(to);
-                z[0] = make_float4(a.m, a.s, a.u, tgt);
-#pragma unroll
-                for (int i = 0; i < TOP_MAX; i += 2)
-                    if (i < o.top) {
-                        const unsigned long long p = best[i], q = best[i + 1];
-                        z[1 + i / 2] = make_float4(p ? key_value(p) : -INFINITY, __int_as_float(key_id(p)),
-                                                   q ? key_value(q) : -INFINITY, __int_as_float(key_id(q)));
-                    }
-            }
-        }
+        if (live && row < rows) r.store(rec + (NARROW ? ((long)cta * 4 + warp) * 32 + row : (long)cta * BM + row) * FIELDS, o.top);
     }
     tc_fence_before();
     __syncthreads();
@@ -533,79 +487,99 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
     if (warp == 1) tmem_dealloc_pair(tb, 2 * BN);
 }
 
-// A warp to a row: its records joined, the outputs written. Row r has records at rec + part(r)'s; tile rows `tr` (128 or
-// 256), `bn` ids to a vocabulary tile, `halves` records to a worker and row tile
-__global__ void __launch_bounds__(128) linear_join_kernel(const float* rec, int rows, int V, int tr, int bn, int halves,
-                                                          int workers, int parts, LogpOut o) {
-    const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5);
-    griddep_wait();
-    griddep_launch_dependents();
-    if (row >= rows) return;
-    const long at = row_at(o, row);
-    if (at < 0) return;
+// A block to a row, its records joined (a record to a thread) and the outputs written. `tr` rows to a tile, `bn` ids to a
+// unit of work, `halves` records to a worker and row tile: of the halves of each unit (pairs), or of every fourth unit
+// from the worker's first on (quarters 1)
+__global__ void __launch_bounds__(1024) linear_join_kernel(const float* rec, int rows, int V, int tr, int bn, int halves,
+                                                           int quarters, int workers, int parts, LogpOut o) {
+    __shared__ RowStat st[32];
+    __shared__ unsigned long long tops[32][TOP_MAX];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    // rows of few records go to the warps of a block of 128, one each
+    const bool small = parts * halves <= 32;
+    const int row = small ? blockIdx.x * 4 + warp : blockIdx.x, first = small ? lane : threadIdx.x;
     const int mt = (rows + tr - 1) / tr, nt = (V + bn - 1) / bn, m = row / tr;
     const Share share(mt * nt, workers);
-    const int w0 = share.owner(m * nt), n = (share.owner((m + 1) * nt - 1) - w0 + 1) * halves;
+    const int w0 = share.owner(m * nt), n = row < rows ? (share.owner((m + 1) * nt - 1) - w0 + 1) * halves : 0;
     const float* base = rec + ((long)m * parts * halves * tr + row % tr) * FIELDS;
+    griddep_wait();
+    griddep_launch_dependents();
+    const long at = row_at(o, row);
+    if (at < 0 || row >= rows) return;  // the whole block, or the whole warp of a small one
     const int t = o.target ? o.target[at] : -1;
     const bool has = t >= 0 && t < V;
     float tgt = 0.f;
-    if (has) {
-        const int k = (share.owner(m * nt + t / bn) - w0) * halves + t % bn / (bn / halves);
-        tgt = base[(long)k * tr * FIELDS + 3];
-    }
     RowStat a = stat_none();
-    unsigned long long best[TOP_MAX] = {};
-    for (int k = lane; k < n; k += 32) {
-        const float4* f = reinterpret_cast<const float4*>(base + (long)k * tr * FIELDS);
+    unsigned long long key[TOP_MAX] = {};
+    if (first < n) {
+        const float4* f = reinterpret_cast<const float4*>(base + (long)first * tr * FIELDS);
         const float4 y = f[0];
         float4 z[TOP_MAX / 2];
 #pragma unroll
         for (int i = 0; i < TOP_MAX / 2; i++)
             if (2 * i < o.top) z[i] = f[1 + i];
-        a = stat_join(a, {y.x, y.y, y.z});
+        a = {y.x, y.y, y.z};
 #pragma unroll
         for (int i = 0; i < TOP_MAX; i++)
             if (i < o.top) {
                 const float4 q = z[i / 2];
-                const unsigned long long key = i & 1 ? top_key(q.z, __float_as_int(q.w)) : top_key(q.x, __float_as_int(q.y));
-                if (key > best[TOP_MAX - 1]) put(best, key);
+                key[i] = i & 1 ? top_key(q.z, __float_as_int(q.w)) : top_key(q.x, __float_as_int(q.y));
             }
     }
+    if (has && first == 0) {
+        const int unit = m * nt + t / bn, w = share.owner(unit);
+        const int k = (w - w0) * halves + (quarters ? (unit - share.first(w)) & 3 : t % bn / (bn / halves));
+        tgt = base[(long)k * tr * FIELDS + 3];
+    }
+    // the lanes' lists, each in order, popped in turn: the i-th largest ends up with lane i
+    auto pop = [&]() {
+        unsigned long long mine = 0;
+        for (int i = 0; i < o.top; i++) {
+            const unsigned hi = __reduce_max_sync(0xffffffff, (unsigned)(key[0] >> 32));
+            const unsigned lo = __reduce_max_sync(0xffffffff, (unsigned)(key[0] >> 32) == hi ? (unsigned)key[0] : 0u);
+            const unsigned long long x = (unsigned long long)hi << 32 | lo;
+            if (lane == i) mine = x;
+            if (key[0] == x && x) {
 #pragma unroll
-    for (int w = 16; w; w >>= 1)
-        a = stat_join(a, {__shfl_xor_sync(0xffffffff, a.m, w), __shfl_xor_sync(0xffffffff, a.s, w),
-                          __shfl_xor_sync(0xffffffff, a.u, w)});
+                for (int j = 0; j + 1 < TOP_MAX; j++) key[j] = key[j + 1];
+                key[TOP_MAX - 1] = 0ull;
+            }
+        }
+        return mine;
+    };
+    unsigned long long mine = pop();
+    a = stat_warp(a);
+    if (!small) {
+        if (lane == 0) st[warp] = a;
+        if (lane < TOP_MAX) tops[warp][lane] = lane < o.top ? mine : 0ull;
+        __syncthreads();
+        if (warp) return;
+        a = lane < nw ? st[lane] : stat_none();
+#pragma unroll
+        for (int i = 0; i < TOP_MAX; i++) key[i] = lane < nw ? tops[lane][i] : 0ull;
+        mine = pop();
+        a = stat_warp(a);
+    }
     float lse = 0.f;
     if (lane == 0) lse = store_row(o, at, a, has, tgt);
     lse = __shfl_sync(0xffffffff, lse, 0);
-    for (int i = 0; i < o.top; i++) {
-        unsigned long long x = best[0];
-#pragma unroll
-        for (int w = 16; w; w >>= 1) {
-            const unsigned long long y = __shfl_xor_sync(0xffffffff, x, w);
-            x = y > x ? y : x;
-        }
-        if (lane == 0) store_top(o, at, i, x, lse);
-        if (best[0] == x && x) {  // one lane's: the next of its own
-#pragma unroll
-            for (int j = 0; j + 1 < TOP_MAX; j++) best[j] = best[j + 1];
-            best[TOP_MAX - 1] = 0ull;
-        }
-    }
+    if (lane < o.top) store_top(o, at, lane, mine, lse);
 }
 
 // the layout of a call, from its sizes
 namespace {
 struct Plan {
     bool pairs;
-    int tr, bn, halves, workers, parts;  // rows of a tile, ids of a unit of work, records to a worker and row tile
+    int tr, bn, halves, quarters, workers, parts;  // as linear_join_kernel has them
     size_t bytes;
 };
 Plan plan(int rows, int V) {
     Plan p;
     p.pairs = rows > 128;
-    p.tr = p.pairs ? 256 : 128, p.bn = p.pairs ? pair::BN : one::UNIT, p.halves = p.pairs ? 2 : 1;
+    p.quarters = rows <= 32;
+    p.tr = p.pairs ? 256 : p.quarters ? 32 : 128;
+    p.bn = p.pairs ? pair::BN : one::UNIT;
+    p.halves = p.pairs ? 2 : p.quarters ? 4 : 1;
     const int mt = (rows + p.tr - 1) / p.tr, nt = (V + p.bn - 1) / p.bn, most = p.pairs ? PAIRS : 2 * PAIRS;
     const long T = (long)mt * nt;
     p.workers = (int)(T < most ? T : most);
@@ -660,8 +634,9 @@ int launch_linear_logprobs(const void* x, long long ldx, const void* emb, int ro
                                  dc.limit_ns),
                       "linear_logprobs");
     if (e) return e;
-    return check_pdl(launch_pdl(linear_join_kernel, dim3((rows + 3) / 4), dim3(128), 0, st, (const float*)rec, rows, V, p.tr,
-                                p.bn, p.halves, p.workers, p.parts, o),
+    const int n = p.parts * p.halves;  // at most 4 x 148
+    return check_pdl(launch_pdl(linear_join_kernel, dim3(n <= 32 ? (rows + 3) / 4 : rows), dim3(n <= 32 ? 128 : (n + 31) & ~31),
+                                0, st, (const float*)rec, rows, V, p.tr, p.bn, p.halves, p.quarters, p.workers, p.parts, o),
                      "linear_logprobs");
 }
 

@@ -346,10 +346,7 @@ __global__ void __launch_bounds__(NT + 32, 2)
         }
         if (cl > 1) cluster_sync();
         if (rank == 0 && warp == 0) {
-            RowStat a = lane < cl ? sm.stat[lane] : stat_none();
-            for (int d = 1; d < cl; d *= 2)
-                a = stat_join(a, {__shfl_xor_sync(0xffffffff, a.m, d), __shfl_xor_sync(0xffffffff, a.s, d),
-                                  __shfl_xor_sync(0xffffffff, a.u, d)});
+            const RowStat a = stat_warp(lane < cl ? sm.stat[lane] : stat_none());
             float lse = 0.f;
             if (lane == 0) lse = store_row(o, at, a, has, tgt);
             lse = __shfl_sync(0xffffffff, lse, 0);

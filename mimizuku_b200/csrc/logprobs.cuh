@@ -15,28 +15,6 @@ struct RowStat {
 
 __device__ __forceinline__ RowStat stat_none() { return {-INFINITY, 0.f, 0.f}; }
 
-__device__ __forceinline__ RowStat stat_join(const RowStat& a, const RowStat& b) {
-    if (b.m == -INFINITY && b.s == 0.f) return a;
-    if (a.m == -INFINITY && a.s == 0.f) return b;
-    const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m, ea = __expf(da), eb = __expf(db);
-    // e^(x - m) (x - m) = e^(x - a) e^(a - m) ((x - a) + (a - m)); nothing where e is 0 (a NaN stays in s)
-    const float ua = ea > 0.f ? ea * (a.u + da * a.s) : 0.f, ub = eb > 0.f ? eb * (b.u + db * b.s) : 0.f;
-    return {m, ea * a.s + eb * b.s, ua + ub};
-}
-__device__ __forceinline__ void stat_add(RowStat& a, float x) {
-    if (x == -INFINITY) return;
-    if (x > a.m) {
-        const float d = a.m - x, e = __expf(d);  // a.m = -inf: e = 0
-        a.u = e > 0.f ? e * (a.u + d * a.s) : 0.f;  // d * s may overflow where e = 0
-        a.s = a.s * e + 1.f;
-        a.m = x;
-    } else {
-        const float d = x - a.m, e = __expf(d);
-        a.s += e;
-        a.u += e > 0.f ? e * d : 0.f;
-    }
-}
-
 constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -81,6 +59,22 @@ struct Run {
         u = fadd2(u, other.u);
     }
 };
+// Whole warp: the lanes' statistics joined, in every lane. e^(x - M) (x - M) = e^(x - m) e^(m - M) ((x - m) + (m - M));
+// nothing where e is 0 (a NaN stays in s)
+__device__ __forceinline__ RowStat stat_warp(const RowStat& a) {
+    float M = a.m;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffff, M, w));
+    const float d = M == -INFINITY ? 0.f : a.m - M, e = __expf(d);
+    float s = e * a.s, u = e > 0.f ? e * (a.u + d * a.s) : 0.f;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) {
+        s += __shfl_xor_sync(0xffffffff, s, w);
+        u += __shfl_xor_sync(0xffffffff, u, w);
+    }
+    return {M, s, u};
+}
+
 // (value, lower id first) as one unsigned comparison; 0 stands for no candidate. -0 counts as +0. A NaN and -inf are no
 // candidates.
 __device__ __forceinline__ unsigned long long top_key(float v, int id) {
