@@ -42,6 +42,21 @@ __device__ __forceinline__ void kv8_load4(uint32_t w, float (&x)[4]) {
         x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
     }
 }
+// The same of numbers known to be finite and within the codes' range. int8: adding 1.5 2^23 rounds to an integer that the
+// low byte of the sum holds
+template <int KIND>
+__device__ __forceinline__ uint32_t kv8_store4_finite(float2 a, float2 b) {
+    if constexpr (KIND == KV8_INT8) {
+        const float2 magic = make_float2(12582912.f, 12582912.f);
+        a = __fadd2_rn(a, magic);
+        b = __fadd2_rn(b, magic);
+        const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+        return __byte_perm(lo, hi, 0x5410);
+    } else {
+        return f2_to_e4m3x2(a.x, a.y) | (f2_to_e4m3x2(b.x, b.y) << 16);
+    }
+}
 // four numbers rounded to codes (half to even; int8 clamped to +-127 with NaN as 0, e4m3 saturating with NaN kept)
 template <int KIND>
 __device__ __forceinline__ uint32_t kv8_store4(const float (&x)[4]) {

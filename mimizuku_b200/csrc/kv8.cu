@@ -60,20 +60,32 @@ __global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* k, const h16* 
     float* scale = (isv ? c.vs : c.ks) + b * c.s_seq + hd * c.s_head + blk;
     const int sub = lane >> 3, d0 = (lane & 7) * 8;
     uint4 val[8];
-    float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const long j = t0 + 4 * i + sub;
         val[i] = make_uint4(0, 0, 0, 0);
         if (any && 4 * i < tw && j >= p0 && j < end) val[i] = *reinterpret_cast<const uint4*>(x + (j - p0) * x_tok + d0);
     }
+    // the largest magnitude, in fp16; a NaN or an infinity among the CTA's values is rare, and asked for only once
+    __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const uint32_t w[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
+        const __half2* w = reinterpret_cast<const __half2*>(&val[i]);
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const float2 p = h2_to_f2(w[q]);
-            amax = fmaxf(amax, fmaxf(fabsf(finite(p.x)), fabsf(finite(p.y))));  // fmaxf drops a NaN
+        for (int q = 0; q < 4; q++) big = __hmax2_nan(big, __habs2(w[q]));
+    }
+    float amax = __half2float(__hmax_nan(__low2half(big), __high2half(big)));
+    const bool odd = __any_sync(0xffffffff, !(amax <= 65504.f));
+    if (odd) {
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t w[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float2 p = h2_to_f2(w[q]);
+                amax = fmaxf(amax, fmaxf(fabsf(finite(p.x)), fabsf(finite(p.y))));  // fmaxf drops a NaN
+            }
         }
     }
 #pragma unroll
@@ -102,6 +114,12 @@ __global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* k, const h16* 
 #pragma unroll
         for (int q = 0; q < 2; q++) {
             const float2 a = h2_to_f2(w[2 * q]), e = h2_to_f2(w[2 * q + 1]);
+            if (!odd) {
+                // (products by the scalar intrinsic: the packed one fuses with the sum after it, which rounds once)
+                op[q] = kv8_store4_finite<KIND>(make_float2(__fmul_rn(a.x, r), __fmul_rn(a.y, r)),
+                                                make_float2(__fmul_rn(e.x, r), __fmul_rn(e.y, r)));
+                continue;
+            }
             const float y[4] = {__fmul_rn(finite(a.x), r), __fmul_rn(finite(a.y), r), __fmul_rn(finite(e.x), r),
                                 __fmul_rn(finite(e.y), r)};
             op[q] = kv8_store4<KIND>(y);

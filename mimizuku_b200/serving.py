@@ -2,17 +2,25 @@
 
 Every call works on the current device and stream (or `stream`), checks its tensors on the host (MmzError) and returns
 without waiting; outputs are tensors that the caller gives."""
+import functools
+
 import torch
 
 from . import MmzError, _check, lib
 
 _KIND = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _I32, _F16, _F32, _U8 = torch.int32, torch.float16, torch.float32, torch.uint8
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _device():
-    return torch.cuda.current_device() if torch.cuda.is_available() else 0
+def _device(what, name, t):
+    """The current device, which has to be tensor t's."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise MmzError(f"{what}: {name} is not a CUDA tensor")
+    dev = t.get_device()
+    if dev != _current():
+        raise MmzError(f"{what}: {name} is on {t.device}, the current device is cuda:{_current()}")
+    return dev
 
 
 def _stream(stream, dev):
@@ -53,21 +61,21 @@ def _dense(what, name, t, dtype, shape, dev):
 
 def _cache(what, k8, v8, ks, vs, block, dev):
     """(batch, heads, cap, kind, pointers and strides) of a cache."""
-    if not isinstance(k8, torch.Tensor) or k8.dtype not in _KIND or k8.dim() != 4 or k8.shape[3] != 64:
+    kind, shape = _KIND.get(k8.dtype), k8.shape
+    if kind is None or len(shape) != 4 or shape[3] != 64:
         raise MmzError(f"{what}: k8 is an int8 or float8_e4m3fn tensor [batch][heads][cap][64]")
     if block not in (16, 32, 64, 128):
         raise MmzError(f"{what}: block is 16, 32, 64 or 128")
-    shape, dtype = k8.shape, k8.dtype
     b, h, cap, _ = shape
     blocks = (b, h, (cap + block - 1) // block)
-    pk, pv = _strided(what, "k8", k8, dtype, shape, dev), _strided(what, "v8", v8, dtype, shape, dev)
+    pv = _strided(what, "v8", v8, k8.dtype, shape, dev)
     qk, qv = _strided(what, "ks", ks, _F32, blocks, dev), _strided(what, "vs", vs, _F32, blocks, dev)
     cs, ss = k8.stride(), ks.stride()
     if v8.stride() != cs or vs.stride() != ss:
         raise MmzError(f"{what}: keys and values of the cache have the same strides")
     if cs[3] != 1 or cap > 1 and cs[2] != 64 or blocks[2] > 1 and ss[2] != 1:
         raise MmzError(f"{what}: a head's rows of the cache, and its scales, lie one after another")
-    return b, h, cap, _KIND[dtype], (pk, pv, qk, qv, cs[0], cs[1], ss[0], ss[1])
+    return b, h, cap, kind, (k8.data_ptr(), pv, qk, qv, cs[0], cs[1], ss[0], ss[1])
 
 
 def _pair(what, k, v, b, h, dev):
@@ -86,7 +94,7 @@ def kv8_write(k, v, k8, v8, ks, vs, block=64, pos=None, stream=None):
     """Quantises the tokens k, v [b][n][heads][64] fp16 into the cache k8, v8 [b][heads][cap][64] (int8 or
     float8_e4m3fn) with the scales ks, vs [b][heads][ceil(cap / block)] float32, at positions pos[b].. (int32 [b]; None:
     from 0). A block that already has tokens keeps at least its scale; its codes are rounded again when it grows."""
-    dev = _device()
+    dev = _device("kv8_write", "k8", k8)
     b, h, cap, kind, c = _cache("kv8_write", k8, v8, ks, vs, block, dev)
     pk, pv, n, s = _pair("kv8_write", k, v, b, h, dev)
     at = _dense("kv8_write", "pos", pos, _I32, (b,), dev)
@@ -97,7 +105,7 @@ def kv8_write(k, v, k8, v8, ks, vs, block=64, pos=None, stream=None):
 def kv8_read(k8, v8, ks, vs, k, v, block=64, pos=None, lens=None, stream=None):
     """The cache's values at positions pos[b].. (None: from 0) into k, v [b][n][heads][64] fp16, zeros from position
     min(lens[b], cap) on (lens None: cap)."""
-    dev = _device()
+    dev = _device("kv8_read", "k8", k8)
     b, h, cap, kind, c = _cache("kv8_read", k8, v8, ks, vs, block, dev)
     pk, pv, n, s = _pair("kv8_read", k, v, b, h, dev)
     at, ln = _dense("kv8_read", "pos", pos, _I32, (b,), dev), _dense("kv8_read", "lens", lens, _I32, (b,), dev)
@@ -105,6 +113,7 @@ def kv8_read(k8, v8, ks, vs, k, v, block=64, pos=None, lens=None, stream=None):
            "kv8_read")
 
 
+@functools.lru_cache(maxsize=256)
 def attn8_scratch_bytes(batch, rows, q_heads, kv_heads, cap, slots=0):
     """Bytes of device scratch attn8 needs for such a call (0: none)."""
     return lib.mmz_attn8_scratch_bytes(batch, rows, q_heads, kv_heads, cap, slots)
@@ -117,7 +126,7 @@ def attn8(q, k8, v8, ks, vs, out, block=64, lens=None, causal=False, scale=0.125
     positions. A row that sees nothing gives zeros. probs [b][slots][rows][cap] fp16 receives the probabilities of the
     heads with pslot[head] >= 0 (int32 [q_heads]). scratch: a uint8 tensor of attn8_scratch_bytes(...) (allocated here
     when None and needed)."""
-    dev = _device()
+    dev = _device("attn8", "k8", k8)
     b, h, cap, kind, c = _cache("attn8", k8, v8, ks, vs, block, dev)
     if not isinstance(q, torch.Tensor) or q.dim() != 4:
         raise MmzError("attn8: q is a tensor [batch][rows][q_heads][64]")
@@ -137,7 +146,7 @@ def attn8(q, k8, v8, ks, vs, out, block=64, lens=None, causal=False, scale=0.125
         pp = _dense("attn8", "probs", probs, _F16, (b, slots, rows, cap), dev)
         ps = _dense("attn8", "pslot", pslot, _I32, (hq,), dev)
     if scratch is None:
-        need = lib.mmz_attn8_scratch_bytes(b, rows, hq, h, cap, slots)
+        need = attn8_scratch_bytes(b, rows, hq, h, cap, slots)
         if need:
             scratch = torch.empty(need, dtype=_U8, device=q.device)
     sp, sb = _scratch("attn8", scratch, dev)
@@ -172,7 +181,7 @@ def token_logprobs(logits, target, logp, entropy=None, lse=None, top_id=None, to
     column col[0] is read and written. A target outside the vocabulary has logp 0."""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in (_F16, _F32) or logits.dim() != 2:
         raise MmzError("token_logprobs: logits is an fp16 or fp32 tensor [rows][vocab]")
-    dev = _device()
+    dev = _device("token_logprobs", "logits", logits)
     rows, vocab = logits.shape
     px = _strided("token_logprobs", "logits", logits, logits.dtype, logits.shape, dev)
     s = logits.stride()
@@ -183,6 +192,7 @@ def token_logprobs(logits, target, logp, entropy=None, lse=None, top_id=None, to
                                   _stream(stream, dev)), "token_logprobs")
 
 
+@functools.lru_cache(maxsize=256)
 def linear_logprobs_scratch_bytes(rows, vocab, d):
     """Bytes of device scratch linear_logprobs needs for such a call."""
     return lib.mmz_linear_logprobs_scratch_bytes(rows, vocab, d)
@@ -195,7 +205,7 @@ def linear_logprobs(x, emb, target, logp, entropy=None, lse=None, top_id=None, t
     what = "linear_logprobs"
     if not isinstance(x, torch.Tensor) or not isinstance(emb, torch.Tensor) or x.dim() != 2 or emb.dim() != 2:
         raise MmzError("linear_logprobs: x [rows][d] and emb [vocab][d] are tensors")
-    dev = _device()
+    dev = _device(what, "x", x)
     (rows, d), vocab = x.shape, emb.shape[0]
     px, pe = _strided(what, "x", x, _F16, x.shape, dev), _dense(what, "emb", emb, _F16, (vocab, d), dev)
     s = x.stride()
@@ -203,7 +213,7 @@ def linear_logprobs(x, emb, target, logp, entropy=None, lse=None, top_id=None, t
         raise MmzError("linear_logprobs: the last dimension of x is dense")
     o = _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col, dev)
     if scratch is None:
-        scratch = torch.empty(lib.mmz_linear_logprobs_scratch_bytes(rows, vocab, d), dtype=_U8, device=x.device)
+        scratch = torch.empty(linear_logprobs_scratch_bytes(rows, vocab, d), dtype=_U8, device=x.device)
     sp, sb = _scratch(what, scratch, dev)
     _check(lib.mmz_linear_logprobs(px, s[0] if rows > 1 else d, pe, rows, vocab, d, *o, sp, sb, _stream(stream, dev)),
            what)

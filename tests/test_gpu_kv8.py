@@ -414,6 +414,7 @@ def test_refusals(cuda):
            lambda: m.attn8(q, *c, out, block=32, probs=torch.empty((1, 1, 1, 63), dtype=torch.float16, device="cuda"),
                            pslot=torch.zeros(2, dtype=torch.int32, device="cuda")),
            lambda: m.attn8(q, *c, out, block=32, probs=torch.empty((1, 1, 1, 64), dtype=torch.float16, device="cuda")),
+           lambda: m.attn8(q, q, q, *c[2:], out, block=32), lambda: m.attn8(q, *c, out, block=20),
            lambda: m.kv8_write(q, q[:, :, :1], *c, block=32), lambda: m.kv8_write(q, q, *c, block=32, pos=lens.float()),
            lambda: m.kv8_read(*c, q, q.float(), block=32)]
     for call in bad:

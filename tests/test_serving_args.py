@@ -103,9 +103,9 @@ def test_python_calls_refuse_what_is_no_cuda_tensor():
     x = torch.zeros((1, 1, 2, 64), dtype=torch.float16)
     with pytest.raises(m.MmzError, match="not a CUDA tensor"):
         m.kv8_write(x, x, k8, k8, s, s)
-    with pytest.raises(m.MmzError, match="int8 or float8"):
-        m.attn8(x, x, x, s, s, x)
-    with pytest.raises(m.MmzError, match="block is"):
+    with pytest.raises(m.MmzError, match="not a CUDA tensor"):
+        m.attn8(x, None, x, s, s, x)
+    with pytest.raises(m.MmzError, match="not a CUDA tensor"):
         m.kv8_read(k8, k8, s, s, x, x, block=20)
     with pytest.raises(m.MmzError, match="fp16 or fp32"):
         m.token_logprobs(k8[0, 0], s, s)
