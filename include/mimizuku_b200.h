@@ -354,8 +354,23 @@ int mmz_engine_enc_attn(mmz_engine* e);
  * Takes effect at the next encode. */
 int mmz_engine_set_enc_gemm(mmz_engine* e, int mode);
 int mmz_engine_enc_gemm(mmz_engine* e);
+/* The cross k/v that the decoder reads: 0 (the default) fp16; 1 int8 or 2 e4m3 codes with an fp32 scale for every 64
+ * positions of a head (mmz_kv8_write after each encode; half the bytes of the decoding step's largest read), attended
+ * over by mmz_attn8, which also records the alignment heads. The fp16 buffer "xkv" stays and is what a change of this
+ * setting quantises, so it takes effect at the next step or capture. The 8-bit buffers are allocated at the first
+ * setting other than 0. Tokens may differ from the fp16 cache's where two logits nearly tie. Native kernel image only. */
+int mmz_engine_set_xkv(mmz_engine* e, int type);
+int mmz_engine_xkv(mmz_engine* e);
+/* on != 0: every decoding step also leaves the log probability of the token it chose and the entropy it was chosen
+ * from (mmz_token_logprobs of the step's fp16 logits over the ids that `suppress` leaves; the two begin_suppress ids
+ * count). Tokens and times do not change. Takes effect at the next step or capture. Native kernel image only. */
+int mmz_engine_set_logprobs(mmz_engine* e, int on);
+int mmz_engine_logprobs(mmz_engine* e);
+/* The last mmz_engine_transcribe's (or _transcribe_audio's) log probabilities and entropies, [n][max_t] each on the
+ * host (either may be NULL): those of the generated tokens, the end-of-text token included; 0 elsewhere. */
+int mmz_engine_read_logprobs(mmz_engine* e, float* logp, float* entropy);
 /* Device address of an engine buffer: "tok", "done", "ctr", "align", "logits", "eh", "eqkv", "eatt", "xkv", "mel",
- * "kc", "vc", "x", "hb", "att", "aslot"; NULL if unknown. */
+ * "kc", "vc", "x", "hb", "att", "aslot", "logp", "entropy" (NULL before mmz_engine_set_logprobs); NULL if unknown. */
 void* mmz_engine_buffer(mmz_engine* e, const char* name);
 void* mmz_engine_stream(mmz_engine* e);
 int mmz_engine_sync(mmz_engine* e);

@@ -109,6 +109,11 @@ SIGNATURES = {
     "mmz_engine_enc_attn": (_I, [_P]),
     "mmz_engine_set_enc_gemm": (_I, [_P, _I]),
     "mmz_engine_enc_gemm": (_I, [_P]),
+    "mmz_engine_set_xkv": (_I, [_P, _I]),
+    "mmz_engine_xkv": (_I, [_P]),
+    "mmz_engine_set_logprobs": (_I, [_P, _I]),
+    "mmz_engine_logprobs": (_I, [_P]),
+    "mmz_engine_read_logprobs": (_I, [_P, _FP, _FP]),
     "mmz_engine_buffer": (_P, [_P, ctypes.c_char_p]),
     "mmz_engine_stream": (_P, [_P]),
     "mmz_engine_sync": (_I, [_P]),

@@ -95,6 +95,10 @@ __device__ __forceinline__ void st_dsmem_f32x4(uint32_t addr, float x, float y, 
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
 }
 
+__device__ __forceinline__ int seq_len(const Attn8& a, long b) {
+    if (a.done && a.done[b]) return 0;
+    return a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap;
+}
 __device__ __forceinline__ float weight(float m, float M) { return m == -INFINITY ? 0.f : ex2_approx(m - M); }
 
 // 1 / the sum of a row's p: 0 for a row that saw nothing, NaN kept
@@ -425,7 +429,7 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part
     w.queries(a, b, hk, group, r0, R, lane);
     w.record(a, raws, b, hk, group, r0, R, lane);
     w.clear();
-    const int L = a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap;
+    const int L = seq_len(a, b);
     // what row r sees; the warp's last row sees the most
     auto limit = [&](int r) { return a.causal ? max(0, L - a.rows + r / group + 1) : L; };
     const int most = r0 < R ? limit(min(r0 + RT, R) - 1) : 0, least = r0 < R ? limit(r0) : 0;
@@ -550,14 +554,17 @@ struct Share {
     }
 };
 struct Flat {
-    const int* lens;
-    int cap, batch, kv_heads;
-    __device__ __forceinline__ int len(int b) const { return lens ? max(0, min(lens[b], cap)) : cap; }
+    const Attn8& a;
+    const int cap, batch, kv_heads;
+    const bool all_alike;  // every sequence has cap positions
+    __device__ __forceinline__ Flat(const Attn8& a)
+        : a(a), cap(a.cap), batch(a.batch), kv_heads(a.kv_heads), all_alike(!a.lens && !a.done) {}
+    __device__ __forceinline__ int len(int b) const { return seq_len(a, b); }
     __device__ __forceinline__ unsigned chunks(int b) const { return b < batch ? (unsigned)(len(b) + CH - 1) / CH : 0; }
     // whole warp: the chunks of the sequences before b, and of all of them
     __device__ __forceinline__ void before(int b, int lane, unsigned& upto, unsigned& all) const {
         upto = all = 0;
-        if (!lens) {
+        if (all_alike) {
             upto = (unsigned)b * chunks(0) * kv_heads;
             all = (unsigned)batch * chunks(0) * kv_heads;
             return;
@@ -574,7 +581,7 @@ struct Flat {
     // sequence's. One load per lane for up to 32 sequences
     __device__ __forceinline__ unsigned find(unsigned w, unsigned W, int lane, int& b, int& len, unsigned& f) const {
         unsigned upto, all, n;
-        if (!lens) {
+        if (all_alike) {
             before(0, lane, upto, all);
             const Share share(all, W);
             const unsigned per = chunks(0) * kv_heads;
@@ -635,7 +642,7 @@ __global__ void __launch_bounds__(NT, 4) attn8_flat_kernel(Attn8 a, float* rec, 
     Smem& sm = *reinterpret_cast<Smem*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = a.q_heads / a.kv_heads, R = a.rows * group;
-    const Flat flat{a.lens, a.cap, a.batch, a.kv_heads};
+    const Flat flat(a);
     uint64_t* full = sm.full[warp];
     if (lane == 0)
         for (int i = 0; i < STG; i++) mbar_init(&full[i], 1);
@@ -751,7 +758,7 @@ __device__ __forceinline__ Parts parts_of(const Attn8& a, const float* part, int
         p.step = REC, p.n = nclus > 1 ? nclus : 0, p.st = HD, p.so = 0;
         return p;
     }
-    const Flat flat{a.lens, a.cap, a.batch, a.kv_heads};
+    const Flat flat(a);
     unsigned upto, all;
     flat.before(b, lane, upto, all);
     const unsigned nch = flat.chunks(b);
@@ -863,10 +870,10 @@ __global__ void __launch_bounds__(512) attn8_post_kernel(Attn8 a, unsigned jbloc
     const bool live = h < a.q_heads;  // a slot that no head has is left as it is
     const int hk = live ? h / group : 0, r = i * group + (live ? h % group : 0);
     if (live && warp == 0) p = parts_of(a, part, nclus, W, b, hk, r, R, lane);
-    const int L = a.lens ? max(0, min(a.lens[b], a.cap)) : a.cap, lim = a.causal ? max(0, L - a.rows + i + 1) : L;
+    const int L = seq_len(a, b), lim = a.causal ? max(0, L - a.rows + i + 1) : L;
     griddep_wait();
     griddep_launch_dependents();
-    if (!live) return;
+    if (!live || (a.done && a.done[b])) return;
     if (warp == 0) {
         float M = 0.f, S = 0.f;
         float2 O;
@@ -877,6 +884,7 @@ __global__ void __launch_bounds__(512) attn8_post_kernel(Attn8 a, unsigned jbloc
     __syncthreads();
     const float off = rowms.x - PSHIFT, inv = rowms.y;
     const long at = (((long)b * a.slots + slot) * a.rows + i) * a.cap;
+    h16* to = a.probs + b * a.p_seq + (a.pctr ? *a.pctr * a.p_step : 0) + ((long)slot * a.rows + i) * a.cap;
     for (int j0 = threadIdx.x; j0 < a.cap; j0 += 8 * blockDim.x) {  // 8 loads at once
         float v[8];
 #pragma unroll
@@ -887,7 +895,7 @@ __global__ void __launch_bounds__(512) attn8_post_kernel(Attn8 a, unsigned jbloc
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const int j = j0 + k * blockDim.x;
-            if (j < a.cap) a.probs[at + j] = __float2half_rn(j < lim ? ex2_approx(v[k] - off) * inv : 0.f);
+            if (j < a.cap) to[j] = __float2half_rn(j < lim ? ex2_approx(v[k] - off) * inv : 0.f);
         }
     }
 }
@@ -968,6 +976,11 @@ int launch_mode(const Attn8& a, const Plan& p, float* part, float2* stats, float
 size_t attn8_scratch_bytes(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     const Plan p = plan(batch, rows, q_heads, kv_heads, cap, slots);
     return p.part + p.stats + p.raws;
+}
+
+int attn8_launches(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
+    const Plan p = plan(batch, rows, q_heads, kv_heads, cap, slots);
+    return p.flat || p.lay.nclus > 1 || slots ? 2 : 1;
 }
 
 int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, cudaStream_t st) {

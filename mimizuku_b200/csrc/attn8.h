@@ -18,6 +18,11 @@ struct Attn8 {
     const int* pslot;            // [q_heads] slot of a head's probabilities, -1: none
     int batch, rows, q_heads, kv_heads, cap, block, causal, slots;
     float scale;
+    // the engine's decoding step: finished sequences (done[b] != 0) count as empty and their probabilities are left as
+    // they are; a sequence's probabilities lie at p_seq * b + p_step * *pctr (null: 0)
+    const int* done = nullptr;
+    long p_seq = 0, p_step = 0;
+    const int* pctr = nullptr;
 };
 
 }  // namespace mmz

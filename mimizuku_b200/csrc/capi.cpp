@@ -160,10 +160,11 @@ int mmz_attn8(const void* q, long long q_seq, long long q_row, long long q_head,
               const int* lens, void* out, long long o_seq, long long o_row, long long o_head, int batch, int rows,
               int q_heads, int kv_heads, int cap, int block, int kind, int causal, float scale, void* probs,
               const int* pslot, int slots, void* scratch, unsigned long long scratch_bytes, void* stream) {
-    const Attn8 a{(const __half*)q, (long)q_seq, (long)q_row, (long)q_head, (const uint8_t*)k8, (const uint8_t*)v8,
+    Attn8 a{(const __half*)q, (long)q_seq, (long)q_row, (long)q_head, (const uint8_t*)k8, (const uint8_t*)v8,
                   ks, vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head, lens,
                   (__half*)out, (long)o_seq, (long)o_row, (long)o_head, (__half*)probs, pslot, batch, rows, q_heads,
                   kv_heads, cap, block, causal != 0, slots, scale};
+    a.p_seq = (long)slots * rows * cap;
     return launch_attn8(a, kind, scratch, (size_t)scratch_bytes, S(stream));
 }
 int mmz_token_logprobs(const void* logits, long long ldx, int type, int rows, int vocab, const unsigned char* sup,
@@ -304,6 +305,13 @@ int mmz_engine_set_enc_attn(mmz_engine* e, int unfused) { return e ? e->e->set_e
 int mmz_engine_enc_attn(mmz_engine* e) { return e ? e->e->enc_attn() : -1; }
 int mmz_engine_set_enc_gemm(mmz_engine* e, int mode) { return e ? e->e->set_enc_gemm(mode) : fail("null engine"); }
 int mmz_engine_enc_gemm(mmz_engine* e) { return e ? e->e->enc_gemm() : -1; }
+int mmz_engine_set_xkv(mmz_engine* e, int type) { return e ? e->e->set_xkv(type) : fail("null engine"); }
+int mmz_engine_xkv(mmz_engine* e) { return e ? e->e->xkv() : -1; }
+int mmz_engine_set_logprobs(mmz_engine* e, int on) { return e ? e->e->set_logprobs(on) : fail("null engine"); }
+int mmz_engine_logprobs(mmz_engine* e) { return e ? e->e->logprobs() : -1; }
+int mmz_engine_read_logprobs(mmz_engine* e, float* logp, float* entropy) {
+    return e ? e->e->read_logprobs(logp, entropy) : fail("null engine");
+}
 void* mmz_engine_buffer(mmz_engine* e, const char* name) { return e && name ? e->e->buffer(name) : nullptr; }
 void* mmz_engine_stream(mmz_engine* e) { return e ? (void*)e->e->stream() : nullptr; }
 int mmz_engine_sync(mmz_engine* e) {

@@ -17,6 +17,7 @@ namespace mmz {
 
 constexpr int HDIM = 64;
 constexpr int TENC_ = 1500;
+constexpr int XKV_BLOCK = 64, XKV_BLOCKS = (TENC_ + XKV_BLOCK - 1) / XKV_BLOCK;  // the 8-bit cross k/v: positions that share a scale
 constexpr int NFRAMES = 3000;
 constexpr int NCH = (TENC_ + 63) / 64;
 constexpr float EPS = 1e-5f;            // model.rs:12
@@ -157,13 +158,14 @@ class NativeKernels : public Kernels {
     int cross_fused_max = 8;
     void* lgscratch = nullptr;
     size_t lgscratch_bytes = 0;
+    void* keep_logits = nullptr;  // where the fused kernel leaves its logits too (for the log probabilities), null: nowhere
     bool fused_logits = true;
     int logits_argmax(const void* hb, int d, const void* emb, int vocab, int b, const unsigned char* sup, int* tok,
                       int* done, int* ctr, int maxT, int prompt_len, int eos, int bs1, int bs2,
                       cudaStream_t st) override {
         if (!fused_logits || b <= 8 || b > 32 || d > 1280 || !lgscratch) return -2;
         return ++launches, launch_logits_argmax(hb, d, emb, vocab, d, b, sup, tok, done, ctr, maxT, prompt_len, eos,
-                                                bs1, bs2, nullptr, true, lgscratch, lgscratch_bytes, st);
+                                                bs1, bs2, keep_logits, true, lgscratch, lgscratch_bytes, st);
     }
 };
 
@@ -815,6 +817,104 @@ int Engine::encode_dev(const void* mel16, int gn, int slot0) {
         CK(matmul(true, false, HDIM, TENC_, d, 1.f, xkv_.w, d, (long long)HDIM * d, xc, d, 0, 1.f, dst, HDIM,
                   (long long)TENC_ * HDIM, nblk));
     }
+    return xkv_type_ ? quantise_xkv(gn, slot0) : 0;
+}
+
+// the fp16 cross k/v of the slots from slot0 on into the 8-bit cache: every (clip, layer) is a sequence of it
+int Engine::quantise_xkv(int gn, int slot0) {
+    const int d = dm_.d, nh = dm_.nh, nl = dm_.dec_layers;
+    const size_t half = (size_t)d * TENC_, s0 = (size_t)slot0 * nl * 2;  // values of a layer's keys
+    const char* k = (const char*)xkv_buf_ + s0 * half * 2;
+    char* k8 = (char*)xkv8_ + s0 * half;
+    float* ks = xkv8s_ + s0 * nh * XKV_BLOCKS;
+    k_->launches++;
+    return launch_kv8_write(k, k + half * 2, 2 * half, HDIM, (long long)TENC_ * HDIM, k8, k8 + half, ks,
+                            ks + (size_t)nh * XKV_BLOCKS, 2 * half, (long long)TENC_ * HDIM, 2ll * nh * XKV_BLOCKS,
+                            XKV_BLOCKS, nullptr, gn * nl, nh, TENC_, TENC_, XKV_BLOCK, xkv_type_ - 1, st_);
+}
+
+// the cross-attention of layer i for the sequences [r0, r0 + bh) over the 8-bit cache
+int Engine::cross_attn8(int i, int r0, int bh, const void* q, void* out, cudaStream_t st) {
+    const int d = dm_.d, nh = dm_.nh, nl = dm_.dec_layers, mt = dm_.max_t, na = (int)gc_.align_heads.size();
+    const size_t half = (size_t)d * TENC_, s0 = ((size_t)r0 * nl + i) * 2;
+    bool rec = false;  // the layer has alignment heads
+    for (const auto& h : gc_.align_heads) rec = rec || h.first == i;
+    Attn8 a{};
+    a.q = (const __half*)q, a.q_seq = a.q_row = d, a.q_head = HDIM;
+    a.out = (__half*)out, a.o_seq = a.o_row = d, a.o_head = HDIM;
+    a.k8 = (const uint8_t*)xkv8_ + s0 * half, a.v8 = a.k8 + half;
+    a.ks = xkv8s_ + s0 * nh * XKV_BLOCKS, a.vs = a.ks + (size_t)nh * XKV_BLOCKS;
+    a.c_seq = (long)nl * 2 * half, a.c_head = (long)TENC_ * HDIM;
+    a.s_seq = (long)nl * 2 * nh * XKV_BLOCKS, a.s_head = XKV_BLOCKS;
+    a.batch = bh, a.rows = 1, a.q_heads = a.kv_heads = nh, a.cap = TENC_, a.block = XKV_BLOCK, a.scale = 0.125f;
+    a.done = done_ + r0;
+    if (rec) {
+        a.probs = (__half*)align_ + (size_t)r0 * mt * na * TENC_;
+        a.pslot = aslot_ + i * nh, a.slots = na;
+        a.p_seq = (long)mt * na * TENC_, a.p_step = (long)na * TENC_, a.pctr = ctr_;
+    }
+    const int lane = r0 > 0;
+    k_->launches += attn8_launches(bh, 1, nh, nh, TENC_, a.slots);
+    return launch_attn8(a, xkv_type_ - 1, a8_[lane], a8_bytes_[lane], st);
+}
+
+void Engine::drop_graph() {
+    if (graph_) cudaGraphExecDestroy(graph_);
+    graph_ = nullptr;
+}
+
+int Engine::set_xkv(int type) {
+    if (type < 0 || type > 2) return fail("set_xkv: 0 (fp16), 1 (int8) or 2 (e4m3)");
+    if (type && !k_->native()) return fail("set_xkv: the 8-bit cache needs the native kernel image");
+    if (type == xkv_type_) return 0;
+    CUDA_CK(cudaStreamSynchronize(st_));  // no step of the other setting in flight
+    drop_graph();
+    if (type) {
+        const int nh = dm_.nh, na = (int)gc_.align_heads.size();
+        const size_t n = (size_t)bmax_ * dm_.dec_layers * 2;
+        if (!xkv8_) xkv8_ = alloc(n * dm_.d * TENC_);
+        if (!xkv8s_) xkv8s_ = (float*)alloc(n * nh * XKV_BLOCKS * 4);
+        for (int l = 0; l < (st2_ ? 2 : 1); l++)
+            if (!a8_[l]) {
+                // the most that any batch of the lane needs: the layout differs with the batch
+                for (int b = 1; b <= (l ? LANE_ROWS : bmax_); b++)
+                    a8_bytes_[l] = std::max(a8_bytes_[l], attn8_scratch_bytes(b, 1, nh, nh, TENC_, na));
+                a8_[l] = alloc(a8_bytes_[l]);
+            }
+        if (!xkv8_ || !xkv8s_ || !a8_[0] || (st2_ && !a8_[1])) return fail("set_xkv: device memory allocation failed");
+    }
+    xkv_type_ = type;
+    return type ? quantise_xkv(bmax_, 0) : 0;
+}
+
+int Engine::set_logprobs(int on) {
+    if (on != 0 && on != 1) return fail("set_logprobs: 0 or 1");
+    if (on && !k_->native()) return fail("set_logprobs: needs the native kernel image");
+    if ((on == 1) == logprobs_) return 0;
+    CUDA_CK(cudaStreamSynchronize(st_));
+    drop_graph();
+    if (on) {
+        const size_t n = (size_t)bmax_ * dm_.max_t * 4;
+        if (!logp_) logp_ = (float*)alloc(n);
+        if (!ent_) ent_ = (float*)alloc(n);
+        if (!logp_ || !ent_) return fail("set_logprobs: device memory allocation failed");
+    }
+    logprobs_ = on == 1;
+    static_cast<NativeKernels*>(k_.get())->keep_logits = logprobs_ ? logits_ : nullptr;
+    return 0;
+}
+
+int Engine::read_logprobs(float* logp, float* entropy) {
+    if (!logprobs_) return fail("read_logprobs: set_logprobs(1) and a transcription come first");
+    const int mt = dm_.max_t, n = (int)last_lens_.size();
+    for (auto [to, from] : {std::pair<float*, float*>{logp, logp_}, {entropy, ent_}}) {
+        if (!to || !n) continue;
+        CUDA_CK(cudaMemcpyAsync(to, from, (size_t)n * mt * 4, cudaMemcpyDeviceToHost, st_));
+        CUDA_CK(cudaStreamSynchronize(st_));
+        for (int s = 0; s < n; s++)  // what the steps left outside the generated tokens means nothing
+            for (int j = 0; j < mt; j++)
+                if (j < last_np_ || j >= last_lens_[s]) to[(size_t)s * mt + j] = 0.f;
+    }
     return 0;
 }
 
@@ -900,7 +1000,8 @@ int Engine::dec_layer(int i, int r0, int bh, cudaStream_t st, cublasHandle_t h) 
     CK(lin_onto_bias_on(att, d, l.o, oo, d, bh, d, d, st, h));
     CK(k_->add_layernorm(x, oo, l.lnx, hb, bh, d, st));
     CK(lin_onto_bias_on(hb, d, l.xq, oxq, d, bh, d, d, st, h));
-    CK(k_->cross_attn(oxq, xkv, xs, stat_, part_, att, align, aslot_, ctr_, done, bh, i, nl, d, nh, na, mt, st));
+    if (xkv_type_) CK(cross_attn8(i, r0, bh, oxq, att, st));
+    else CK(k_->cross_attn(oxq, xkv, xs, stat_, part_, att, align, aslot_, ctr_, done, bh, i, nl, d, nh, na, mt, st));
     CK(lin_onto_bias_on(att, d, l.xo, oxo, d, bh, d, d, st, h));
     CK(k_->add_layernorm(x, oxo, l.ln3, hb, bh, d, st));
     // up to 8 sequences the fc1 product and its GELU are one kernel where the image has it (model.rs:708-709)
@@ -946,7 +1047,14 @@ int Engine::step(int b, int prompt_len) {
     const int bs1 = gc_.bs[0], bs2 = gc_.bs[1];
     const int fr = k_->logits_argmax(hb_, d, emb_, dm_.vocab, b, sup_, tok_, done_, ctr_, mt, prompt_len, gc_.eos, bs1,
                                      bs2, st_);
-    if (fr != -2) return fr;  // one kernel did all three (model.rs:714-735)
+    // the chosen token's log probability and entropy, at the position that the step has just advanced to
+    auto logp = [&]() {
+        if (!logprobs_) return 0;
+        k_->launches++;
+        const LogpOut o{tok_, logp_, ent_, nullptr, nullptr, nullptr, mt, ctr_, 0};
+        return launch_token_logprobs(logits_, dm_.vocab, 0, b, dm_.vocab, sup_, o, st_);
+    };
+    if (fr != -2) return fr ? fr : logp();  // one kernel did all three (model.rs:714-735)
     const int lr = k_->logits(hb_, d, emb_, logits_, dm_.vocab, b, d, st_);
     if (lr == -1) return -1;
     if (lr == 0) {
@@ -958,7 +1066,8 @@ int Engine::step(int b, int prompt_len) {
         CK(matmul(true, false, dm_.vocab, b, d, 1.f, emb_, d, 0, hb_, d, 0, 0.f, logits_, dm_.vocab, 0, 1));
     }
     CK(k_->argmax_tok(logits_, dm_.vocab, sup_, tok_, done_, ctr_, b, mt, prompt_len, gc_.eos, bs1, bs2, st_));
-    return k_->advance(ctr_, st_);
+    CK(k_->advance(ctr_, st_));
+    return logp();
 }
 
 int Engine::capture(int b, int prompt_len) {
@@ -1180,6 +1289,8 @@ int Engine::decode_and_times(const int* frames, int n, const int* prompt, int np
         work(0);
         for (auto& t : th) t.join();
     }
+    last_lens_ = nseq;
+    last_np_ = np;
     auto t3 = clk::now();
     if (stage_s) {
         stage_s[0] = std::chrono::duration<double>(t1 - t0).count();
@@ -1208,6 +1319,8 @@ void* Engine::buffer(const std::string& name) const {
     if (name == "hb") return hb_;
     if (name == "att") return att_;
     if (name == "aslot") return aslot_;
+    if (name == "logp") return logp_;
+    if (name == "entropy") return ent_;
     return nullptr;
 }
 

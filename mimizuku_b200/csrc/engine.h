@@ -101,6 +101,14 @@ class Engine {
     // projection stored into the head blocks, cuBLASLt for the others (o, fc2, the convolutions: faster there)
     int set_enc_gemm(int mode);
     int enc_gemm() const { return enc_tc_ ? 1 : 0; }
+    // the cross k/v that the decoder reads (native image): 0 fp16, 1 int8 and 2 e4m3 codes with a scale for every 64
+    // positions of a head, quantised from the fp16 buffer after each encode
+    int set_xkv(int type);
+    int xkv() const { return xkv_type_; }
+    // the chosen tokens' log probabilities and entropies, left by every step (native image)
+    int set_logprobs(int on);
+    int logprobs() const { return logprobs_ ? 1 : 0; }
+    int read_logprobs(float* logp, float* entropy);
 
    private:
     int lin(const void* x, int ldx, const Lin& l, void* y, int ldy, int m, int n, int k);
@@ -119,6 +127,9 @@ class Engine {
     // decoder layer i (model.rs:665-705) for the sequences [r0, r0 + bh) on stream st with cuBLAS handle h
     int dec_layer(int i, int r0, int bh, cudaStream_t st, cublasHandle_t h);
     int lanes_rows_match();
+    int quantise_xkv(int gn, int slot0);
+    int cross_attn8(int i, int r0, int bh, const void* q, void* out, cudaStream_t st);
+    void drop_graph();
     int enc_attn_unfused(int gn);
     void* alloc(size_t bytes);
     int decode_and_times(const int* frames, int n, const int* prompt, int np, int max_steps, bool graph, int threads,
@@ -190,6 +201,15 @@ class Engine {
     void* lmw_ = nullptr;            // log-mel work space
     size_t lmw_bytes_ = 0;
     cudaEvent_t poll_ev_ = nullptr;  // recorded after that copy
+    int xkv_type_ = 0;
+    void* xkv8_ = nullptr;           // codes [bmax][layer][k|v][head][1500][64], allocated on first use
+    float* xkv8s_ = nullptr;         // and scales [bmax][layer][k|v][head][24]
+    void* a8_[2] = {nullptr, nullptr};  // attn8 scratch of the two decoder lanes
+    size_t a8_bytes_[2] = {0, 0};
+    bool logprobs_ = false;
+    float *logp_ = nullptr, *ent_ = nullptr;  // [bmax][max_t], allocated on first use
+    std::vector<int> last_lens_;     // sequence lengths of the last transcribe, and its prompt's
+    int last_np_ = 0;
     int *tok_, *done_, *ctr_, *aslot_;
     unsigned char *sup_;
     float* mel32_;

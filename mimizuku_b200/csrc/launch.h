@@ -129,6 +129,7 @@ int launch_kv8_read(const void* k8, const void* v8, const float* ks, const float
                     int kind, cudaStream_t st);
 // attention over that cache (attn8.cu); scratch of attn8_scratch_bytes, no initial contents required
 size_t attn8_scratch_bytes(int batch, int rows, int q_heads, int kv_heads, int cap, int slots);
+int attn8_launches(int batch, int rows, int q_heads, int kv_heads, int cap, int slots);  // kernels of such a call
 int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, cudaStream_t st);
 // log probabilities of given tokens, entropy and alternatives: of rows of logits (logprobs.cu; type 0 fp16, 1 fp32) and
 // of hidden states against an embedding (linear_logprobs.cu; scratch of linear_logprobs_scratch_bytes)

@@ -31,6 +31,9 @@ LARGE_V3 = ModelConfig("large-v3", 1280, 5120, 20, 32, 32, 128, 51866, n_align=1
 LARGE_V3_TURBO = ModelConfig("large-v3-turbo", 1280, 5120, 20, 32, 4, 128, 51866, n_align=6)
 
 
+_XKV = ("fp16", "int8", "e4m3")  # the decoder's cross k/v, in mmz_engine_set_xkv's order
+
+
 def align_heads(cfg: ModelConfig, n: Optional[int] = None, seed: int = 0):
     """(layer, head) pairs: every head of the second half of the decoder layers (the reference's default,
     src/model.rs:99-101), or n of them drawn with a seed."""
@@ -105,7 +108,7 @@ class Engine:
                                          prompt.ctypes.data_as(_IP), np_, max_steps, int(graph), threads,
                                          tokens.ctypes.data_as(_IP), lens.ctypes.data_as(_IP),
                                          times.ctypes.data_as(_FP), stage.ctypes.data_as(_DP)), "transcribe")
-        return {"tokens": tokens, "lens": lens, "times": times, "stage_s": stage}
+        return self._with_logprobs({"tokens": tokens, "lens": lens, "times": times, "stage_s": stage}, n)
 
     def transcribe_audio(self, clips, prompt=None, max_new=None, graph=True, threads=0):
         """src/transcribe.rs:25-167 from host audio: clips is a list of float32 sample arrays at 16 kHz (n <= bmax);
@@ -128,7 +131,8 @@ class Engine:
                                                lens.ctypes.data_as(_IP), times.ctypes.data_as(_FP),
                                                frames.ctypes.data_as(_IP), stage.ctypes.data_as(_DP)),
                "transcribe_audio")
-        return {"tokens": tokens, "lens": lens, "times": times, "frames": frames, "stage_s": stage}
+        return self._with_logprobs({"tokens": tokens, "lens": lens, "times": times, "frames": frames, "stage_s": stage},
+                                   n)
 
     def encode(self, mel16, gn, slot0=0):
         """Engine::encode (src/model.rs:545-625) of gn clips of fp16 log-mel at device address mel16."""
@@ -183,6 +187,38 @@ class Engine:
         if mode not in ("cublaslt", "native"):
             raise MmzError("enc_gemm: 'cublaslt' or 'native'")
         _check(lib.mmz_engine_set_enc_gemm(self._h, 1 if mode == "native" else 0), "set_enc_gemm")
+
+    @property
+    def xkv(self):
+        """The cross k/v that the decoder reads: "fp16" (the default), or "int8" / "e4m3" codes with an fp32 scale for
+        every 64 positions of a head, quantised from the fp16 ones (native image; half the bytes of the decoding step's
+        largest read). Takes effect at the next step or capture."""
+        return _XKV[lib.mmz_engine_xkv(self._h)]
+
+    @xkv.setter
+    def xkv(self, kind):
+        if kind not in _XKV:
+            raise MmzError("xkv: 'fp16', 'int8' or 'e4m3'")
+        _check(lib.mmz_engine_set_xkv(self._h, _XKV.index(kind)), "set_xkv")
+
+    @property
+    def logprobs(self):
+        """True: every step leaves the log probability of the token it chose and the entropy it was chosen from;
+        transcribe and transcribe_audio return them too, as logprobs and entropy [n][max_t] (0 outside the generated
+        tokens). False is the default. Native image."""
+        return lib.mmz_engine_logprobs(self._h) == 1
+
+    @logprobs.setter
+    def logprobs(self, on):
+        _check(lib.mmz_engine_set_logprobs(self._h, int(bool(on))), "set_logprobs")
+
+    def _with_logprobs(self, r, n):
+        if self.logprobs:
+            for name in ("logprobs", "entropy"):
+                r[name] = np.zeros((n, self.cfg.max_t), np.float32)
+            _check(lib.mmz_engine_read_logprobs(self._h, r["logprobs"].ctypes.data_as(_FP),
+                                                r["entropy"].ctypes.data_as(_FP)), "read_logprobs")
+        return r
 
     def buffer(self, name):
         p = lib.mmz_engine_buffer(self._h, name.encode())
