@@ -44,9 +44,9 @@ struct RowState {
     Run run;
     float v[TOP_MAX], tgt, kth;
     int id[TOP_MAX];
-    __device__ __forceinline__ void clear() {
+    __device__ __forceinline__ void clear(bool live) {  // a row that does not exist takes no alternatives
         run = {LOWEST, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        tgt = kth = -INFINITY;
+        tgt = -INFINITY, kth = live ? -INFINITY : INFINITY;
 #pragma unroll
         for (int i = 0; i < TOP_MAX; i++) v[i] = -INFINITY, id[i] = -1;
     }
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
         const int target = live && row < rows && o.target ? o.target[row_at(o, row)] : -1;
         const uint32_t tl = tb + ((uint32_t)(NARROW ? 0 : warp * 32) << 16);
         RowState r;
-        r.clear();
+        r.clear(row < rows);
         for (int i = 0; i < my; i++) {
             const int a = i & 1, n = min(4, units - 4 * i), id0 = (u0 + 4 * i) * UNIT;
             if (NARROW) {
@@ -267,14 +267,13 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
                         0xffffffff, mbar_wait_spin(&s.accf[a], (i >> 1) & 1, abort, limit_ns, status, K_LOGP, 6));
                     if (ok) {
                         tc_fence_after();
-#pragma unroll 1
-                        for (int u = 0; u < n; u++) {
-                            uint32_t acc[32];
-                            __syncwarp();
-                            tmem_ld32(tl + a * 128 + 32 * u, acc);
+                        uint32_t acc[128];  // (columns past the tile's ids hold an earlier tile's and go nowhere)
+                        tmem_ld128(tl + a * 128, acc);
 #pragma unroll
-                            for (int k = 0; k < 32; k++) box[u][k * 32 + lane] = __uint_as_float(acc[k]);
-                        }
+                        for (int u = 0; u < 4; u++)
+                            if (u < n)
+#pragma unroll
+                                for (int k = 0; k < 32; k++) box[u][k * 32 + lane] = __uint_as_float(acc[32 * u + k]);
                         tc_fence_before();
                     }
                     __syncwarp();
@@ -432,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
         const uint32_t tl = tb + ((uint32_t)(qd * 32) << 16) + half * (BN / 2);
         const uint32_t acce0 = dsmem_addr(&s.acce[0], 0);
         RowState r;
-        r.clear();
+        r.clear(false);
         int m = -1, target = -1;  // row tile
         auto finish = [&]() {
             if (m < 0 || m * 2 * BMC + lrow >= rows || col < 0) return;
@@ -444,8 +443,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
             if ((t0 + i) / nt != m) {
                 finish();
                 m = (t0 + i) / nt;
-                r.clear();
                 const int row = m * 2 * BMC + lrow;
+                r.clear(row < rows);
                 target = row < rows && o.target && col >= 0 ? o.target[row_at(o, row)] : -1;
             }
             const bool ok =

@@ -47,16 +47,17 @@ struct Run {
     template <int K, int N>
     __device__ __forceinline__ void add(const float (&x)[K][N], float h) {  // h: the largest of x
         raise(h);
-        Run other{m, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // the pieces' sums apart from the running ones, which so take one step for all of them (fp32 rounding)
+        Run one{m, make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, other = one;
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
             for (int i = 0; i < N; i += 4) {
-                add2(x[k][i], x[k][i + 1]);
+                one.add2(x[k][i], x[k][i + 1]);
                 other.add2(x[k][i + 2], x[k][i + 3]);
             }
-        s = fadd2(s, other.s);
-        u = fadd2(u, other.u);
+        s = fadd2(s, fadd2(one.s, other.s));
+        u = fadd2(u, fadd2(one.u, other.u));
     }
 };
 // Whole warp: the lanes' statistics joined, in every lane. e^(x - M) (x - M) = e^(x - m) e^(m - M) ((x - m) + (m - M));

@@ -68,14 +68,17 @@ def _cache(what, k8, v8, ks, vs, block, dev):
         raise MmzError(f"{what}: block is 16, 32, 64 or 128")
     b, h, cap, _ = shape
     blocks = (b, h, (cap + block - 1) // block)
-    pv = _strided(what, "v8", v8, k8.dtype, shape, dev)
-    qk, qv = _strided(what, "ks", ks, _F32, blocks, dev), _strided(what, "vs", vs, _F32, blocks, dev)
+    if not (isinstance(v8, torch.Tensor) and v8.dtype is k8.dtype and v8.shape == shape and v8.get_device() == dev):
+        _refuse(what, "v8", v8, k8.dtype, shape, dev)
+    for t, name in ((ks, "ks"), (vs, "vs")):
+        if not (isinstance(t, torch.Tensor) and t.dtype is _F32 and t.shape == blocks and t.get_device() == dev):
+            _refuse(what, name, t, _F32, blocks, dev)
     cs, ss = k8.stride(), ks.stride()
     if v8.stride() != cs or vs.stride() != ss:
         raise MmzError(f"{what}: keys and values of the cache have the same strides")
     if cs[3] != 1 or cap > 1 and cs[2] != 64 or blocks[2] > 1 and ss[2] != 1:
         raise MmzError(f"{what}: a head's rows of the cache, and its scales, lie one after another")
-    return b, h, cap, kind, (k8.data_ptr(), pv, qk, qv, cs[0], cs[1], ss[0], ss[1])
+    return b, h, cap, kind, (k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), cs[0], cs[1], ss[0], ss[1])
 
 
 def _pair(what, k, v, b, h, dev):
@@ -83,11 +86,14 @@ def _pair(what, k, v, b, h, dev):
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise MmzError(f"{what}: k is a tensor [batch][n][heads][64]")
     n = k.shape[1]
-    pk, pv = _strided(what, "k", k, _F16, (b, n, h, 64), dev), _strided(what, "v", v, _F16, (b, n, h, 64), dev)
+    shape = (b, n, h, 64)
+    for t, name in ((k, "k"), (v, "v")):
+        if not (isinstance(t, torch.Tensor) and t.dtype is _F16 and t.shape == shape and t.get_device() == dev):
+            _refuse(what, name, t, _F16, shape, dev)
     s = k.stride()
     if v.stride() != s or s[3] != 1:
         raise MmzError(f"{what}: k and v have the same strides, the last dimension dense")
-    return pk, pv, n, s
+    return k.data_ptr(), v.data_ptr(), n, s
 
 
 def kv8_write(k, v, k8, v8, ks, vs, block=64, pos=None, stream=None):
