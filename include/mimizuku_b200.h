@@ -183,9 +183,9 @@ int mmz_logits_argmax(const void* x, int ldx, const void* emb, int vocab, int d,
  * the cache at positions pos[b] .. pos[b] + n - 1 (pos NULL: from 0); tokens outside [0, cap) are left out. Per block
  * touched and head: scale = max |x| / 127 (int8) or / 448 (e4m3) over its new tokens, but at least the block's earlier
  * scale where it has tokens before pos[b], whose codes are rounded again onto the new scale when it is larger; code =
- * x / scale, to nearest even. Rows behind the new tokens are left as they are (and mean nothing). An infinity counts
- * as +-65504; a NaN becomes 0 (int8) or stays (e4m3). One call's positions and another's must not be written
- * concurrently. */
+ * x / scale, to nearest even. The cache's sequences and heads must not overlap (they may in the calls that read it: a
+ * sequence stride of 0 lets several share one cache). Rows behind the new tokens are left as they are (and mean nothing). An infinity counts
+ * as +-65504; a NaN becomes 0 (int8) or stays (e4m3). */
 int mmz_kv8_write(const void* k, const void* v, long long x_seq, long long x_tok, long long x_head, void* k8, void* v8,
                   float* ks, float* vs, long long c_seq, long long c_head, long long s_seq, long long s_head,
                   const int* pos, int batch, int heads, int n, int cap, int block, int kind, void* stream);

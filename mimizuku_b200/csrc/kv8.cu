@@ -13,6 +13,8 @@
 // Bound by memory: 2 bytes read and 1 written per value. A warp takes 32 tokens of one block (8 lanes to a token, 16
 // bytes each), so that its 8 loads are all in flight before the maximum is known and the values are read once; blocks
 // of 64 and 128 tokens are shared by 2 and 4 warps of the CTA, which exchange their maxima in shared memory.
+#include <cstdlib>
+
 #include "fp8_cache.cuh"
 #include "launch.h"
 
@@ -193,6 +195,7 @@ static int kv8_check(const char* what, const void* k, const void* v, const void*
                      const void* vs, long long x_seq, long long x_tok, long long x_head, long long c_seq,
                      long long c_head, int batch, int heads, int n, int cap, int block, int kind) {
     if (batch < 0 || heads < 1 || n < 0 || cap < 1) return failf("%s: batch >= 0, heads >= 1, n >= 0, cap >= 1", what);
+    if (cap > 0x7fff0000) return failf("%s: cap up to 2^31 - 65536", what);
     if (!kv8_block_ok(block)) return failf("%s: block is 16, 32, 64 or 128", what);
     if (kind != KV8_INT8 && kind != KV8_E4M3) return failf("%s: kind is 0 (int8) or 1 (e4m3)", what);
     if (batch == 0 || n == 0) return 0;
@@ -212,6 +215,11 @@ int launch_kv8_write(const void* k, const void* v, long long x_seq, long long x_
                   kind))
         return -1;
     if (batch == 0 || n == 0) return 0;
+    // two sequences or heads in one place would be written by two blocks at once
+    const long long room = (long long)cap * HD, scales = (cap + block - 1) / block;
+    if ((batch > 1 && (llabs(c_seq) < room || llabs(s_seq) < scales)) ||
+        (heads > 1 && (llabs(c_head) < room || llabs(s_head) < scales)))
+        return fail("kv8_write: the cache's sequences and heads overlap");
     // blocks that n tokens can touch, from any position
     const int most = (cap + block - 1) / block;
     const long touched = pos ? ((long)n + block - 2) / block + 1 : ((long)n + block - 1) / block;

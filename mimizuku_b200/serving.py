@@ -78,11 +78,13 @@ def _cache(what, k8, v8, ks, vs, block, dev):
         raise MmzError(f"{what}: keys and values of the cache have the same strides")
     if cs[3] != 1 or cap > 1 and cs[2] != 64 or blocks[2] > 1 and ss[2] != 1:
         raise MmzError(f"{what}: a head's rows of the cache, and its scales, lie one after another")
-    return b, h, cap, kind, (k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), cs[0], cs[1], ss[0], ss[1])
+    # (the stride of a dimension of one may be anything)
+    return b, h, cap, kind, (k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), cs[0] if b > 1 else 0,
+                             cs[1] if h > 1 else 0, ss[0] if b > 1 else 0, ss[1] if h > 1 else 0)
 
 
 def _pair(what, k, v, b, h, dev):
-    """Pointers, token count and shared strides of k and v [batch][n][heads][64] fp16."""
+    """Pointers, token count and shared strides of k and v [batch][n][heads][64] fp16 (0 for a dimension of one)."""
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise MmzError(f"{what}: k is a tensor [batch][n][heads][64]")
     n = k.shape[1]
@@ -93,7 +95,11 @@ def _pair(what, k, v, b, h, dev):
     s = k.stride()
     if v.stride() != s or s[3] != 1:
         raise MmzError(f"{what}: k and v have the same strides, the last dimension dense")
-    return k.data_ptr(), v.data_ptr(), n, s
+    return k.data_ptr(), v.data_ptr(), n, _steps(s, shape)
+
+
+def _steps(s, shape):
+    return [t if n > 1 else 0 for t, n in zip(s, shape)]
 
 
 def kv8_write(k, v, k8, v8, ks, vs, block=64, pos=None, stream=None):
@@ -144,6 +150,7 @@ def attn8(q, k8, v8, ks, vs, out, block=64, lens=None, causal=False, scale=0.125
     s, o = q.stride(), out.stride()
     if s[3] != 1 or o[3] != 1:
         raise MmzError("attn8: the last dimension of q and out is dense")
+    s, o = _steps(s, shape), _steps(o, shape)
     ln = _dense("attn8", "lens", lens, _I32, (b,), dev)
     pp = ps = None
     slots = 0
@@ -154,10 +161,18 @@ def attn8(q, k8, v8, ks, vs, out, block=64, lens=None, causal=False, scale=0.125
     if scratch is None:
         need = attn8_scratch_bytes(b, rows, hq, h, cap, slots)
         if need:
-            scratch = torch.empty(need, dtype=_U8, device=q.device)
+            scratch = _own_scratch(need, q.device, stream)
     sp, sb = _scratch("attn8", scratch, dev)
     _check(lib.mmz_attn8(pq, s[0], s[1], s[2], *c, ln, po, o[0], o[1], o[2], b, rows, hq, h, cap, block, kind, causal,
                          scale, pp, ps, slots, sp, sb, _stream(stream, dev)), "attn8")
+
+
+def _own_scratch(need, device, stream):
+    """Scratch of one call: the allocator gives it to nobody else before the call's stream is through with it."""
+    t = torch.empty(need, dtype=_U8, device=device)
+    if stream is not None:
+        t.record_stream(torch.cuda.ExternalStream(stream, device) if isinstance(stream, int) else stream)
+    return t
 
 
 def _scratch(what, t, dev):
@@ -170,6 +185,8 @@ def _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, su
         raise MmzError(f"{what}: logp is a tensor [rows], or [rows][steps] with col")
     ld = 1 if col is None else logp.shape[1]
     shape = (rows,) if col is None else (rows, ld)
+    if col is not None and not (isinstance(col, torch.Tensor) and col.numel()):
+        raise MmzError(f"{what}: col is an int32 tensor of one number")
     one = top_id if top_id is not None else top_logp
     top = one.shape[-1] if isinstance(one, torch.Tensor) and one.dim() else 0
     return (_dense(what, "sup", sup, _U8, (vocab,), dev), _dense(what, "target", target, _I32, shape, dev),
@@ -219,7 +236,7 @@ def linear_logprobs(x, emb, target, logp, entropy=None, lse=None, top_id=None, t
         raise MmzError("linear_logprobs: the last dimension of x is dense")
     o = _outputs(what, rows, vocab, target, logp, entropy, lse, top_id, top_logp, sup, col, dev)
     if scratch is None:
-        scratch = torch.empty(linear_logprobs_scratch_bytes(rows, vocab, d), dtype=_U8, device=x.device)
+        scratch = _own_scratch(linear_logprobs_scratch_bytes(rows, vocab, d), x.device, stream)
     sp, sb = _scratch(what, scratch, dev)
     _check(lib.mmz_linear_logprobs(px, s[0] if rows > 1 else d, pe, rows, vocab, d, *o, sp, sb, _stream(stream, dev)),
            what)

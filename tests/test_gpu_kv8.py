@@ -402,6 +402,47 @@ def test_decoding_in_a_graph_and_on_two_streams(cuda):
         assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(c, eager[i][1]))
 
 
+def test_sequences_that_share_a_cache(cuda):
+    """Several sequences over one cache (a sequence stride of 0), each with its own length; odd strides of dimensions of
+    one."""
+    gen = torch.Generator().manual_seed(8)
+    b, h, cap, block = 5, 3, 150, 32
+    c = filled(gen, 1, h, cap, block, "int8")
+    shared = [x.expand(b, *x.shape[1:]) for x in c]
+    lens = torch.tensor([1, 150, 33, 0, 64], dtype=torch.int32)
+    q = torch.randn((b, 1, h, HD), generator=gen).to(torch.float16)
+    out = torch.empty_like(q, device="cuda")
+    m.attn8(q.cuda(), *shared, out, block=block, lens=lens.cuda())
+    k, v = (np.repeat(values(x, s, block), b, 0) for x, s in ((c[0], c[2]), (c[1], c[3])))
+    want, tol, _, _ = attend_ref(q.double().numpy(), k, v, lens.tolist(), False)
+    check(out, want, tol)
+    with pytest.raises(m.MmzError, match="overlap"):
+        m.kv8_write(out, out, *shared, block=block)
+    one = torch.empty((1, 3, h, HD), dtype=torch.float16, device="cuda").as_strided((1, 1, h, HD), (7, 13, HD, 1))
+    one.copy_(q[:1].cuda())
+    o1 = torch.empty((1, 1, h, HD), dtype=torch.float16, device="cuda").as_strided((1, 1, h, HD), (3, 5, HD, 1))
+    m.attn8(one, *c, o1, block=block, lens=lens[:1].cuda())
+    assert torch.equal(o1, out[:1])
+
+
+def test_scratch_of_a_call_on_another_stream(cuda):
+    """Calls without scratch on a stream that is not the current one, while the current one allocates and writes."""
+    gen = torch.Generator().manual_seed(9)
+    c = filled(gen, 1, 2, 60000, 64, "int8")
+    q = torch.randn((1, 1, 2, HD), generator=gen).to(torch.float16).cuda()
+    want = torch.empty_like(q)
+    assert m.attn8_scratch_bytes(1, 1, 2, 2, 60000) > 0
+    m.attn8(q, *c, want, block=64)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    outs = [torch.empty_like(q) for _ in range(20)]
+    for i, out in enumerate(outs):
+        m.attn8(q, *c, out, block=64, stream=st if i % 2 else st.cuda_stream)
+        torch.full((m.attn8_scratch_bytes(1, 1, 2, 2, 60000),), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs)
+
+
 def test_refusals(cuda):
     c = cache(1, 2, 64, 32, "int8")
     q = torch.zeros((1, 1, 2, HD), dtype=torch.float16, device="cuda")

@@ -201,6 +201,30 @@ def test_columns_of_a_captured_step(cuda):
     assert all((v[:, steps - 1] == 77).all() for v in o.values())
 
 
+def test_refusals(cuda):
+    x = torch.zeros((2, 10), dtype=torch.float16, device="cuda")
+    t = torch.zeros(2, dtype=torch.int32, device="cuda")
+    f = torch.zeros(2, device="cuda")
+    emb = torch.zeros((10, 64), dtype=torch.float16, device="cuda")
+    h = torch.zeros((2, 64), dtype=torch.float16, device="cuda")
+    t2, f2 = t[:, None].contiguous(), f[:, None].contiguous()
+    bad = [lambda: m.token_logprobs(x.double(), t, f), lambda: m.token_logprobs(x, t.long(), f),
+           lambda: m.token_logprobs(x, t, f.half()), lambda: m.token_logprobs(x, t[:1], f), lambda: m.token_logprobs(x.t(), t, f),
+           lambda: m.token_logprobs(x, t, f, top_id=torch.zeros((2, 9), dtype=torch.int32, device="cuda")),
+           lambda: m.token_logprobs(x, t, f, top_id=torch.zeros((2, 3), dtype=torch.int32, device="cuda"), top_logp=f2),
+           lambda: m.token_logprobs(x, t, f, sup=torch.zeros(9, dtype=torch.uint8, device="cuda")),
+           lambda: m.token_logprobs(x, t, f, col=t[:1]), lambda: m.token_logprobs(x, t2, f2, col=t[:0]),
+           lambda: m.token_logprobs(x, None, f), lambda: m.token_logprobs(x[:, :0], t, f),
+           lambda: m.linear_logprobs(h[:, :32], emb[:, :32].contiguous(), t, f), lambda: m.linear_logprobs(h, emb[:, :32], t, f),
+           lambda: m.linear_logprobs(h.float(), emb, t, f), lambda: m.linear_logprobs(h, emb.cpu(), t, f),
+           lambda: m.linear_logprobs(h, emb, t, f, scratch=torch.zeros(16, dtype=torch.uint8, device="cuda"))]
+    for call in bad:
+        with pytest.raises(m.MmzError):
+            call()
+    m.token_logprobs(x[:0], t[:0], f[:0])  # no rows: nothing to do
+    m.linear_logprobs(h[:0], emb, t[:0], f[:0])
+
+
 def test_row_offsets_past_32_bits(cuda):
     V, ld = 1000, (1 << 31) + 8
     big = torch.empty(ld + V, dtype=torch.float16, device="cuda")

@@ -21,13 +21,19 @@ def read(k=A, v=A, xs=(64, 64, 64), k8=A, v8=A, ks=A, vs=A, cs=(6400, 6400), bat
 @pytest.mark.parametrize("bad,word", [
     (dict(block=0), b"block"), (dict(block=48), b"block"), (dict(block=256), b"block"), (dict(kind=2), b"kind"),
     (dict(kind=-1), b"kind"), (dict(batch=-1), b"batch"), (dict(heads=0), b"heads"), (dict(n=-1), b"n >= 0"),
-    (dict(cap=0), b"cap"), (dict(k=None), b"null"), (dict(ks=None), b"null"), (dict(v8=None), b"null"),
+    (dict(cap=0), b"cap"), (dict(cap=0x7fffffff), b"cap"), (dict(k=None), b"null"), (dict(ks=None), b"null"), (dict(v8=None), b"null"),
     (dict(k=A + 8), b"aligned"), (dict(k8=A + 4), b"aligned"), (dict(xs=(64, 60, 64)), b"strides"),
-    (dict(cs=(6400, 6392)), b"strides"), (dict(batch=1 << 20, heads=1 << 12, n=99), b"2^31")])
+    (dict(cs=(6400, 6392)), b"strides"),
+    (dict(batch=1 << 20, heads=1 << 12, n=99, cs=(1 << 40, 6400)), b"2^31")])
 def test_cache_calls_refuse(fn, name, bad, word):
     assert fn(**bad) == -1
     msg = L.mmz_last_error()
     assert name in msg and word in msg
+
+
+def test_a_cache_that_overlaps_is_read_only():
+    for bad in (dict(batch=2, cs=(0, 6400)), dict(heads=2, cs=(12800, 3200)), dict(batch=2, cs=(6384, 6400))):
+        assert write(**bad) == -1 and b"overlap" in L.mmz_last_error()
 
 
 def test_nothing_to_do_is_no_error():
