@@ -394,7 +394,7 @@ struct Lay {
 }  // namespace a8
 using namespace a8;
 
-// grid: cluster rank fastest, then cluster along the sequence, row block, (sequence, key head); cluster of cs CTAs.
+// grid: cluster rank fastest, then cluster along the sequence, (sequence, key head), row block; cluster of cs CTAs.
 // nclus 1: the cluster's rows go to out (and their statistics to stats, if not null); else to part
 template <int KIND, int MODE>
 __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part, float2* stats, float* raws, unsigned* status,
@@ -409,8 +409,9 @@ __global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part
     x /= cs;
     const int clus = x % lay.nclus;
     x /= lay.nclus;
-    const int tile = lay.tiles - 1 - (int)(x % lay.tiles);  // the last rows first: with causal they have the most to do
-    const unsigned pair = x / lay.tiles;
+    // every pair's last rows first: with causal they have the most to do, and the first rows' blocks fill up the end
+    const unsigned pairs = (unsigned)a.batch * a.kv_heads, pair = x % pairs;
+    const int tile = lay.tiles - 1 - (int)(x / pairs);
     const int hk = (int)(pair % a.kv_heads), group = a.q_heads / a.kv_heads;
     const long b = pair / a.kv_heads;
     const int R = a.rows * group;

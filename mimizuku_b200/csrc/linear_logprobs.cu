@@ -505,9 +505,8 @@ __global__ void __launch_bounds__(1024) linear_join_kernel(const float* rec, int
     griddep_launch_dependents();
     const long at = row_at(o, row);
     if (at < 0 || row >= rows) return;  // the whole block, or the whole warp of a small one
-    const int t = o.target ? o.target[at] : -1;
-    const bool has = t >= 0 && t < V;
-    float tgt = 0.f;
+    int t = -1;
+    if (first == 0 && o.target) t = o.target[at];
     RowStat a = stat_none();
     unsigned long long key[TOP_MAX] = {};
     if (first < n) {
@@ -525,7 +524,9 @@ __global__ void __launch_bounds__(1024) linear_join_kernel(const float* rec, int
                 key[i] = i & 1 ? top_key(q.z, __float_as_int(q.w)) : top_key(q.x, __float_as_int(q.y));
             }
     }
-    if (has && first == 0) {
+    const bool has = t >= 0 && t < V;  // (only the first thread looks)
+    float tgt = 0.f;
+    if (has) {
         const int unit = m * nt + t / bn, w = share.owner(unit);
         const int k = (w - w0) * halves + (quarters ? (unit - share.first(w)) & 3 : t % bn / (bn / halves));
         tgt = base[(long)k * tr * FIELDS + 3];
