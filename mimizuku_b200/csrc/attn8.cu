@@ -397,7 +397,7 @@ using namespace a8;
 // grid: cluster rank fastest, then cluster along the sequence, (sequence, key head), row block; cluster of cs CTAs.
 // nclus 1: the cluster's rows go to out (and their statistics to stats, if not null); else to part
 template <int KIND, int MODE>
-__global__ void __launch_bounds__(NT) attn8_kernel(Attn8 a, Lay lay, float* part, float2* stats, float* raws, unsigned* status,
+__global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* part, float2* stats, float* raws, unsigned* status,
                                                    unsigned long long limit_ns) {
     constexpr int NTL = Rows<KIND, MODE>::NTL, RT = 8 * NTL;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -936,7 +936,8 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     p.lay.cs = cs;
     p.lay.nclus = (int)(s / cs);
     const size_t n = (size_t)p.lay.block * cs * (p.lay.wrows ? 1 : WARPS);  // (row, source) pairs
-    p.smem = sizeof(Smem) + (n + (n & 1)) * 8 + n * (HD / cs) * 4;
+    const bool alone = p.lay.wrows && s == 1;  // a warp has its rows' whole results, nothing is exchanged
+    p.smem = sizeof(Smem) + (alone ? 0 : (n + (n & 1)) * 8 + n * (HD / cs) * 4);
     p.part = p.lay.nclus > 1 ? ((size_t)pairs * R * p.lay.nclus * REC * 4 + 15) & ~(size_t)15 : 0;
     return p;
 }
