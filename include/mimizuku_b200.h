@@ -173,66 +173,88 @@ int mmz_logits_argmax(const void* x, int ldx, const void* emb, int vocab, int d,
                       int advance, void* scratch, unsigned long long scratch_bytes, void* stream);
 
 /* ---------------------------------------------------------------- the 8-bit key/value cache (device pointers)
- * No counterpart in the reference, whose caches are fp16 (src/model.rs:440-455). k8, v8 [batch][heads][cap][64] hold one
- * byte per value (rows of 64 bytes one after another; c_seq and c_head: bytes from one sequence and head to the next,
- * multiples of 16), ks, vs [batch][heads][ceil(cap / block)] the fp32 scale of each `block` (16, 32, 64 or 128) tokens
- * of a head (s_seq, s_head: strides in floats). kind 0: int8 codes in -127..127; 1: e4m3. value = code * scale.
- * fp16 tensors are 16-byte aligned with strides (in values) that are multiples of 8. */
+ * No counterpart in the reference, whose caches are fp16 (src/model.rs:440-455). value = code * scale. fp16 tensors are
+ * 16-byte aligned with strides (in values) that are multiples of 8. */
+
+typedef struct {
+    void *k, *v;              /* codes [batch][heads][cap][64], one byte each, a head's rows one after another */
+    float *k_scale, *v_scale; /* [batch][heads][ceil(cap / block)]: the scale of each `block` tokens of a head */
+    long long seq, head;      /* bytes of codes from one sequence and from one head to the next, multiples of 16 */
+    long long scale_seq, scale_head; /* the same of the scales, in floats */
+    int heads, cap;
+    int block;                /* 16, 32, 64 or 128 */
+    int kind;                 /* 0: int8 codes in -127..127; 1: e4m3 */
+} mmz_kv8;
 
 /* Quantises n tokens per sequence, k and v [batch][n][heads][64] fp16 with shared strides x_seq, x_tok, x_head, into
  * the cache at positions pos[b] .. pos[b] + n - 1 (pos NULL: from 0); tokens outside [0, cap) are left out. Per block
  * touched and head: scale = max |x| / 127 (int8) or / 448 (e4m3) over its new tokens, but at least the block's earlier
  * scale where it has tokens before pos[b], whose codes are rounded again onto the new scale when it is larger; code =
  * x / scale, to nearest even. The cache's sequences and heads must not overlap (they may in the calls that read it: a
- * sequence stride of 0 lets several share one cache). Rows behind the new tokens are left as they are (and mean nothing). An infinity counts
- * as +-65504; a NaN becomes 0 (int8) or stays (e4m3). */
-int mmz_kv8_write(const void* k, const void* v, long long x_seq, long long x_tok, long long x_head, void* k8, void* v8,
-                  float* ks, float* vs, long long c_seq, long long c_head, long long s_seq, long long s_head,
-                  const int* pos, int batch, int heads, int n, int cap, int block, int kind, void* stream);
+ * sequence stride of 0 lets several share one cache). Rows behind the new tokens are left as they are (and mean
+ * nothing). An infinity counts as +-65504; a NaN becomes 0 (int8) or stays (e4m3). */
+int mmz_kv8_write(const mmz_kv8* cache, const void* k, const void* v, long long x_seq, long long x_tok, long long x_head,
+                  const int* pos, int batch, int n, void* stream);
 /* The values of positions pos[b] .. pos[b] + n - 1 (pos NULL: from 0) as fp16, k and v [batch][n][heads][64]; zeros
  * outside [0, min(lens[b], cap)) (lens NULL: cap). */
-int mmz_kv8_read(const void* k8, const void* v8, const float* ks, const float* vs, long long c_seq, long long c_head,
-                 long long s_seq, long long s_head, void* k, void* v, long long y_seq, long long y_tok,
-                 long long y_head, const int* pos, const int* lens, int batch, int heads, int n, int cap, int block,
-                 int kind, void* stream);
-/* Attention over the cache: q, out [batch][rows][q_heads][64] fp16; q_heads a multiple of kv_heads, query head h reads
- * key head h / (q_heads / kv_heads). Row i of sequence b sees the first L = min(lens[b], cap) positions (lens NULL:
- * cap), or with causal != 0 the first L - rows + i + 1: the rows are the last of the sequence. out = softmax(scale q k) v
- * with everything between the inputs and the one rounding of out in fp32; a row that sees nothing gives zeros, and what
- * lies behind the sequence (NaN included) is never used. probs (may be NULL) [batch][slots][rows][cap] fp16, 16-byte
- * aligned, receives the probabilities of the heads h with 0 <= pslot[h] < slots (pslot [q_heads], each slot given once),
- * zeros where a row sees nothing. scratch: mmz_attn8_scratch_bytes bytes, 16-byte aligned, no initial contents required
- * (NULL where that is 0); launches that share it must not overlap on the GPU. */
+int mmz_kv8_read(const mmz_kv8* cache, void* k, void* v, long long y_seq, long long y_tok, long long y_head,
+                 const int* pos, const int* lens, int batch, int n, void* stream);
+
+typedef struct {
+    const void* q;                   /* [batch][rows][q_heads][64] fp16 */
+    long long q_seq, q_row, q_head;  /* its strides in values */
+    void* out;                       /* the same */
+    long long o_seq, o_row, o_head;
+    const int* lens;                 /* [batch], NULL: cap */
+    void* probs;                     /* [batch][slots][rows][cap] fp16, 16-byte aligned; NULL: none */
+    const int* pslot;                /* [q_heads]: the slot of a head's probabilities, -1: none; each slot given once */
+    void* scratch;                   /* mmz_attn8_scratch_bytes bytes, 16-byte aligned (NULL where that is 0) */
+    unsigned long long scratch_bytes;
+    int batch, rows, q_heads, slots;
+    int causal;
+    float scale;                     /* of the scores: 0.125 in every Whisper model */
+} mmz_attn8_args;
+
+/* Attention over the cache: query head h reads key head h / (q_heads / heads), q_heads a multiple of the cache's heads.
+ * Row i of sequence b sees the first L = min(lens[b], cap) positions, or with causal != 0 the first L - rows + i + 1: the
+ * rows are the last of the sequence. out = softmax(scale q k) v with everything between the inputs and the one rounding of
+ * out in fp32; a row that sees nothing gives zeros, and what lies behind the sequence, or behind what a causal row sees
+ * (NaN included), is not used. probs receives the probabilities of the heads h with 0 <= pslot[h] < slots, zeros where a
+ * row sees nothing; a slot that no head has is left as it is. scratch has no initial contents required; launches that
+ * share it must not overlap on the GPU. cap up to 2^31 - 65536. */
 unsigned long long mmz_attn8_scratch_bytes(int batch, int rows, int q_heads, int kv_heads, int cap, int slots);
-int mmz_attn8(const void* q, long long q_seq, long long q_row, long long q_head, const void* k8, const void* v8,
-              const float* ks, const float* vs, long long c_seq, long long c_head, long long s_seq, long long s_head,
-              const int* lens, void* out, long long o_seq, long long o_row, long long o_head, int batch, int rows,
-              int q_heads, int kv_heads, int cap, int block, int kind, int causal, float scale, void* probs,
-              const int* pslot, int slots, void* scratch, unsigned long long scratch_bytes, void* stream);
+int mmz_attn8(const mmz_kv8* cache, const mmz_attn8_args* args, void* stream);
 
 /* ---------------------------------------------------------------- token log probabilities (device pointers) */
 
+/* What is asked of each row. Row r's target and outputs are at index r * ld + *col (col: a device int32, NULL = 0;
+ * nothing is written where it is outside [0, ld)), the alternatives at that index times top; any output may be NULL. */
+typedef struct {
+    const int* target;  /* may be NULL where logp is */
+    float *logp, *entropy, *lse;
+    int* top_id;        /* the `top` (0 to 8) largest logits' ids, equal ones by the lower id, */
+    float* top_logp;    /* and their log probabilities */
+    long long ld;
+    const int* col;
+    int top;
+} mmz_logprobs;
+
 /* For each row of logits [rows][ldx] (type 0 fp16, 1 fp32), over the ids with sup[id] == 0 (sup [vocab], may be NULL):
- * lse = log sum e^x; logp = x[target] - lse; entropy = -sum p log p (nats); and the `top` (0 to 8) largest logits'
- * ids, equal ones by the lower id, with their log probabilities. Sums in fp32. Row r's target and outputs are at index
- * r * ld + *col (col: a device int32, NULL = 0; nothing is written where it is outside [0, ld)), the alternatives at that
- * index times top; any output may be NULL.
- * A target outside [0, vocab) has logp 0 (padding), a suppressed one -inf. Fewer than `top` ids with a logit above
- * -inf: the rest have id -1 and -inf. No such id at all: lse -inf and entropy 0. A NaN or +inf logit makes the row's
- * lse, logp and entropy NaN; a NaN is never an alternative. No counterpart in the reference, whose argmax_tok
+ * lse = log sum e^x; logp = x[target] - lse; entropy = -sum p log p (nats); and the alternatives. Sums in fp32. A target
+ * outside [0, vocab) has logp 0 (padding), a suppressed one -inf. Fewer than `top` ids with a logit above -inf: the rest
+ * have id -1 and -inf. No such id at all: lse -inf and entropy 0. A NaN or +inf logit makes the row's lse, logp and
+ * entropy NaN; a NaN is never an alternative. No counterpart in the reference, whose argmax_tok
  * (kernels/whisper.cu:451-493) keeps the choice only. */
 int mmz_token_logprobs(const void* logits, long long ldx, int type, int rows, int vocab, const unsigned char* sup,
-                       const int* target, float* logp, float* entropy, float* lse, int* top_id, float* top_logp,
-                       int top, long long ld, const int* col, void* stream);
+                       const mmz_logprobs* out, void* stream);
 /* mmz_token_logprobs of the logits x . emb^T, x [rows][ldx] and emb [vocab][d] fp16 (d a multiple of 64, 16-byte aligned
  * operands and row pitches): the product's fp32 sums are used as they are. scratch:
  * mmz_linear_logprobs_scratch_bytes bytes, 16-byte aligned, no initial contents required; launches that share it must
  * not overlap on the GPU. */
 unsigned long long mmz_linear_logprobs_scratch_bytes(int rows, int vocab, int d);
 int mmz_linear_logprobs(const void* x, long long ldx, const void* emb, int rows, int vocab, int d,
-                        const unsigned char* sup, const int* target, float* logp, float* entropy, float* lse,
-                        int* top_id, float* top_logp, int top, long long ld, const int* col, void* scratch,
-                        unsigned long long scratch_bytes, void* stream);
+                        const unsigned char* sup, const mmz_logprobs* out, void* scratch, unsigned long long scratch_bytes,
+                        void* stream);
 
 /* ---------------------------------------------------------------- token timestamps (host, src/align.rs) */
 

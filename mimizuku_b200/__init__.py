@@ -78,14 +78,13 @@ SIGNATURES = {
     "mmz_gemm_bias": (_I, [_P, _I, _P, _P, _P, _LL, _I, _I, _I, _I, _LL, _P]),
     "mmz_logits_argmax_scratch_bytes": (_ULL, []),
     "mmz_logits_argmax": (_I, [_P, _I, _P, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _ULL, _P]),
-    "mmz_kv8_write": (_I, [_P, _P, _LL, _LL, _LL, _P, _P, _P, _P, _LL, _LL, _LL, _LL, _P, _I, _I, _I, _I, _I, _I, _P]),
-    "mmz_kv8_read": (_I, [_P, _P, _P, _P, _LL, _LL, _LL, _LL, _P, _P, _LL, _LL, _LL, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "mmz_kv8_write": (_I, [_P, _P, _P, _LL, _LL, _LL, _P, _I, _I, _P]),
+    "mmz_kv8_read": (_I, [_P, _P, _P, _LL, _LL, _LL, _P, _P, _I, _I, _P]),
     "mmz_attn8_scratch_bytes": (_ULL, [_I, _I, _I, _I, _I, _I]),
-    "mmz_attn8": (_I, [_P, _LL, _LL, _LL, _P, _P, _P, _P, _LL, _LL, _LL, _LL, _P, _P, _LL, _LL, _LL, _I, _I, _I, _I, _I,
-                       _I, _I, _I, _F, _P, _P, _I, _P, _ULL, _P]),
-    "mmz_token_logprobs": (_I, [_P, _LL, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _LL, _P, _P]),
+    "mmz_attn8": (_I, [_P, _P, _P]),
+    "mmz_token_logprobs": (_I, [_P, _LL, _I, _I, _I, _P, _P, _P]),
     "mmz_linear_logprobs_scratch_bytes": (_ULL, [_I, _I, _I]),
-    "mmz_linear_logprobs": (_I, [_P, _LL, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _LL, _P, _P, _ULL, _P]),
+    "mmz_linear_logprobs": (_I, [_P, _LL, _P, _I, _I, _I, _P, _P, _P, _ULL, _P]),
     "mmz_times_from_cost": (_I, [_FP, _I, _I, _I, _FP]),
     "mmz_log_mel": (_I, [_FP, _L, _I, _FP, _IP]),
     "mmz_log_mel_gpu_work_bytes": (_ULL, [_I]),

@@ -138,50 +138,47 @@ int mmz_logits_argmax(const void* x, int ldx, const void* emb, int vocab, int d,
                                 advance != 0, scratch, (size_t)scratch_bytes, S(stream));
 }
 
-int mmz_kv8_write(const void* k, const void* v, long long x_seq, long long x_tok, long long x_head, void* k8, void* v8,
-                  float* ks, float* vs, long long c_seq, long long c_head, long long s_seq, long long s_head,
-                  const int* pos, int batch, int heads, int n, int cap, int block, int kind, void* stream) {
-    return launch_kv8_write(k, v, x_seq, x_tok, x_head, k8, v8, ks, vs, c_seq, c_head, s_seq, s_head, pos, batch, heads,
-                            n, cap, block, kind, S(stream));
+int mmz_kv8_write(const mmz_kv8* c, const void* k, const void* v, long long x_seq, long long x_tok, long long x_head,
+                  const int* pos, int batch, int n, void* stream) {
+    if (!c) return fail("kv8_write: null cache");
+    return launch_kv8_write(k, v, x_seq, x_tok, x_head, c->k, c->v, c->k_scale, c->v_scale, c->seq, c->head, c->scale_seq,
+                            c->scale_head, pos, batch, c->heads, n, c->cap, c->block, c->kind, S(stream));
 }
-int mmz_kv8_read(const void* k8, const void* v8, const float* ks, const float* vs, long long c_seq, long long c_head,
-                 long long s_seq, long long s_head, void* k, void* v, long long y_seq, long long y_tok,
-                 long long y_head, const int* pos, const int* lens, int batch, int heads, int n, int cap, int block,
-                 int kind, void* stream) {
-    return launch_kv8_read(k8, v8, ks, vs, c_seq, c_head, s_seq, s_head, k, v, y_seq, y_tok, y_head, pos, lens, batch,
-                           heads, n, cap, block, kind, S(stream));
+int mmz_kv8_read(const mmz_kv8* c, void* k, void* v, long long y_seq, long long y_tok, long long y_head, const int* pos,
+                 const int* lens, int batch, int n, void* stream) {
+    if (!c) return fail("kv8_read: null cache");
+    return launch_kv8_read(c->k, c->v, c->k_scale, c->v_scale, c->seq, c->head, c->scale_seq, c->scale_head, k, v, y_seq,
+                           y_tok, y_head, pos, lens, batch, c->heads, n, c->cap, c->block, c->kind, S(stream));
 }
 unsigned long long mmz_attn8_scratch_bytes(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     if (batch < 1 || rows < 1 || kv_heads < 1 || q_heads < kv_heads || cap < 1 || slots < 0) return 0;
     return attn8_scratch_bytes(batch, rows, q_heads, kv_heads, cap, slots);
 }
-int mmz_attn8(const void* q, long long q_seq, long long q_row, long long q_head, const void* k8, const void* v8,
-              const float* ks, const float* vs, long long c_seq, long long c_head, long long s_seq, long long s_head,
-              const int* lens, void* out, long long o_seq, long long o_row, long long o_head, int batch, int rows,
-              int q_heads, int kv_heads, int cap, int block, int kind, int causal, float scale, void* probs,
-              const int* pslot, int slots, void* scratch, unsigned long long scratch_bytes, void* stream) {
-    Attn8 a{(const __half*)q, (long)q_seq, (long)q_row, (long)q_head, (const uint8_t*)k8, (const uint8_t*)v8,
-                  ks, vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head, lens,
-                  (__half*)out, (long)o_seq, (long)o_row, (long)o_head, (__half*)probs, pslot, batch, rows, q_heads,
-                  kv_heads, cap, block, causal != 0, slots, scale};
-    a.p_seq = (long)slots * rows * cap;
-    return launch_attn8(a, kind, scratch, (size_t)scratch_bytes, S(stream));
+int mmz_attn8(const mmz_kv8* c, const mmz_attn8_args* x, void* stream) {
+    if (!c || !x) return fail("attn8: null cache or arguments");
+    Attn8 a{(const __half*)x->q, (long)x->q_seq, (long)x->q_row, (long)x->q_head, (const uint8_t*)c->k, (const uint8_t*)c->v,
+            c->k_scale, c->v_scale, (long)c->seq, (long)c->head, (long)c->scale_seq, (long)c->scale_head, x->lens,
+            (__half*)x->out, (long)x->o_seq, (long)x->o_row, (long)x->o_head, (__half*)x->probs, x->pslot, x->batch, x->rows,
+            x->q_heads, c->heads, c->cap, c->block, x->causal != 0, x->slots, x->scale};
+    a.p_seq = (long)x->slots * x->rows * c->cap;
+    return launch_attn8(a, c->kind, x->scratch, (size_t)x->scratch_bytes, S(stream));
+}
+static LogpOut logp_out(const mmz_logprobs* o) {
+    return {o->target, o->logp, o->entropy, o->lse, o->top_id, o->top_logp, (long)o->ld, o->col, o->top};
 }
 int mmz_token_logprobs(const void* logits, long long ldx, int type, int rows, int vocab, const unsigned char* sup,
-                       const int* target, float* logp, float* entropy, float* lse, int* top_id, float* top_logp,
-                       int top, long long ld, const int* col, void* stream) {
-    const LogpOut o{target, logp, entropy, lse, top_id, top_logp, (long)ld, col, top};
-    return launch_token_logprobs(logits, ldx, type, rows, vocab, sup, o, S(stream));
+                       const mmz_logprobs* o, void* stream) {
+    if (!o) return fail("token_logprobs: null outputs");
+    return launch_token_logprobs(logits, ldx, type, rows, vocab, sup, logp_out(o), S(stream));
 }
 unsigned long long mmz_linear_logprobs_scratch_bytes(int rows, int vocab, int d) {
     return rows < 1 || vocab < 1 || d < 64 ? 0 : linear_logprobs_scratch_bytes(rows, vocab, d);
 }
 int mmz_linear_logprobs(const void* x, long long ldx, const void* emb, int rows, int vocab, int d,
-                        const unsigned char* sup, const int* target, float* logp, float* entropy, float* lse,
-                        int* top_id, float* top_logp, int top, long long ld, const int* col, void* scratch,
-                        unsigned long long scratch_bytes, void* stream) {
-    const LogpOut o{target, logp, entropy, lse, top_id, top_logp, (long)ld, col, top};
-    return launch_linear_logprobs(x, ldx, emb, rows, vocab, d, sup, o, scratch, (size_t)scratch_bytes, S(stream));
+                        const unsigned char* sup, const mmz_logprobs* o, void* scratch, unsigned long long scratch_bytes,
+                        void* stream) {
+    if (!o) return fail("linear_logprobs: null outputs");
+    return launch_linear_logprobs(x, ldx, emb, rows, vocab, d, sup, logp_out(o), scratch, (size_t)scratch_bytes, S(stream));
 }
 
 int mmz_align_cost(const void* align, const int* rows, const int* cols, int n, int np, int max_t, int na, void* cost,

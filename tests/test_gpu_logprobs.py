@@ -6,9 +6,12 @@ exponentials; so log sum is off by E = (V / 256 + 64) 2^-23 + 2^-19, lse and a l
 the largest number involved. The entropy's second sum has terms e^d |d|: E times (1 + their weighted mean), taken with
 the mean of |d| from the 64-bit row. For hidden states, the products' sums are exact (operands on a grid), as in fp32.
 """
+import ctypes
+
 import numpy as np
 import pytest
 import torch
+from test_serving_args import Logprobs
 
 import mimizuku_b200 as m
 
@@ -152,9 +155,9 @@ def test_outputs_left_out(cuda, outputs):
     o = buffers(3, 4)
     P = lambda n: o[n].data_ptr() if n in outputs else None  # noqa: E731
     xd, td = x.cuda(), target.cuda()
-    rc = m.lib.mmz_token_logprobs(xd.data_ptr(), 5000, 1, 3, 5000, None, td.data_ptr() if "logp" in outputs else None,
-                                  P("logp"), P("entropy"), P("lse"), P("top_id"), P("top_logp"),
-                                  4 if "top_id" in outputs or "top_logp" in outputs else 0, 1, None,
+    out = Logprobs(td.data_ptr() if "logp" in outputs else None, P("logp"), P("entropy"), P("lse"), P("top_id"),
+                   P("top_logp"), 1, None, 4 if "top_id" in outputs or "top_logp" in outputs else 0)
+    rc = m.lib.mmz_token_logprobs(xd.data_ptr(), 5000, 1, 3, 5000, None, ctypes.byref(out),
                                   torch.cuda.current_stream().cuda_stream)
     assert rc == 0
     torch.cuda.synchronize()

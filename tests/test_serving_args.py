@@ -1,4 +1,6 @@
 """The 8-bit cache and the log probabilities refuse bad arguments on the host, before a device is touched."""
+import ctypes
+
 import pytest
 
 import mimizuku_b200 as m
@@ -7,14 +9,53 @@ L = m.lib
 A = 1 << 20  # an aligned address that nothing reads
 
 
-def write(k=A, v=A, xs=(64, 64, 64), k8=A, v8=A, ks=A, vs=A, cs=(6400, 6400), batch=1, heads=1, n=1, cap=100, block=64,
-          kind=0):
-    return L.mmz_kv8_write(k, v, *xs, k8, v8, ks, vs, *cs, 2, 2, None, batch, heads, n, cap, block, kind, None)
+class Kv8(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, ctypes.c_longlong) for n in ("seq", "head", "scale_seq", "scale_head")] + [
+        (n, ctypes.c_int) for n in ("heads", "cap", "block", "kind")]
 
 
-def read(k=A, v=A, xs=(64, 64, 64), k8=A, v8=A, ks=A, vs=A, cs=(6400, 6400), batch=1, heads=1, n=1, cap=100, block=64,
-         kind=0):
-    return L.mmz_kv8_read(k8, v8, ks, vs, *cs, 2, 2, k, v, *xs, None, None, batch, heads, n, cap, block, kind, None)
+class Attn8(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("qs", ctypes.c_longlong * 3), ("out", ctypes.c_void_p),
+                ("os", ctypes.c_longlong * 3)] + [(n, ctypes.c_void_p) for n in ("lens", "probs", "pslot", "scratch")] + [
+        ("scratch_bytes", ctypes.c_ulonglong)] + [(n, ctypes.c_int) for n in ("batch", "rows", "q_heads", "slots", "causal")] + [
+        ("scale", ctypes.c_float)]
+
+
+class Logprobs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("target", "logp", "entropy", "lse", "top_id", "top_logp")] + [
+        ("ld", ctypes.c_longlong), ("col", ctypes.c_void_p), ("top", ctypes.c_int)]
+
+
+def cache(k8=A, v8=A, ks=A, vs=A, cs=(6400, 6400), heads=1, cap=100, block=64, kind=0):
+    return Kv8(k8, v8, ks, vs, *cs, 2, 2, heads, cap, block, kind)
+
+
+def write(k=A, v=A, xs=(64, 64, 64), batch=1, n=1, **kw):
+    return L.mmz_kv8_write(ctypes.byref(cache(**kw)), k, v, *xs, None, batch, n, None)
+
+
+def read(k=A, v=A, xs=(64, 64, 64), batch=1, n=1, **kw):
+    return L.mmz_kv8_read(ctypes.byref(cache(**kw)), k, v, *xs, None, None, batch, n, None)
+
+
+def test_structs_are_packed_as_the_header_has_them():
+    from mimizuku_b200 import serving
+    for packed, there in ((serving._KV8, Kv8), (serving._ATTN8, Attn8), (serving._LOGPROBS, Logprobs)):
+        assert packed.size == ctypes.sizeof(there)
+    raw = serving._ATTN8.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18, 0.5)
+    a = Attn8.from_buffer_copy(raw)
+    assert (a.q, *a.qs, a.out, *a.os) == tuple(range(1, 9)) and (a.lens, a.probs, a.pslot, a.scratch) == (9, 10, 11, 12)
+    assert (a.scratch_bytes, a.batch, a.rows, a.q_heads, a.slots, a.causal, a.scale) == (13, 14, 15, 16, 17, 18, 0.5)
+    k = Kv8.from_buffer_copy(serving._KV8.pack(*range(1, 13)))
+    assert [getattr(k, f[0]) for f in Kv8._fields_] == list(range(1, 13))
+    o = Logprobs.from_buffer_copy(serving._LOGPROBS.pack(*range(1, 10)))
+    assert [getattr(o, f[0]) for f in Logprobs._fields_] == list(range(1, 10))
+    for call in (lambda: L.mmz_kv8_write(None, A, A, 64, 64, 64, None, 1, 1, None), lambda: L.mmz_attn8(None, None, None),
+                 lambda: L.mmz_kv8_read(None, A, A, 64, 64, 64, None, None, 1, 1, None),
+                 lambda: L.mmz_token_logprobs(A, 9, 0, 1, 9, None, None, None),
+                 lambda: L.mmz_linear_logprobs(A, 64, A, 1, 9, 64, None, None, None, 0, None)):
+        assert call() == -1 and b"null" in L.mmz_last_error()
 
 
 @pytest.mark.parametrize("fn,name", [(write, b"kv8_write"), (read, b"kv8_read")])
@@ -43,10 +84,11 @@ def test_nothing_to_do_is_no_error():
     assert logits(rows=0, x=None) == 0 and hidden(rows=0, x=None) == 0
 
 
-def attend(q=A, qs=(64, 64, 64), k8=A, cs=(6400, 6400), ks=A, out=A, os=(64, 64, 64), batch=1, rows=1, hq=1, hkv=1, cap=100,
-           block=64, kind=0, probs=None, pslot=None, slots=0, scratch=None, sb=0):
-    return L.mmz_attn8(q, *qs, k8, A, ks, A, *cs, 2, 2, None, out, *os, batch, rows, hq, hkv, cap, block, kind, 0, 0.125,
-                       probs, pslot, slots, scratch, sb, None)
+def attend(q=A, qs=(64, 64, 64), out=A, os=(64, 64, 64), batch=1, rows=1, hq=1, hkv=1, probs=None, pslot=None, slots=0,
+           scratch=None, sb=0, **kw):
+    a = Attn8(q, (ctypes.c_longlong * 3)(*qs), out, (ctypes.c_longlong * 3)(*os), None, probs, pslot, scratch, sb, batch, rows,
+              hq, slots, 0, 0.125)
+    return L.mmz_attn8(ctypes.byref(cache(heads=hkv, **kw)), ctypes.byref(a), None)
 
 
 @pytest.mark.parametrize("bad,word", [
@@ -65,13 +107,16 @@ def test_attention_refuses(bad, word):
     assert b"attn8" in msg and word in msg
 
 
-def logits(x=A, ldx=100, type=0, rows=1, vocab=100, target=A, logp=A, top=0, ld=1):
-    return L.mmz_token_logprobs(x, ldx, type, rows, vocab, None, target, logp, None, None, None, None, top, ld, None, None)
+def outs(target=A, logp=A, top=0, ld=1):
+    return ctypes.byref(Logprobs(target, logp, None, None, None, None, ld, None, top))
 
 
-def hidden(x=A, ldx=64, emb=A, rows=1, vocab=100, d=64, target=A, logp=A, top=0, ld=1, scratch=None, sb=0):
-    return L.mmz_linear_logprobs(x, ldx, emb, rows, vocab, d, None, target, logp, None, None, None, None, top, ld, None,
-                                 scratch, sb, None)
+def logits(x=A, ldx=100, type=0, rows=1, vocab=100, **kw):
+    return L.mmz_token_logprobs(x, ldx, type, rows, vocab, None, outs(**kw), None)
+
+
+def hidden(x=A, ldx=64, emb=A, rows=1, vocab=100, d=64, scratch=None, sb=0, **kw):
+    return L.mmz_linear_logprobs(x, ldx, emb, rows, vocab, d, None, outs(**kw), scratch, sb, None)
 
 
 @pytest.mark.parametrize("bad,word", [
