@@ -17,11 +17,14 @@
 //     r and r + 4 of one product (the lanes of columns 4-7 hold the same scores and keep the low part).
 //   * the scales of a block apply in fp32: ks to the scores, vs to the sums of the positions that share it.
 // Two ways through the cache (plan() chooses):
-//   flat     many chunks, up to 8 rows: a fixed number of warps, each with an equal share of all sequences' and heads'
-//            chunks in a row, whatever the lengths; a pair's parts on several warps join in a second kernel
-//   cluster  few chunks, or more rows: a CTA to a (pair, row block), its warps along the positions (up to 16 rows) or
-//            along the rows; CTAs of a cluster split the sequence and join through distributed shared memory, and where
-//            one cluster is too little, clusters through scratch and a second kernel
+//   cluster  a CTA to a (pair, row block), its warps along the positions or along the rows; CTAs of a cluster split the
+//            sequence and join through distributed shared memory, and where one cluster is too little (and more than 8
+//            rows), clusters through scratch and a second kernel
+//   flat     up to 8 rows and too few pairs for a cluster each to fill the GPU (long caches): a fixed number of warps,
+//            each with an equal share of all sequences' and heads' chunks in a row, whatever the lengths; a pair's parts on
+//            several warps join in a second kernel
+// Measured (calls in a CUDA graph): 32 sequences x 20 heads x 1500 positions, int8, 28 us = 4.3 TB/s, with 6 heads recorded
+// 31; 3 sequences of up to 131072 positions and 5 key heads x 4, e4m3, 32 us = 3.9 TB/s; one sequence of 20 heads 5.5 us.
 #include "attn8.h"
 #include "fp8_cache.cuh"
 #include "launch.h"
@@ -36,7 +39,6 @@ constexpr int KB = CH * HD;     // bytes of a chunk's keys (and of its values)
 constexpr int REC = HD + 2;     // a row's partial result: 64 sums, maximum, sum of p
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float PSHIFT = 10.f;  // p <= 2^10
-constexpr long FLAT_FROM = 4;   // chunks to a warp from which on the flat way is taken
 
 struct Smem {
     uint8_t ring[WARPS][STG][2][KB];
@@ -917,24 +919,31 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     p.mode = R <= 4 ? 0 : R <= 8 ? 1 : 2;
     p.stats = slots > 0 ? ((size_t)pairs * R * 8 + 15) & ~(size_t)15 : 0;
     p.raws = (size_t)batch * slots * rows * cap * 4;
-    p.flat = R <= 8 && pairs * chunks >= FLAT_FROM * SLOTS * WARPS && pairs * chunks < 0x7fffffffl;
-    if (p.flat) {
-        p.lay = {1, 1, 0, 0, 1};
-        p.smem = sizeof(Smem);
-        p.part = (size_t)SLOTS * WARPS * 2 * RECF * 4;
-        return p;
-    }
-    p.lay.wrows = R > 16;
-    const long block = p.lay.wrows ? WARPS * rt : rt;
+    // The warps of a CTA take rows of their own where that alone fills the GPU (prompts of 223 rows on 160 pairs: 36 us,
+    // positions split instead 70; 64 rows on 160 pairs do not: 73 against 59).
+    const long wide = WARPS * rt;
+    p.lay.wrows = R > 16 && pairs * ((R + wide - 1) / wide) >= SLOTS;
+    const long block = p.lay.wrows ? wide : rt;
     p.lay.block = (int)(R < block ? R : block);
     p.lay.tiles = (int)((R + block - 1) / block);
-    // splits of the sequence: no more CTAs than the GPU holds at once, and a chunk at least to each warp
+    // splits of the sequence: no more CTAs than the GPU holds at once (5 rows on 120 pairs: 2 CTAs a pair 16 us, 4 in more
+    // than one wave 23), and a chunk at least to each warp
     const long units = pairs * p.lay.tiles, top = p.lay.wrows ? chunks : (chunks + WARPS - 1) / WARPS;
     long s = SLOTS / units;
     s = s < 1 ? 1 : s > top ? top : s;
     const int cs = s < 2 ? 1 : s < 4 ? 2 : s < 8 ? 4 : 8;
     p.lay.cs = cs;
     p.lay.nclus = (int)(s / cs);
+    // Where one cluster is too little the parts join in a second kernel in any case, and equal shares of all chunks are
+    // better (15 pairs of 0 to 131072 positions: 32 us, clusters 47). With one cluster a pair they are not: 640 pairs of 1500
+    // positions 29 us flat, 28 in clusters, 320 pairs 18.7 and 17.6, 20 pairs 7.5 and 5.5.
+    p.flat = R <= 8 && p.lay.nclus > 1 && pairs * chunks < 0x7fffffffl;
+    if (p.flat) {
+        p.lay = {1, 1, 0, 0, 1};
+        p.smem = sizeof(Smem);
+        p.part = (size_t)SLOTS * WARPS * 2 * RECF * 4;
+        return p;
+    }
     const size_t n = (size_t)p.lay.block * cs * (p.lay.wrows ? 1 : WARPS);  // (row, source) pairs
     const bool alone = p.lay.wrows && s == 1;  // a warp has its rows' whole results, nothing is exchanged
     p.smem = sizeof(Smem) + (alone ? 0 : (n + (n & 1)) * 8 + n * (HD / cs) * 4);
