@@ -174,7 +174,7 @@ int mmz_logits_argmax(const void* x, int ldx, const void* emb, int vocab, int d,
 
 /* ---------------------------------------------------------------- the 8-bit key/value cache (device pointers)
  * No counterpart in the reference, whose caches are fp16 (src/model.rs:440-455). value = code * scale. fp16 tensors are
- * 16-byte aligned with strides (in values) that are multiples of 8. */
+ * 16-byte aligned with strides (in values) that are multiples of 8; no two rows of one that is written may overlap. */
 
 typedef struct {
     void *k, *v;              /* codes [batch][heads][cap][64], one byte each, a head's rows one after another */

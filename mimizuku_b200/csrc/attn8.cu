@@ -1021,6 +1021,7 @@ int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, 
     const long jblocks = (jall + jrows - 1) / jrows;
     const long post = jblocks + (long)a.batch * slots * a.rows;
     if (grid > 0x7fffffffl || post > 0x7fffffffl) return fail("attn8: more than 2^31 blocks in one call");
+    if (!apart(HD, {{a.batch, a.o_seq}, {a.rows, a.o_row}, {a.q_heads, a.o_head}})) return fail("attn8: rows of out overlap");
     const size_t need = p.part + p.stats + p.raws;
     if (need && (!scratch || ((uintptr_t)scratch & 15) || scratch_bytes < need))
         return fail("attn8: scratch too small or not 16-byte aligned");

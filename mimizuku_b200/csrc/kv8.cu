@@ -14,8 +14,6 @@
 // values: written in 68 us = 5.4 TB/s, read back in 55 us = 6.7 TB/s. A warp takes 32 tokens of one block (8 lanes to a token, 16
 // bytes each), so that its 8 loads are all in flight before the maximum is known and the values are read once; blocks
 // of 64 and 128 tokens are shared by 2 and 4 warps of the CTA, which exchange their maxima in shared memory.
-#include <cstdlib>
-
 #include "fp8_cache.cuh"
 #include "launch.h"
 
@@ -216,11 +214,6 @@ int launch_kv8_write(const void* k, const void* v, long long x_seq, long long x_
                   kind))
         return -1;
     if (batch == 0 || n == 0) return 0;
-    // two sequences or heads in one place would be written by two blocks at once
-    const long long room = (long long)cap * HD, scales = (cap + block - 1) / block;
-    if ((batch > 1 && (llabs(c_seq) < room || llabs(s_seq) < scales)) ||
-        (heads > 1 && (llabs(c_head) < room || llabs(s_head) < scales)))
-        return fail("kv8_write: the cache's sequences and heads overlap");
     // blocks that n tokens can touch, from any position
     const int most = (cap + block - 1) / block;
     const long touched = pos ? ((long)n + block - 2) / block + 1 : ((long)n + block - 1) / block;
@@ -229,6 +222,9 @@ int launch_kv8_write(const void* k, const void* v, long long x_seq, long long x_
     const int per = block <= 32 ? 4 : 128 / block;
     const long grid = (items + per - 1) / per;
     if (items > 0xffffff00l || grid > 0x7fffffffl) return fail("kv8_write: more than 2^31 blocks in one call");
+    // two sequences or heads in one place would be written by two blocks at once
+    if (!apart((long long)cap * HD, {{batch, c_seq}, {heads, c_head}}) || !apart(most, {{batch, s_seq}, {heads, s_head}}))
+        return fail("kv8_write: the cache's sequences and heads overlap");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     const Cache c{(uint8_t*)k8, (uint8_t*)v8, ks, vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head};
@@ -248,6 +244,7 @@ int launch_kv8_read(const void* k8, const void* v8, const float* ks, const float
     if (batch == 0 || n == 0) return 0;
     const long tiles = ((long)n + 127) / 128, grid = (long)batch * heads * 2 * tiles;
     if (grid > 0x7fffffffl) return fail("kv8_read: more than 2^31 blocks in one call");
+    if (!apart(HD, {{batch, y_seq}, {n, y_tok}, {heads, y_head}})) return fail("kv8_read: tokens of k and v overlap");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     const Cache c{(uint8_t*)k8, (uint8_t*)v8, (float*)ks, (float*)vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head};

@@ -5,6 +5,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <initializer_list>
+#include <utility>
+
 #include "attn8.h"
 #include "logprobs.h"
 
@@ -33,6 +37,22 @@ int failf(const char* fmt, ...);
 const char* last_error();
 // cudaGetLastError after a launch: 0 or fail
 int check_launch(const char* what);
+
+// Whether items of `room` elements, laid out by nested dimensions of (count, stride), lie apart from one another. Layouts
+// that are not nested (no order of the dimensions in which each stride spans the dimensions inside it) count as overlapping.
+inline bool apart(long long room, std::initializer_list<std::pair<int, long long>> dims) {
+    std::pair<unsigned long long, int> d[4];
+    int n = 0;
+    for (const auto& x : dims)
+        if (x.first > 1) d[n++] = {x.second < 0 ? 0ull - (unsigned long long)x.second : (unsigned long long)x.second, x.first};
+    std::sort(d, d + n);
+    unsigned __int128 extent = room;
+    for (int i = 0; i < n; i++) {
+        if (d[i].first < extent) return false;
+        extent += (unsigned __int128)d[i].first * (d[i].second - 1);
+    }
+    return true;
+}
 
 // fp16 tensor maps; swizzle: 0 (none), 64 or 128 (bytes)
 int make_tmap_2d(CUtensorMap* map, const void* base, const uint64_t dims[2], const uint64_t strides[1],

@@ -77,6 +77,21 @@ def test_a_cache_that_overlaps_is_read_only():
         assert write(**bad) == -1 and b"overlap" in L.mmz_last_error()
 
 
+def test_sequences_that_start_where_heads_do_overlap():
+    # each stride alone is wide enough: sequence 1's first head lies on sequence 0's second
+    assert write(batch=2, heads=2, cs=(6400, 6400)) == -1 and b"overlap" in L.mmz_last_error()
+    assert write(batch=2, heads=2, cs=(12800, 6400)) == -1 and b"overlap" in L.mmz_last_error()  # (the scales: 2 and 2)
+
+
+def test_outputs_in_one_place_are_refused():
+    for xs in ((0, 64, 64), (64, 128, 128), (4096, 64, 64), (1024, 64, 120)):
+        assert read(batch=2, n=2, heads=2, xs=xs) == -1 and b"overlap" in L.mmz_last_error()
+        assert attend(batch=2, rows=2, hq=2, hkv=2, os=xs) == -1 and b"overlap" in L.mmz_last_error()
+    for xs in ((256, 128, 64), (64, 256, 128), (-256, 64, 128), (1 << 62, 128, 64)):  # any order that nests is one
+        assert attend(batch=2, rows=2, hq=2, hkv=2, os=xs, probs=A, pslot=A, slots=1) == -1
+        assert b"scratch" in L.mmz_last_error()  # the next check
+
+
 def test_nothing_to_do_is_no_error():
     assert write(batch=0, k=None) == 0 and write(n=0, k=None) == 0
     assert read(batch=0) == 0 and read(n=0) == 0
