@@ -914,6 +914,11 @@ struct Plan {
     Lay lay;
     size_t smem, part, stats, raws;
 };
+// sizes that the products below can take; a call's blocks and scratch are fewer
+bool sizes_ok(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
+    return within(0x7fffff00l, {rows, q_heads / kv_heads}) && within(1l << 40, {batch, rows, q_heads}) &&
+           within(1l << 46, {batch, rows, slots, cap});
+}
 Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     Plan p;
     const long R = (long)rows * (q_heads / kv_heads), pairs = (long)batch * kv_heads, chunks = ((long)cap + CH - 1) / CH;
@@ -987,6 +992,7 @@ int launch_mode(const Attn8& a, const Plan& p, float* part, float2* stats, float
 }  // namespace
 
 size_t attn8_scratch_bytes(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
+    if (!sizes_ok(batch, rows, q_heads, kv_heads, cap, slots)) return 0;
     const Plan p = plan(batch, rows, q_heads, kv_heads, cap, slots);
     return p.part + p.stats + p.raws;
 }
@@ -1012,7 +1018,7 @@ int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, 
         return fail("attn8: strides of q and out multiples of 8 values");
     if ((a.c_seq | a.c_head) & 15) return fail("attn8: strides of the cache multiples of 16 bytes");
     const int slots = a.probs ? a.slots : 0;
-    if ((long)a.rows * (a.q_heads / a.kv_heads) > 0x7fffff00l) return fail("attn8: too many rows in one call");
+    if (!sizes_ok(a.batch, a.rows, a.q_heads, a.kv_heads, a.cap, slots)) return fail("attn8: too many rows in one call");
     const Plan p = plan(a.batch, a.rows, a.q_heads, a.kv_heads, a.cap, slots);
     const long grid = (long)a.batch * a.kv_heads * p.lay.tiles * p.lay.nclus * p.lay.cs;
     // rows with parts: one to a warp, or where a row has more than 32 parts or so one to a block

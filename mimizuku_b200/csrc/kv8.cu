@@ -218,10 +218,10 @@ int launch_kv8_write(const void* k, const void* v, long long x_seq, long long x_
     const int most = (cap + block - 1) / block;
     const long touched = pos ? ((long)n + block - 2) / block + 1 : ((long)n + block - 1) / block;
     const int nblk = (int)(touched < most ? touched : most);
-    const long items = (long)batch * heads * 2 * nblk;
     const int per = block <= 32 ? 4 : 128 / block;
-    const long grid = (items + per - 1) / per;
-    if (items > 0xffffff00l || grid > 0x7fffffffl) return fail("kv8_write: more than 2^31 blocks in one call");
+    if (!within(std::min(0xffffff00l, 0x7fffffffl * per), {batch, heads, 2, nblk}))
+        return fail("kv8_write: more than 2^31 blocks in one call");
+    const long items = (long)batch * heads * 2 * nblk, grid = (items + per - 1) / per;
     // two sequences or heads in one place would be written by two blocks at once
     if (!apart((long long)cap * HD, {{batch, c_seq}, {heads, c_head}}) || !apart(most, {{batch, s_seq}, {heads, s_head}}))
         return fail("kv8_write: the cache's sequences and heads overlap");
@@ -242,8 +242,9 @@ int launch_kv8_read(const void* k8, const void* v8, const float* ks, const float
                   kind))
         return -1;
     if (batch == 0 || n == 0) return 0;
-    const long tiles = ((long)n + 127) / 128, grid = (long)batch * heads * 2 * tiles;
-    if (grid > 0x7fffffffl) return fail("kv8_read: more than 2^31 blocks in one call");
+    const long tiles = ((long)n + 127) / 128;
+    if (!within(0x7fffffffl, {batch, heads, 2, tiles})) return fail("kv8_read: more than 2^31 blocks in one call");
+    const long grid = (long)batch * heads * 2 * tiles;
     if (!apart(HD, {{batch, y_seq}, {n, y_tok}, {heads, y_head}})) return fail("kv8_read: tokens of k and v overlap");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);

@@ -38,6 +38,15 @@ const char* last_error();
 // cudaGetLastError after a launch: 0 or fail
 int check_launch(const char* what);
 
+// whether a product of numbers >= 0 is at most `most`
+inline bool within(long long most, std::initializer_list<long long> factors) {
+    unsigned __int128 p = 1;
+    for (long long f : factors) {
+        if (f == 0) return true;
+        if (p <= (unsigned long long)most) p *= (unsigned long long)f;
+    }
+    return p <= (unsigned long long)most;
+}
 // Whether items of `room` elements, laid out by nested dimensions of (count, stride), lie apart from one another. Layouts
 // that are not nested (no order of the dimensions in which each stride spans the dimensions inside it) count as overlapping.
 inline bool apart(long long room, std::initializer_list<std::pair<int, long long>> dims) {

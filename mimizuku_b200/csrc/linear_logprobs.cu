@@ -582,11 +582,11 @@ Plan plan(int rows, int V) {
     p.tr = p.pairs ? 256 : p.quarters ? 32 : 128;
     p.bn = p.pairs ? pair::BN : one::UNIT;
     p.halves = p.pairs ? 2 : p.quarters ? 4 : 1;
-    const int mt = (rows + p.tr - 1) / p.tr, nt = (V + p.bn - 1) / p.bn, most = p.pairs ? PAIRS : 2 * PAIRS;
-    const long T = (long)mt * nt;
+    const long mt = ((long)rows + p.tr - 1) / p.tr, nt = ((long)V + p.bn - 1) / p.bn, most = p.pairs ? PAIRS : 2 * PAIRS;
+    const long T = mt * nt;
     p.workers = (int)(T < most ? T : most);
-    const int per = (int)(T / p.workers);
-    p.parts = (nt + per - 1) / per + 1;  // workers that a row tile's vocabulary can lie on
+    const long per = T / p.workers;
+    p.parts = (int)((nt + per - 1) / per) + 1;  // workers that a row tile's vocabulary can lie on
     if (p.parts > p.workers) p.parts = p.workers;
     p.bytes = (size_t)mt * p.parts * p.halves * FIELDS * p.tr * 4;
     return p;

@@ -162,6 +162,21 @@ def test_scratch_sizes():
     assert m.linear_logprobs_scratch_bytes(7, 51866, 1280) % 16 == 0
 
 
+def test_sizes_whose_products_pass_64_bits():
+    big, top = 1 << 30, 0x7fffffff
+    for rows, vocab in ((top, top), (top, 1), (1, top), (top, 1 << 30), (0x7fffff01, 0x40000000)):
+        assert L.mmz_linear_logprobs_scratch_bytes(rows, vocab, 64) > 0
+    for dims in ((big, top, big, big, top, 0), (big, top, big, 1, 1, 0), (top, top, 1, 1, top, top), (1 << 16, 1, 1, 1, 1 << 24, 1 << 24)):
+        assert L.mmz_attn8_scratch_bytes(*dims) == 0
+    wide = 1 << 40
+    for bad in (dict(batch=big, heads=big, n=16), dict(batch=big, heads=1 << 31 >> 1, n=64)):
+        for call in (write, read):
+            assert call(cs=(wide, 6400), **bad) == -1 and b"2^31" in L.mmz_last_error()
+    for bad in (dict(batch=big, rows=0x7fffff00, hq=big, hkv=big), dict(batch=big, hq=big, hkv=1),
+                dict(batch=1 << 16, slots=1 << 24, cap=1 << 24, probs=A, pslot=A, scratch=A, sb=1 << 30)):
+        assert attend(**bad) == -1 and b"attn8: too many rows" in L.mmz_last_error()
+
+
 def test_python_calls_refuse_what_is_no_cuda_tensor():
     import torch
     k8 = torch.zeros((1, 2, 8, 64), dtype=torch.int8)
