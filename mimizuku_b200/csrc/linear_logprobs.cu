@@ -218,9 +218,10 @@ __global__ void __launch_bounds__(one::NTHREADS, 1)
                     if (++st == NS) st = 0, ph++;
                 }
             }
-            if (*abort)  // let every issued copy land before the shared memory is released
-                for (int q = issued > NS ? issued - NS : 0; q < issued; q++)
-                    mbar_wait(&s.full[q % NS], (q / NS) & 1, nullptr, limit_ns, nullptr, 0, 0);
+            // the last copies land before the shared memory is released, whoever's wait gave up (else the issuer waits for
+            // them too)
+            for (int q = issued > NS ? issued - NS : 0; q < issued; q++)
+                mbar_wait(&s.full[q % NS], (q / NS) & 1, nullptr, limit_ns, nullptr, 0, 0);
         }
     } else if (warp == 5) {
         // ---------------------------------------------------------------- MMA issuer
@@ -385,9 +386,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::NTHREADS, 1)
                 }
                 if (!ok) break;
             }
-            // let the copies counted on this CTA's barriers land before shared memory is released (the odd CTA's land on
-            // the even CTA's barriers, which the even CTA waits for here; the pair leaves together)
-            if (*abort && lead)
+            // the last copies land before shared memory is released, whoever's wait gave up: both CTAs' are counted on the
+            // even CTA's barriers, and the pair leaves together
+            if (lead)
                 for (int q = issued > NS ? issued - NS : 0; q < issued; q++)
                     mbar_wait(&s.full[q % NS], (q / NS) & 1, nullptr, limit_ns, nullptr, 0, 0);
         }

@@ -132,9 +132,9 @@ __global__ void __launch_bounds__(NT + 32, 2)
                     bulk_g2s(sm.ring[st], (const uint8_t*)(w.x + w.head) + 16l * p, bytes, &sm.full[st]);
                 }
             }
-            if (!ok)  // a wait gave up: let the copies in flight land before the CTA ends
-                for (unsigned i = q > NS ? q - NS : 0; i < q; i++)
-                    mbar_wait(&sm.full[i % NS], (i / NS) & 1, nullptr, limit_ns, nullptr, 0, 0);
+            // the last copies land before the CTA ends, whoever's wait gave up (else the consumers wait for them too)
+            for (unsigned i = q > NS ? q - NS : 0; i < q; i++)
+                mbar_wait(&sm.full[i % NS], (i / NS) & 1, nullptr, limit_ns, nullptr, 0, 0);
         }
         __syncwarp();
         if (cl > 1) {
