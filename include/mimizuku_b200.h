@@ -389,7 +389,8 @@ int mmz_engine_xkv(mmz_engine* e);
 int mmz_engine_set_logprobs(mmz_engine* e, int on);
 int mmz_engine_logprobs(mmz_engine* e);
 /* The last mmz_engine_transcribe's (or _transcribe_audio's) log probabilities and entropies, [n][max_t] each on the
- * host (either may be NULL): those of the generated tokens, the end-of-text token included; 0 elsewhere. */
+ * host (either may be NULL): those of the generated tokens, the end-of-text token included; 0 elsewhere. An error where
+ * none was done since mmz_engine_set_logprobs or mmz_engine_reset. */
 int mmz_engine_read_logprobs(mmz_engine* e, float* logp, float* entropy);
 /* Device address of an engine buffer: "tok", "done", "ctr", "align", "logits", "eh", "eqkv", "eatt", "xkv", "mel",
  * "kc", "vc", "x", "hb", "att", "aslot", "logp", "entropy" (NULL before mmz_engine_set_logprobs); NULL if unknown. */

@@ -899,16 +899,17 @@ int Engine::set_logprobs(int on) {
         if (!ent_) ent_ = (float*)alloc(n);
         if (!logp_ || !ent_) return fail("set_logprobs: device memory allocation failed");
     }
+    last_lens_.clear();  // an earlier transcription left none
     logprobs_ = on == 1;
     static_cast<NativeKernels*>(k_.get())->keep_logits = logprobs_ ? logits_ : nullptr;
     return 0;
 }
 
 int Engine::read_logprobs(float* logp, float* entropy) {
-    if (!logprobs_) return fail("read_logprobs: set_logprobs(1) and a transcription come first");
+    if (!logprobs_ || last_lens_.empty()) return fail("read_logprobs: set_logprobs(1) and a transcription come first");
     const int mt = dm_.max_t, n = (int)last_lens_.size();
     for (auto [to, from] : {std::pair<float*, float*>{logp, logp_}, {entropy, ent_}}) {
-        if (!to || !n) continue;
+        if (!to) continue;
         CUDA_CK(cudaMemcpyAsync(to, from, (size_t)n * mt * 4, cudaMemcpyDeviceToHost, st_));
         CUDA_CK(cudaStreamSynchronize(st_));
         for (int s = 0; s < n; s++)  // what the steps left outside the generated tokens means nothing
@@ -954,6 +955,7 @@ int Engine::set_enc_attn(int unfused) {
 }
 
 int Engine::reset(const int* prompts, int b, int np) {
+    last_lens_.clear();
     if (b < 1 || b > bmax_ || np < 1 || np >= dm_.max_t) return fail("reset: bad batch or prompt");
     const int mt = dm_.max_t;
     std::vector<int> t((size_t)b * mt, 0);

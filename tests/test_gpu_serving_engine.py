@@ -154,3 +154,20 @@ def test_settings_refuse(cuda):
         e.xkv = "int4"
     assert e.xkv == "fp16" and not e.logprobs
     e.close()
+
+
+def test_logprobs_are_those_of_a_transcription_since_the_setting(cuda):
+    mel, frames = clips(1)
+    e = engine(1)
+    read = lambda: m.lib.mmz_engine_read_logprobs(e._h, None, None)
+    e.transcribe(mel, frames, max_new=2)
+    e.logprobs = True  # after the transcription, which left none
+    assert read() == -1 and b"a transcription come first" in m.lib.mmz_last_error()
+    e.transcribe(mel, frames, max_new=2)
+    assert read() == 0
+    e.reset(np.array([m.TINY.prompt], np.int32))  # the next steps write over them
+    assert read() == -1
+    e.logprobs = False
+    e.logprobs = True
+    assert read() == -1
+    e.close()
