@@ -1,15 +1,18 @@
 """Builds libmimizuku_b200.so in-tree: the sm_100a kernels (nvcc, -gencode arch=compute_100a,code=sm_100a), the C++
-engine and CPU stages, linked against cuBLAS with a static CUDA runtime.
+engine and CPU stages, linked against cuBLAS with a static CUDA runtime; and, where torch is installed, the compiled
+calls over torch tensors (_serving.so).
 
     python mimizuku_b200/build.py [--force] [-j N]      (by path: importing the package needs the library)
 
 Objects go to mimizuku_b200/_build/; a source is recompiled when it or a header changed.
 """
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -32,6 +35,9 @@ HEADERS = ["common.cuh", "launch.h", "engine.h", "host_cpu.h", "ln_row.cuh", "ge
 # kernels under the reference's own names, as an image its host loads by name (not linked into the library)
 DROPIN_SRC = os.path.join(CSRC, "dropin.cu")
 DROPIN = os.path.join(HERE, "dropin_sm100a.fatbin")
+# the calls over torch tensors: a Python module that links the library (which itself knows nothing of torch or Python)
+SERVING_SRC = os.path.join(CSRC, "serving.cpp")
+SERVING = os.path.join(HERE, "_serving.so")
 
 
 def _newest_header():
@@ -84,6 +90,21 @@ def build(force=False, jobs=None, verbose=False):
         shutil.move(tmp, LIB)
         if verbose:
             print(f"built {LIB}")
+    torch = importlib.util.find_spec("torch")
+    if torch and (force or not os.path.exists(SERVING) or os.path.getmtime(SERVING) < max(os.path.getmtime(SERVING_SRC), hdr)):
+        at = torch.submodule_search_locations[0]
+        cmd = [os.environ.get("CXX", "g++")] + CXX_FLAGS + [
+            "-shared", SERVING_SRC, "-o", SERVING + ".tmp", "-I", os.path.join(HERE, "..", "include"),
+            "-isystem", sysconfig.get_path("include"), "-isystem", os.path.join(at, "include"),
+            "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"), f"-L{HERE}",
+            "-l:" + os.path.basename(LIB), "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda",
+            "-lc10", "-Wl,-rpath,$ORIGIN"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"build failed:\n{' '.join(cmd)}\n{r.stdout}{r.stderr}")
+        shutil.move(SERVING + ".tmp", SERVING)
+        if verbose:
+            print(f"built {SERVING}")
     return LIB
 
 

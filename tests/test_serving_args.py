@@ -39,18 +39,7 @@ def read(k=A, v=A, xs=(64, 64, 64), batch=1, n=1, **kw):
     return L.mmz_kv8_read(ctypes.byref(cache(**kw)), k, v, *xs, None, None, batch, n, None)
 
 
-def test_structs_are_packed_as_the_header_has_them():
-    from mimizuku_b200 import serving
-    for packed, there in ((serving._KV8, Kv8), (serving._ATTN8, Attn8), (serving._LOGPROBS, Logprobs)):
-        assert packed.size == ctypes.sizeof(there)
-    raw = serving._ATTN8.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18, 0.5)
-    a = Attn8.from_buffer_copy(raw)
-    assert (a.q, *a.qs, a.out, *a.os) == tuple(range(1, 9)) and (a.lens, a.probs, a.pslot, a.scratch) == (9, 10, 11, 12)
-    assert (a.scratch_bytes, a.batch, a.rows, a.q_heads, a.slots, a.causal, a.scale) == (13, 14, 15, 16, 17, 18, 0.5)
-    k = Kv8.from_buffer_copy(serving._KV8.pack(*range(1, 13)))
-    assert [getattr(k, f[0]) for f in Kv8._fields_] == list(range(1, 13))
-    o = Logprobs.from_buffer_copy(serving._LOGPROBS.pack(*range(1, 10)))
-    assert [getattr(o, f[0]) for f in Logprobs._fields_] == list(range(1, 10))
+def test_null_structs_are_refused():
     for call in (lambda: L.mmz_kv8_write(None, A, A, 64, 64, 64, None, 1, 1, None), lambda: L.mmz_attn8(None, None, None),
                  lambda: L.mmz_kv8_read(None, A, A, 64, 64, 64, None, None, 1, 1, None),
                  lambda: L.mmz_token_logprobs(A, 9, 0, 1, 9, None, None, None),
@@ -196,3 +185,24 @@ def test_python_calls_refuse_what_is_no_cuda_tensor():
         m.linear_logprobs(x[0, 0], x[0, 0], s[0, 0], s[0, 0])
     with pytest.raises(AttributeError):
         m.no_such_call
+
+
+def test_python_calls_take_their_arguments_by_name():
+    import inspect
+    for f, first, last in ((m.kv8_write, "k", "stream"), (m.kv8_read, "k8", "stream"), (m.attn8, "q", "stream"),
+                           (m.token_logprobs, "logits", "stream"), (m.linear_logprobs, "x", "stream")):
+        names = list(inspect.signature(f).parameters)
+        assert (names[0], names[-1]) == (first, last) and f.__doc__
+        with pytest.raises(TypeError, match="missing required argument"):
+            f()
+        with pytest.raises(TypeError, match="unexpected keyword argument 'colour'"):
+            f(*[None] * 3, colour=1)
+        with pytest.raises(TypeError, match="multiple values for argument"):
+            f(None, **{first: None})
+        with pytest.raises(TypeError, match="at most"):
+            f(*[None] * (len(names) + 1))
+        required = [n for n, p in inspect.signature(f).parameters.items() if p.default is p.empty]
+        with pytest.raises(m.MmzError):
+            f(**{"".join(n): None for n in names})  # every name is one, interned or not
+        with pytest.raises(TypeError, match="missing required argument '%s'" % required[-1]):
+            f(*[None] * (len(required) - 1))
