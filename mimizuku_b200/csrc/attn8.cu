@@ -121,6 +121,7 @@ struct Rows {
     float m[NTL][2], l[NTL][2], o[4][NTL][4];  // o[i][n][e + 2 k]: dimension 8 g + 2 i + k, column 8 n + 2 t + e
     float* raw[NTL][2];                        // where the scores of the lane's columns go, null: nowhere
     bool any;                                  // some lane of the warp has a raw
+    int badpos;                                // the first position whose value scale is not finite (odd_scales)
 
     // the row of column c of tile n
     static __device__ __forceinline__ int row(int n, int c) { return MODE == 0 ? c & 3 : 8 * n + c; }
@@ -152,6 +153,7 @@ struct Rows {
         any = to && __any_sync(0xffffffff, have_one);
     }
     __device__ __forceinline__ void clear() {
+        badpos = 0x7fffffff;
 #pragma unroll
         for (int n = 0; n < NTL; n++) {
             m[n][0] = m[n][1] = -INFINITY;
@@ -197,6 +199,16 @@ struct Rows {
                         for (int e = 0; e < 4; e++) o[i][n][e] += vsc * acc[n][e];
                 }
             }
+        }
+    }
+    // A value scale (chunk_scale's lanes 4-7) that is not finite, in a chunk that some rows see only a part of: left out of
+    // the sums (a weight of 0 times it would not be 0), and the rows that do see its positions are NaN in the end
+    __device__ __forceinline__ void odd_scales(float& sc, int base, int lane) {
+        const bool odd = lane >= 4 && !(fabsf(sc) <= 3.402823466e38f);
+        const unsigned tiles = __ballot_sync(0xffffffff, odd) >> 4;
+        if (tiles) {
+            badpos = min(badpos, base + 16 * (__ffs(tiles) - 1));
+            if (odd) sc = 0.f;
         }
     }
     // One chunk: codes at ck, cv (shared memory), positions base .. base + 63 of which those below `most` exist. sc:
@@ -340,11 +352,14 @@ struct Rows {
         }
     }
     // after the last chunk: the lanes' sums of p added up, and the two parts of MODE 0. Columns with have(t) are valid
-    __device__ __forceinline__ void finish() {
+    __device__ __forceinline__ void finish(const int (&lim)[NTL][2]) {
 #pragma unroll
         for (int n = 0; n < NTL; n++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
+                if (badpos < lim[n][e])
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[i][n][e] = o[i][n][e + 2] = NAN;
                 l[n][e] += __shfl_xor_sync(0xffffffff, l[n][e], 4);
                 l[n][e] += __shfl_xor_sync(0xffffffff, l[n][e], 8);
                 l[n][e] += __shfl_xor_sync(0xffffffff, l[n][e], 16);
@@ -470,7 +485,8 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
         const int st = it % STG;
         ok = __all_sync(0xffffffff, mbar_wait(&full[st], (it / STG) & 1, &sm.abort, limit_ns, status, K_ATTN8, 1));
         if (!ok) break;
-        const float sc = sc_next;
+        float sc = sc_next;
+        if (least < most && c * CH + CH > least) w.odd_scales(sc, c * CH, lane);
         sc_next = scale_of(c + wstep);
         w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], c * CH, most, c * CH + CH <= least, sc, a.scale, lim,
                 a.block, lane);
@@ -482,7 +498,7 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
         for (int i = 0; i < STG; i++, it++)
             if (at + i * wstep < c1) mbar_wait(&full[it % STG], (it / STG) & 1, nullptr, limit_ns, nullptr, 0, 0);
     }
-    w.finish();
+    w.finish(lim);
 
     const int nsrc = cs * wstep;
     if (nsrc == 1 && lay.nclus == 1) {  // every warp has its rows' whole results
@@ -704,6 +720,7 @@ __global__ void __launch_bounds__(NT, 4) attn8_flat_kernel(Attn8 a, float* rec, 
         ok = __all_sync(0xffffffff, mbar_wait(&full[st], (it / STG) & 1, &sm.abort, limit_ns, status, K_ATTN8, 2));
         if (!ok) break;
         const int base = cur.c * CH, least = a.causal ? max(0, cur.len - a.rows + 1) : cur.len;
+        if (least < cur.len && base + CH > least) w.odd_scales(sc[0], base, lane);
         w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], base, cur.len, base + CH <= least, sc[0], a.scale, lim,
                 a.block, lane);
         if (base + CH > cur.len) fence_proxy_async_smem();  // zeros written behind the end, before the next copy
@@ -713,7 +730,7 @@ __global__ void __launch_bounds__(NT, 4) attn8_flat_kernel(Attn8 a, float* rec, 
         if (sent < n) sc[STG - 1] = issue(st);
         const bool last = cur.c + 1 == cur.nch;
         if (last || it + 1 == n) {
-            w.finish();
+            w.finish(lim);
             if (last && from == 0) {
                 w.store(a, cur.b, cur.hk, group, 0, R, stats, lane);
             } else {

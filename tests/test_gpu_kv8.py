@@ -282,6 +282,35 @@ def test_nan_behind_the_sequence_is_not_used(cuda, rows):
     check(probs[:, 0], p[:, 1], ptol[:, 1] * p[:, 1])
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("rows,block,bad", [(4, 16, "nan"), (6, 16, "inf"), (40, 16, "nan"), (40, 32, "inf"), (130, 64, "nan")])
+def test_scales_that_are_not_finite_reach_only_the_rows_that_see_them(cuda, kind, rows, block, bad):
+    """Causal rows over one sequence; the scales of the block that ends the sequence are NaN or infinite. The rows before
+    it come out bit for bit as with a finite scale there, those that see it are NaN."""
+    gen = torch.Generator().manual_seed(rows)
+    L = 3 * block + 1 if rows < block else rows + 1  # the last block starts inside the rows
+    cap = -(-L // block) * block
+    last = (L - 1) // block
+    k8, v8, ks, vs = cache(1, 2, cap, block, kind)
+    for c8, s in ((k8, ks), (v8, vs)):
+        c8.copy_((torch.randn(c8.shape, generator=gen) * 30).clamp(-120, 120).round().cuda().to(c8.dtype))
+        s.copy_((0.001 + torch.rand(s.shape, generator=gen) * 0.02).cuda())
+    q = torch.randn((1, rows, 2, HD), generator=gen).half().cuda()
+    lens = torch.tensor([L], dtype=torch.int32, device="cuda")
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    m.attn8(q, k8, v8, ks, vs, want, block=block, lens=lens, causal=True)
+    sees = L - rows + 1 + torch.arange(rows, device="cuda") > last * block
+    assert sees.any() and not sees.all()
+    for s in (vs, ks):
+        keep = s[:, :, last].clone()
+        s[:, :, last] = float(bad)
+        m.attn8(q, k8, v8, ks, vs, out, block=block, lens=lens, causal=True)
+        s[:, :, last] = keep
+        assert torch.equal(out[0, ~sees], want[0, ~sees])
+        if s is vs or bad == "nan":
+            assert out[0, sees].isnan().all()
+
+
 def test_large_and_small_scores(cuda):
     """Scores far apart: one position holds all the weight, then none does (equal scores)."""
     b, h, cap, block = 1, 1, 300, 64
