@@ -943,7 +943,7 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     p.mode = R <= 4 ? 0 : R <= 8 ? 1 : 2;
     p.stats = slots > 0 ? ((size_t)pairs * R * 8 + 15) & ~(size_t)15 : 0;
     p.raws = (size_t)batch * slots * rows * cap * 4;
-    // The warps of a CTA take rows of their own where that alone fills the GPU (prompts of 223 rows on 160 pairs: 36 us,
+    // The warps of a CTA take rows of their own where that alone fills the GPU (prompts of 223 rows on 160 pairs: 37 us,
     // positions split instead 70; 64 rows on 160 pairs do not: 73 against 59).
     const long wide = WARPS * rt;
     p.lay.wrows = R > 16 && pairs * ((R + wide - 1) / wide) >= SLOTS;
