@@ -16,10 +16,11 @@
 //     largest p, so the one rounding that counts stays that of the output. Up to 4 rows the two parts are columns
 //     r and r + 4 of one product (the lanes of columns 4-7 hold the same scores and keep the low part).
 //   * the scales of a block apply in fp32: ks to the scores, vs to the sums of the positions that share it.
-// Two ways through the cache (plan() chooses):
-//   cluster  a CTA to a (pair, row block), its warps along the positions or along the rows; CTAs of a cluster split the
-//            sequence and join through distributed shared memory, and where one cluster is too little (and more than 8
-//            rows), clusters through scratch and a second kernel
+// Three ways through the cache (plan() chooses):
+//   cluster  a CTA to a (pair, row block), its warps along the positions; CTAs of a cluster split the sequence and join
+//            through distributed shared memory, and where one cluster is too little (and more than 8 rows), clusters
+//            through scratch and a second kernel
+//   rows     more than 16 rows, enough of them to fill the GPU (prompts): a CTA of one warp to 16 rows, which takes all they see
 //   flat     up to 8 rows and too few pairs for a cluster each to fill the GPU (long caches): a fixed number of warps,
 //            each with an equal share of all sequences' and heads' chunks in a row, whatever the lengths; a pair's parts on
 //            several warps join in a second kernel
@@ -403,7 +404,6 @@ __device__ __forceinline__ float chunk_scale(const float* ks, const float* vs, i
 // How a cluster call is laid out along its CTAs (plan() below).
 struct Lay {
     int cs, nclus;  // CTAs of a cluster, clusters along the sequence
-    int wrows;      // 0: the warps of a CTA share its rows and split the positions; 1: each has rows of its own
     int block;      // rows of a CTA that exist at most (what its shared memory holds)
     int tiles;      // CTAs along the rows
 };
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
     extern __shared__ __align__(128) uint8_t smem[];
     Smem& sm = *reinterpret_cast<Smem*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int cs = lay.cs, wstep = lay.wrows ? 1 : WARPS;
+    const int cs = lay.cs;
     unsigned x = blockIdx.x;
     const int rank = x % cs;
     x /= cs;
@@ -432,8 +432,7 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
     const int hk = (int)(pair % a.kv_heads), group = a.q_heads / a.kv_heads;
     const long b = pair / a.kv_heads;
     const int R = a.rows * group;
-    const int b0 = tile * (lay.wrows ? WARPS * RT : RT);        // first row of the CTA
-    const int r0 = b0 + (lay.wrows ? warp * RT : 0);            // first row of the warp
+    const int r0 = tile * RT;  // first row
     if (lane == 0)
         for (int i = 0; i < STG; i++) mbar_init(&sm.full[warp][i], 1);
     if (threadIdx.x == 0) sm.abort = 0;
@@ -454,7 +453,7 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
     const int nch = (most + CH - 1) / CH;
     const int ns = cs * lay.nclus, per = (nch + ns - 1) / ns, split = clus * cs + rank;
     const int c0 = min(split * per, nch), c1 = min(c0 + per, nch);
-    const int cw = c0 + (lay.wrows ? 0 : warp);  // the warp's first chunk; then every wstep-th
+    const int cw = c0 + warp;  // the warp's first chunk; then every WARPS-th
     const uint8_t* k8 = a.k8 + b * a.c_seq + hk * a.c_head;
     const uint8_t* v8 = a.v8 + b * a.c_seq + hk * a.c_head;
     const float* ks = a.ks + b * a.s_seq + hk * a.s_head;
@@ -471,7 +470,7 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
     auto scale_of = [&](int c) { return c < c1 ? chunk_scale(ks, vs, c, most, shift, lane) : 0.f; };
     int at = cw;
     if (lane == 0)
-        for (int i = 0; i < STG && cw + i * wstep < c1; i++) issue(cw + i * wstep, i);
+        for (int i = 0; i < STG && cw + i * WARPS < c1; i++) issue(cw + i * WARPS, i);
     float sc_next = scale_of(cw);
     int lim[NTL][2];
 #pragma unroll
@@ -481,34 +480,29 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
 
     bool ok = true;
     int it = 0;
-    for (int c = cw; c < c1; c += wstep, it++) {
+    for (int c = cw; c < c1; c += WARPS, it++) {
         const int st = it % STG;
         ok = __all_sync(0xffffffff, mbar_wait(&full[st], (it / STG) & 1, &sm.abort, limit_ns, status, K_ATTN8, 1));
         if (!ok) break;
         float sc = sc_next;
         if (least < most && c * CH + CH > least) w.odd_scales(sc, c * CH, lane);
-        sc_next = scale_of(c + wstep);
+        sc_next = scale_of(c + WARPS);
         w.chunk(sm.ring[warp][st][0], sm.ring[warp][st][1], c * CH, most, c * CH + CH <= least, sc, a.scale, lim,
                 a.block, lane);
         __syncwarp();
-        if (lane == 0 && c + STG * wstep < c1) issue(c + STG * wstep, st);
-        at = c + wstep;
+        if (lane == 0 && c + STG * WARPS < c1) issue(c + STG * WARPS, st);
+        at = c + WARPS;
     }
     if (!ok && lane == 0) {  // a wait gave up: let the copies in flight land before the CTA ends
         for (int i = 0; i < STG; i++, it++)
-            if (at + i * wstep < c1) mbar_wait(&full[it % STG], (it / STG) & 1, nullptr, limit_ns, nullptr, 0, 0);
+            if (at + i * WARPS < c1) mbar_wait(&full[it % STG], (it / STG) & 1, nullptr, limit_ns, nullptr, 0, 0);
     }
     w.finish(lim);
 
-    const int nsrc = cs * wstep;
-    if (nsrc == 1 && lay.nclus == 1) {  // every warp has its rows' whole results
-        w.store(a, b, hk, group, r0, R, stats, lane);
-        return;
-    }
     // ---------------------------------------------------------------- the parts of a row joined
     // Each warp sends its rows' statistics to every CTA of the cluster and its sums to the CTA that joins those
     // dimensions (the lane's 8 have one owner): stores, and one barrier, instead of loads that are waited for.
-    const int src = rank * wstep + (lay.wrows ? 0 : warp), share = HD / cs;
+    const int nsrc = cs * WARPS, src = rank * WARPS + warp, share = HD / cs;
     float2* ms = reinterpret_cast<float2*>(smem + sizeof(Smem));
     float* sums = reinterpret_cast<float*>(ms + lay.block * nsrc + (lay.block * nsrc & 1));
     if (cs > 1) cluster_wait();
@@ -516,7 +510,7 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
     for (int n = 0; n < NTL; n++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const int r = r0 - b0 + 8 * n + 2 * t + e;  // row of the block
+            const int r = 8 * n + 2 * t + e;  // row of the block
             if (!w.have(t) || r >= lay.block) continue;
             if (g < cs) st_dsmem_f32x2(dsmem_addr(&ms[r * nsrc + src], g), make_float2(w.m[n][e], w.l[n][e]));
             const uint32_t to = dsmem_addr(&sums[(r * nsrc + src) * share + 8 * g % share], 8 * g / share);
@@ -527,7 +521,7 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
     else __syncthreads();
     for (int i = threadIdx.x; i < lay.block * (share / 2); i += NT) {
         const int r = i / (share / 2), dl = 2 * (i % (share / 2)), d = rank * share + dl;
-        if (b0 + r >= R) break;
+        if (r0 + r >= R) break;
         float M = -INFINITY, S = 0.f;
         float2 O = make_float2(0.f, 0.f);
 #pragma unroll 4
@@ -540,19 +534,94 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
             O.x += f * x.x;
             O.y += f * x.y;
         }
-        const long row = (long)pair * R + b0 + r;
+        const long row = (long)pair * R + r0 + r;
         if (lay.nclus > 1) {
             float* rec = part + (row * lay.nclus + clus) * REC;
             *reinterpret_cast<float2*>(rec + d) = O;
             if (d == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(M, S);
         } else {
             const float inv = inverse(S);
-            const int qi = (b0 + r) / group, h = hk * group + (b0 + r) % group;
+            const int qi = (r0 + r) / group, h = hk * group + (r0 + r) % group;
             *reinterpret_cast<__half2*>(a.out + b * a.o_seq + qi * a.o_row + h * a.o_head + d) =
                 __floats2half2_rn(O.x * inv, O.y * inv);
             if (stats && d == 0) stats[row] = make_float2(M, inv);
         }
     }
+}
+
+// ---------------------------------------------------------------- rows of a warp's own
+namespace a8 {
+// A CTA of one warp: the last ones of a grid fill the GPU evenly, whatever the lengths (223 causal rows on 160 pairs of 150 to
+// 448 positions: 30 us, with four such warps to a CTA 37)
+struct RowsSmem {
+    uint8_t ring[STG][2][KB];
+    uint64_t full[STG];
+};
+}  // namespace a8
+
+// grid: (sequence, key head) fastest, then tile of 16 rows, the last tile first (with causal it has the most to do).
+// Static shared memory above 16 KB of ring: 12 CTAs to an SM
+template <int KIND>
+__global__ void __launch_bounds__(32, 12) attn8_rows_kernel(Attn8 a, int tiles, float2* stats, float* raws, unsigned* status,
+                                                            unsigned long long limit_ns) {
+    constexpr int NTL = Rows<KIND, 2>::NTL, RT = 8 * NTL;
+    __shared__ __align__(128) RowsSmem sm;
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    const unsigned pairs = (unsigned)a.batch * a.kv_heads, pair = blockIdx.x % pairs;
+    const int hk = (int)(pair % a.kv_heads), group = a.q_heads / a.kv_heads;
+    const long b = pair / a.kv_heads;
+    const int R = a.rows * group, r0 = (tiles - 1 - (int)(blockIdx.x / pairs)) * RT;
+    if (lane == 0)
+        for (int i = 0; i < STG; i++) mbar_init(&sm.full[i], 1);
+    fence_mbar_init();
+    __syncwarp();
+    griddep_wait();
+    griddep_launch_dependents();
+
+    Rows<KIND, 2> w;
+    w.queries(a, b, hk, group, r0, R, lane);
+    w.record(a, raws, b, hk, group, r0, R, lane);
+    w.clear();
+    const int L = seq_len(a, b);
+    auto limit = [&](int r) { return a.causal ? max(0, L - a.rows + r / group + 1) : L; };
+    const int most = limit(min(r0 + RT, R) - 1), least = limit(r0), nch = (most + CH - 1) / CH;
+    const uint8_t* k8 = a.k8 + b * a.c_seq + hk * a.c_head;
+    const uint8_t* v8 = a.v8 + b * a.c_seq + hk * a.c_head;
+    const float* ks = a.ks + b * a.s_seq + hk * a.s_head;
+    const float* vs = a.vs + b * a.s_seq + hk * a.s_head;
+    const int shift = 31 - __clz(a.block);
+    auto issue = [&](int c) {  // lane 0
+        const uint32_t bytes = (uint32_t)min(CH, most - c * CH) * HD;
+        uint64_t* full = &sm.full[c % STG];
+        mbar_expect_tx(full, 2 * bytes);
+        bulk_g2s(sm.ring[c % STG][0], k8 + (long)c * KB, bytes, full);
+        bulk_g2s(sm.ring[c % STG][1], v8 + (long)c * KB, bytes, full);
+    };
+    auto scale_of = [&](int c) { return c < nch ? chunk_scale(ks, vs, c, most, shift, lane) : 0.f; };
+    if (lane == 0)
+        for (int c = 0; c < STG && c < nch; c++) issue(c);
+    float sc_next = scale_of(0);
+    int lim[NTL][2];
+#pragma unroll
+    for (int n = 0; n < NTL; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) lim[n][e] = limit(min(r0 + w.row(n, 2 * t + e), R - 1));
+
+    int c = 0;
+    for (; c < nch; c++) {
+        const int st = c % STG;
+        if (!__all_sync(0xffffffff, mbar_wait(&sm.full[st], (c / STG) & 1, nullptr, limit_ns, status, K_ATTN8, 3))) break;
+        float sc = sc_next;
+        if (least < most && c * CH + CH > least) w.odd_scales(sc, c * CH, lane);
+        sc_next = scale_of(c + 1);
+        w.chunk(sm.ring[st][0], sm.ring[st][1], c * CH, most, c * CH + CH <= least, sc, a.scale, lim, a.block, lane);
+        __syncwarp();
+        if (lane == 0 && c + STG < nch) issue(c + STG);
+    }
+    if (lane == 0)  // after a wait that gave up: let the copies in flight land before the CTA ends
+        for (int i = c; i < min(c + STG, nch); i++) mbar_wait(&sm.full[i % STG], (i / STG) & 1, nullptr, limit_ns, nullptr, 0, 0);
+    w.finish(lim);
+    w.store(a, b, hk, group, r0, R, stats, lane);
 }
 
 // ---------------------------------------------------------------- flat
@@ -927,7 +996,7 @@ namespace {
 constexpr long SLOTS = 148 * 3;  // CTAs that a B200 holds at once (shared memory: 3 to an SM)
 struct Plan {
     int mode;   // Rows' MODE
-    bool flat;
+    bool rows, flat;
     Lay lay;
     size_t smem, part, stats, raws;
 };
@@ -943,16 +1012,19 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     p.mode = R <= 4 ? 0 : R <= 8 ? 1 : 2;
     p.stats = slots > 0 ? ((size_t)pairs * R * 8 + 15) & ~(size_t)15 : 0;
     p.raws = (size_t)batch * slots * rows * cap * 4;
-    // The warps of a CTA take rows of their own where that alone fills the GPU (prompts of 223 rows on 160 pairs: 37 us,
-    // positions split instead 70; 64 rows on 160 pairs do not: 73 against 59).
-    const long wide = WARPS * rt;
-    p.lay.wrows = R > 16 && pairs * ((R + wide - 1) / wide) >= SLOTS;
-    const long block = p.lay.wrows ? wide : rt;
-    p.lay.block = (int)(R < block ? R : block);
-    p.lay.tiles = (int)((R + block - 1) / block);
+    // Warps take rows of their own where that gives every SM half of the 12 warps it can hold. On 160 pairs of prompts of 223
+    // rows 30 us, positions split instead 70; of 128 rows 82 against 98 us; 64 rows would give an SM 4 warps: 61 against 59
+    p.rows = R > 16 && pairs * ((R + rt - 1) / rt) >= 2 * SLOTS;
+    p.lay.block = (int)(R < rt ? R : rt);
+    p.lay.tiles = (int)((R + rt - 1) / rt);
+    if (p.rows) {
+        p.flat = false, p.smem = 0, p.part = 0;
+        p.lay.cs = p.lay.nclus = 1;
+        return p;
+    }
     // splits of the sequence: no more CTAs than the GPU holds at once (5 rows on 120 pairs: 2 CTAs a pair 16 us, 4 in more
     // than one wave 23), and a chunk at least to each warp
-    const long units = pairs * p.lay.tiles, top = p.lay.wrows ? chunks : (chunks + WARPS - 1) / WARPS;
+    const long units = pairs * p.lay.tiles, top = (chunks + WARPS - 1) / WARPS;
     long s = SLOTS / units;
     s = s < 1 ? 1 : s > top ? top : s;
     const int cs = s < 2 ? 1 : s < 4 ? 2 : s < 8 ? 4 : 8;
@@ -963,14 +1035,13 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     // positions 29 us flat, 28 in clusters, 320 pairs 18.7 and 17.6, 20 pairs 7.5 and 5.5.
     p.flat = R <= 8 && p.lay.nclus > 1 && pairs * chunks < 0x7fffffffl;
     if (p.flat) {
-        p.lay = {1, 1, 0, 0, 1};
+        p.lay = {1, 1, 0, 1};
         p.smem = sizeof(Smem);
         p.part = (size_t)SLOTS * WARPS * 2 * RECF * 4;
         return p;
     }
-    const size_t n = (size_t)p.lay.block * cs * (p.lay.wrows ? 1 : WARPS);  // (row, source) pairs
-    const bool alone = p.lay.wrows && s == 1;  // a warp has its rows' whole results, nothing is exchanged
-    p.smem = sizeof(Smem) + (alone ? 0 : (n + (n & 1)) * 8 + n * (HD / cs) * 4);
+    const size_t n = (size_t)p.lay.block * cs * WARPS;  // (row, source) pairs
+    p.smem = sizeof(Smem) + (n + (n & 1)) * 8 + n * (HD / cs) * 4;
     p.part = p.lay.nclus > 1 ? ((size_t)pairs * R * p.lay.nclus * REC * 4 + 15) & ~(size_t)15 : 0;
     return p;
 }
@@ -982,6 +1053,10 @@ int launch_main(const Attn8& a, const Plan& p, float* part, float2* stats, float
             return check_pdl(launch_pdl(attn8_flat_kernel<KIND, MODE>, dim3(SLOTS), dim3(NT), p.smem, st, a, part, stats, raws,
                                         dc.status, dc.limit_ns),
                              "attn8");
+    } else if (p.rows) {
+        return check_pdl(launch_pdl(attn8_rows_kernel<KIND>, dim3((unsigned)((long)a.batch * a.kv_heads * p.lay.tiles)),
+                                    dim3(32), 0, st, a, p.lay.tiles, stats, raws, dc.status, dc.limit_ns),
+                         "attn8");
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long)a.batch * a.kv_heads * p.lay.tiles * p.lay.nclus * p.lay.cs));
@@ -1074,6 +1149,8 @@ void init_attn8_attrs() {
         carve(fn);
     };
     carve(attn8_post_kernel);
+    carve(attn8_rows_kernel<KV8_INT8>);
+    carve(attn8_rows_kernel<KV8_E4M3>);
     set(attn8_kernel<KV8_INT8, 0>);
     set(attn8_kernel<KV8_INT8, 1>);
     set(attn8_kernel<KV8_INT8, 2>);

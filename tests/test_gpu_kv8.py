@@ -223,7 +223,10 @@ ATTENDS = [  # b, rows, kv heads, group, cap, lens (None: cap), causal
     (32, 1, 20, 1, 448, [14 * i for i in range(32)], False), (2, 1, 4, 2, 30000, [30000, 17], False),
     (40, 3, 16, 1, 400, [(37 * i) % 401 for i in range(40)], True), (4, 2, 8, 4, 8000, [8000, 1, 0, 7999], True),
     (64, 1, 16, 1, 300, [i % 3 * 32 for i in range(64)], False), (60, 1, 20, 1, 200, [0] * 60, False),
-    (100, 1, 12, 1, 257, [200 + i % 58 for i in range(100)], False), (1, 8, 1, 1, 230000, None, True)]
+    (100, 1, 12, 1, 257, [200 + i % 58 for i in range(100)], False), (1, 8, 1, 1, 230000, None, True),
+    # prompts that fill the GPU: each warp takes rows of its own
+    (38, 37, 8, 1, 150, [4 * i - 1 for i in range(38)], True), (40, 11, 8, 3, 90, [(29 * i) % 91 for i in range(40)], True),
+    (45, 17, 10, 1, 65, [63 + i % 3 for i in range(45)], False), (30, 33, 10, 1, 128, None, True)]
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
@@ -259,10 +262,10 @@ def test_attention(cuda, kind, block, case):
     assert m.status()[0] == 0
 
 
-@pytest.mark.parametrize("rows", [1, 20])
-def test_nan_behind_the_sequence_is_not_used(cuda, rows):
+@pytest.mark.parametrize("rows,h", [(1, 2), (20, 2), (20, 230)])
+def test_nan_behind_the_sequence_is_not_used(cuda, rows, h):
     gen = torch.Generator().manual_seed(1)
-    b, h, cap, block = 2, 2, 150, 32
+    b, cap, block = 2, 150, 32
     c = filled(gen, b, h, cap, block, "e4m3")
     lens = [70, 0]
     for x in c[:2]:
@@ -275,7 +278,7 @@ def test_nan_behind_the_sequence_is_not_used(cuda, rows):
     out = torch.empty((b, rows, h, HD), dtype=torch.float16, device="cuda")
     probs = torch.empty((b, 1, rows, cap), dtype=torch.float16, device="cuda")
     m.attn8(q.cuda(), *c, out, block=block, lens=torch.tensor(lens, dtype=torch.int32, device="cuda"), probs=probs,
-            pslot=torch.tensor([-1, 0], dtype=torch.int32, device="cuda"))
+            pslot=torch.tensor([-1, 0] + [-1] * (h - 2), dtype=torch.int32, device="cuda"))
     k, v = (np.nan_to_num(values(x, s, block)) for x, s in ((c[0], c[2]), (c[1], c[3])))
     want, tol, p, ptol = attend_ref(q.double().numpy(), k, v, lens, False)
     check(out, want, tol)
@@ -283,19 +286,21 @@ def test_nan_behind_the_sequence_is_not_used(cuda, rows):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("rows,block,bad", [(4, 16, "nan"), (6, 16, "inf"), (40, 16, "nan"), (40, 32, "inf"), (130, 64, "nan")])
-def test_scales_that_are_not_finite_reach_only_the_rows_that_see_them(cuda, kind, rows, block, bad):
+@pytest.mark.parametrize("rows,block,heads,bad", [
+    (4, 16, 2, "nan"), (6, 16, 2, "inf"), (40, 16, 2, "nan"), (40, 32, 2, "inf"), (130, 64, 2, "nan"), (40, 16, 300, "nan"),
+    (130, 64, 100, "inf")])
+def test_scales_that_are_not_finite_reach_only_the_rows_that_see_them(cuda, kind, rows, block, heads, bad):
     """Causal rows over one sequence; the scales of the block that ends the sequence are NaN or infinite. The rows before
     it come out bit for bit as with a finite scale there, those that see it are NaN."""
     gen = torch.Generator().manual_seed(rows)
     L = 3 * block + 1 if rows < block else rows + 1  # the last block starts inside the rows
     cap = -(-L // block) * block
     last = (L - 1) // block
-    k8, v8, ks, vs = cache(1, 2, cap, block, kind)
+    k8, v8, ks, vs = cache(1, heads, cap, block, kind)
     for c8, s in ((k8, ks), (v8, vs)):
         c8.copy_((torch.randn(c8.shape, generator=gen) * 30).clamp(-120, 120).round().cuda().to(c8.dtype))
         s.copy_((0.001 + torch.rand(s.shape, generator=gen) * 0.02).cuda())
-    q = torch.randn((1, rows, 2, HD), generator=gen).half().cuda()
+    q = torch.randn((1, rows, heads, HD), generator=gen).half().cuda()
     lens = torch.tensor([L], dtype=torch.int32, device="cuda")
     out, want = torch.empty_like(q), torch.empty_like(q)
     m.attn8(q, k8, v8, ks, vs, want, block=block, lens=lens, causal=True)
