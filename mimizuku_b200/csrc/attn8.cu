@@ -406,6 +406,7 @@ struct Lay {
     int cs, nclus;  // CTAs of a cluster, clusters along the sequence
     int block;      // rows of a CTA that exist at most (what its shared memory holds)
     int tiles;      // CTAs along the rows
+    int inside;     // the parts are exchanged where the ring was
 };
 
 }  // namespace a8
@@ -503,7 +504,8 @@ __global__ void __launch_bounds__(NT, 3) attn8_kernel(Attn8 a, Lay lay, float* p
     // Each warp sends its rows' statistics to every CTA of the cluster and its sums to the CTA that joins those
     // dimensions (the lane's 8 have one owner): stores, and one barrier, instead of loads that are waited for.
     const int nsrc = cs * WARPS, src = rank * WARPS + warp, share = HD / cs;
-    float2* ms = reinterpret_cast<float2*>(smem + sizeof(Smem));
+    if (MODE == 2 && lay.inside) __syncthreads();
+    float2* ms = reinterpret_cast<float2*>(smem + (MODE == 2 && lay.inside ? 0 : sizeof(Smem)));
     float* sums = reinterpret_cast<float*>(ms + lay.block * nsrc + (lay.block * nsrc & 1));
     if (cs > 1) cluster_wait();
 #pragma unroll
@@ -993,7 +995,9 @@ __global__ void __launch_bounds__(512) attn8_post_kernel(Attn8 a, unsigned jbloc
 
 // The layout of a call, from its sizes alone (lens is on the device), and its scratch.
 namespace {
-constexpr long SLOTS = 148 * 3;  // CTAs that a B200 holds at once (shared memory: 3 to an SM)
+constexpr long SLOTS = 148 * 3;   // CTAs that a B200 holds at once (shared memory: 3 to an SM)
+constexpr long PAIRED = 148 * 2;  // the same at two to an SM
+constexpr size_t ALONE3 = 78 << 10;  // shared memory of which an SM has two, not three
 struct Plan {
     int mode;   // Rows' MODE
     bool rows, flat;
@@ -1012,9 +1016,10 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     p.mode = R <= 4 ? 0 : R <= 8 ? 1 : 2;
     p.stats = slots > 0 ? ((size_t)pairs * R * 8 + 15) & ~(size_t)15 : 0;
     p.raws = (size_t)batch * slots * rows * cap * 4;
-    // Warps take rows of their own where that gives every SM half of the 12 warps it can hold. On 160 pairs of prompts of 223
-    // rows 30 us, positions split instead 70; of 128 rows 82 against 98 us; 64 rows would give an SM 4 warps: 61 against 59
-    p.rows = R > 16 && pairs * ((R + rt - 1) / rt) >= 2 * SLOTS;
+    // Warps take rows of their own where their tiles fill the GPU well enough: with few, four warps to a tile finish sooner,
+    // and the longer the cache the less their join weighs. 7 chunks: 640 tiles 20.0 us, positions split 22.7; 320 tiles 16.9
+    // and 13.5. 24 chunks: 640 tiles 61 and 46, 1280 tiles 82 and 76. 223 causal rows on 160 pairs of 150 to 448: 30 and 61
+    p.rows = R > 16 && pairs * ((R + rt - 1) / rt) >= 64 * (chunks < 28 ? chunks : 28);
     p.lay.block = (int)(R < rt ? R : rt);
     p.lay.tiles = (int)((R + rt - 1) / rt);
     if (p.rows) {
@@ -1022,10 +1027,10 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
         p.lay.cs = p.lay.nclus = 1;
         return p;
     }
-    // splits of the sequence: no more CTAs than the GPU holds at once (5 rows on 120 pairs: 2 CTAs a pair 16 us, 4 in more
+    // Splits of the sequence: no more CTAs than the GPU holds at once (5 rows on 120 pairs: 2 CTAs a pair 16 us, 4 in more
     // than one wave 23), and a chunk at least to each warp
     const long units = pairs * p.lay.tiles, top = (chunks + WARPS - 1) / WARPS;
-    long s = SLOTS / units;
+    long s = (p.mode == 2 ? PAIRED : SLOTS) / units;  // (16 rows in a cluster: two CTAs to an SM)
     s = s < 1 ? 1 : s > top ? top : s;
     const int cs = s < 2 ? 1 : s < 4 ? 2 : s < 8 ? 4 : 8;
     p.lay.cs = cs;
@@ -1035,13 +1040,19 @@ Plan plan(int batch, int rows, int q_heads, int kv_heads, int cap, int slots) {
     // positions 29 us flat, 28 in clusters, 320 pairs 18.7 and 17.6, 20 pairs 7.5 and 5.5.
     p.flat = R <= 8 && p.lay.nclus > 1 && pairs * chunks < 0x7fffffffl;
     if (p.flat) {
-        p.lay = {1, 1, 0, 1};
+        p.lay = {1, 1, 0, 1, 0};
         p.smem = sizeof(Smem);
         p.part = (size_t)SLOTS * WARPS * 2 * RECF * 4;
         return p;
     }
     const size_t n = (size_t)p.lay.block * cs * WARPS;  // (row, source) pairs
-    p.smem = sizeof(Smem) + (n + (n & 1)) * 8 + n * (HD / cs) * 4;
+    // 16 rows' exchange beside the ring leaves room for two CTAs to an SM. More CTAs than that exchange inside the ring, behind
+    // a barrier more (320 tiles of 7 chunks 13.5 us, beside it 20)
+    p.lay.inside = p.mode == 2 && cs == 1 && units > PAIRED;
+    p.smem = sizeof(Smem) + (p.lay.inside ? 0 : (n + (n & 1)) * 8 + n * (HD / cs) * 4);
+    // Up to two CTAs to an SM: shared memory that no third one fits into, or the first SMs get three and others one (240 CTAs
+    // of 12 chunks 13.9 us, without 16.4)
+    if (units * cs * p.lay.nclus <= PAIRED) p.smem = p.smem > ALONE3 ? p.smem : ALONE3;
     p.part = p.lay.nclus > 1 ? ((size_t)pairs * R * p.lay.nclus * REC * 4 + 15) & ~(size_t)15 : 0;
     return p;
 }
@@ -1138,7 +1149,7 @@ int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, 
 }
 
 void init_attn8_attrs() {
-    const int most = (int)(sizeof(Smem) + WARPS * 16 * (8 * 8 + HD * 4));  // any layout's shared memory
+    const int most = (int)(sizeof(Smem) + WARPS * 16 * (8 * 8 + HD * 4));  // any layout's shared memory (above ALONE3)
     // every kernel asks for the largest shared memory of an SM: the split from the L1 cache changes only on an idle SM,
     // and a CTA of the main kernel that finds too little beside the last call's blocks starts when the others end
     auto carve = [&](auto* fn) {

@@ -224,6 +224,9 @@ ATTENDS = [  # b, rows, kv heads, group, cap, lens (None: cap), causal
     (40, 3, 16, 1, 400, [(37 * i) % 401 for i in range(40)], True), (4, 2, 8, 4, 8000, [8000, 1, 0, 7999], True),
     (64, 1, 16, 1, 300, [i % 3 * 32 for i in range(64)], False), (60, 1, 20, 1, 200, [0] * 60, False),
     (100, 1, 12, 1, 257, [200 + i % 58 for i in range(100)], False), (1, 8, 1, 1, 230000, None, True),
+    # tiles of 16 rows, more than two to an SM
+    (25, 20, 6, 1, 448, [18 * i + 16 for i in range(25)], True), (10, 11, 13, 3, 400, [40 * i for i in range(10)], True),
+    (40, 9, 8, 1, 300, [300 - i for i in range(40)], False),
     # prompts that fill the GPU: each warp takes rows of its own
     (38, 37, 8, 1, 150, [4 * i - 1 for i in range(38)], True), (40, 11, 8, 3, 90, [(29 * i) % 91 for i in range(40)], True),
     (45, 17, 10, 1, 65, [63 + i % 3 for i in range(45)], False), (30, 33, 10, 1, 128, None, True)]
