@@ -5,13 +5,15 @@
 // kv8_write, tokens x at positions pos .. pos + n: for each block touched
 //     a = max |x| over the block's new tokens,  s = a / Q  (Q = 127 for int8, 448 for e4m3)
 //     s = max(s, the block's earlier scale)  where the block has tokens before pos
-//     code = round_to_even(x * r),  r = 1 / s  (0 where s is 0: an all-zero block)
-// and, where s grew, the earlier tokens' codes become round_to_even(code * (s_old * r)): a scale only grows while its
-// block fills, so a code is rounded again at most as often as the block's maximum grows. All of it in fp32: quotients
-// and products each rounded once.
+//     code = round_to_even(x / s)  (0 where s is 0: an all-zero block)
+// and, where s grew, the earlier tokens' codes become round_to_even(code * s_old / s): a scale only grows while its
+// block fills, so a code is rounded again at most as often as the block's maximum grows. x / s is the quotient by the
+// unrounded scale, x Q / a, rounded to fp32 once: 1 / s is kept as r + rl, and x / s = x r + x rl with one rounding that
+// counts. (fp16 values often lie halfway between two codes exactly; a product by a rounded 1 / s misses so many of
+// them that 1 code in 21 thousand is the wrong one, a whole step off.)
 //
 // Bound by memory: 2 bytes read and 1 written per value (and the reverse to read). 32 x 20 heads x 1500 tokens, keys and
-// values: written in 68 us = 5.4 TB/s, read back in 55 us = 6.7 TB/s. A warp takes 32 tokens of one block (8 lanes to a token, 16
+// values: written in 71 us = 5.2 TB/s, read back in 55 us = 6.7 TB/s. A warp takes 32 tokens of one block (8 lanes to a token, 16
 // bytes each), so that its 8 loads are all in flight before the maximum is known and the values are read once; blocks
 // of 64 and 128 tokens are shared by 2 and 4 warps of the CTA, which exchange their maxima in shared memory.
 #include "fp8_cache.cuh"
@@ -102,8 +104,11 @@ __global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* k, const h16* 
         __syncwarp();
     }
     if (!any) return;
-    const float s = fmaxf(__fdiv_rn(amax, kv8_top<KIND>()), s_old);
-    const float r = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    const float s_new = __fdiv_rn(amax, kv8_top<KIND>());
+    const bool kept = s_old > s_new;  // the earlier scale stays
+    const float s = kept ? s_old : s_new, num = kept ? 1.f : kv8_top<KIND>(), den = kept ? s_old : amax;
+    const float r = s > 0.f ? __fdiv_rn(num, den) : 0.f, rl = r > 0.f ? __fdiv_rn(__fmaf_rn(-r, den, num), den) : 0.f;
+    auto over = [&](float x) { return __fmaf_rn(x, r, __fmul_rn(x, rl)); };
     if (lane == 0 && warp % W == 0) *scale = s;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -116,19 +121,16 @@ __global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* k, const h16* 
         for (int q = 0; q < 2; q++) {
             const float2 a = h2_to_f2(w[2 * q]), e = h2_to_f2(w[2 * q + 1]);
             if (!odd) {
-                // (products by the scalar intrinsic: the packed one fuses with the sum after it, which rounds once)
-                op[q] = kv8_store4_finite<KIND>(make_float2(__fmul_rn(a.x, r), __fmul_rn(a.y, r)),
-                                                make_float2(__fmul_rn(e.x, r), __fmul_rn(e.y, r)));
+                op[q] = kv8_store4_finite<KIND>(make_float2(over(a.x), over(a.y)), make_float2(over(e.x), over(e.y)));
                 continue;
             }
-            const float y[4] = {__fmul_rn(finite(a.x), r), __fmul_rn(finite(a.y), r), __fmul_rn(finite(e.x), r),
-                                __fmul_rn(finite(e.y), r)};
+            const float y[4] = {over(finite(a.x)), over(finite(a.y)), over(finite(e.x)), over(finite(e.y))};
             op[q] = kv8_store4<KIND>(y);
         }
         *reinterpret_cast<uint2*>(codes + j * HD + d0) = o;
     }
     if (older && s != s_old) {  // the scale grew: the block's earlier codes on the new one
-        const float f = __fmul_rn(s_old, r);
+        const float f = __fmul_rn(s_old, r), fl = __fmaf_rn(s_old, rl, __fmaf_rn(s_old, r, -f));
         for (long j = t0 + sub; j < min(t0 + tw, (long)p0); j += 4) {
             uint2* at = reinterpret_cast<uint2*>(codes + j * HD + d0);
             uint2 o = *at;
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(NT) kv8_write_kernel(const h16* k, const h16* 
                 float y[4];
                 kv8_load4<KIND>(op[q], y);
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = __fmul_rn(y[e], f);
+                for (int e = 0; e < 4; e++) y[e] = __fmaf_rn(y[e], f, __fmul_rn(y[e], fl));
                 op[q] = kv8_store4<KIND>(y);
             }
             *at = o;

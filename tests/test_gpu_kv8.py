@@ -54,10 +54,11 @@ def define_write(codes, scales, x, pos, block, kind):
                     s, old = a / top, scales[i, g, c]
                     if c * block < p:
                         s = max(s, old)
-                    r = np.float32(1) / s if s > 0 else np.float32(0)
+                    # the quotient by the unrounded scale, rounded to fp32
+                    r = 1 / np.float64(s) if s != a / top else np.float64(top) / np.float64(a) if a > 0 else 0.0
                     if c * block < p and s != old:
-                        codes[i, g, c * block:p] = snap(codes[i, g, c * block:p] * np.float32(old * r), kind)
-                    codes[i, g, j0:j1] = snap(part * r, kind)
+                        codes[i, g, c * block:p] = snap((codes[i, g, c * block:p] * np.float64(old) * r).astype(np.float32), kind)
+                    codes[i, g, j0:j1] = snap((part * r).astype(np.float32), kind)
                     scales[i, g, c] = s
     return codes, scales
 
