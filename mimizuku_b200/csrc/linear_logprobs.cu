@@ -563,10 +563,10 @@ __global__ void __launch_bounds__(1024) linear_join_kernel(const float* rec, int
         mine = pop();
         a = stat_warp(a);
     }
-    float lse = 0.f;
-    if (lane == 0) lse = store_row(o, at, a, has, tgt);
-    lse = __shfl_sync(0xffffffff, lse, 0);
-    if (lane < o.top) store_top(o, at, lane, mine, lse);
+    float ls = 0.f;
+    if (lane == 0) ls = store_row(o, at, a, has, tgt);
+    ls = __shfl_sync(0xffffffff, ls, 0);
+    if (lane < o.top) store_top(o, at, lane, mine, a.m, ls);
 }
 
 // the layout of a call, from its sizes

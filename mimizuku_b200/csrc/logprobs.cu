@@ -348,16 +348,16 @@ __global__ void __launch_bounds__(NT + 32, 2)
         if (cl > 1) cluster_sync();
         if (rank == 0 && warp == 0) {
             const RowStat a = stat_warp(lane < cl ? sm.stat[lane] : stat_none());
-            float lse = 0.f;
-            if (lane == 0) lse = store_row(o, at, a, has, tgt);
-            lse = __shfl_sync(0xffffffff, lse, 0);
+            float ls = 0.f;
+            if (lane == 0) ls = store_row(o, at, a, has, tgt);
+            ls = __shfl_sync(0xffffffff, ls, 0);
             const int n = cl * o.top;
             for (int i = lane; i < n; i += 32) {
                 const unsigned long long key = sm.all[i];
                 int above = 0;
 #pragma unroll 8
                 for (int k = 0; k < n; k++) above += sm.all[k] > key || (sm.all[k] == key && k < i);  // only empty ones are equal
-                if (above < o.top) store_top(o, at, above, key, lse);
+                if (above < o.top) store_top(o, at, above, key, a.m, ls);
             }
             __syncwarp();
         }

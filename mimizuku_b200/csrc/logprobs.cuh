@@ -90,14 +90,15 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
-// the row's outputs except its alternatives; tgt: the target's logit (read only where the target is in [0, V))
+// The row's outputs except its alternatives; tgt: the target's logit (read only where the target is in [0, V)). Returns
+// log s: a log probability is (x - m) - log s, which loses less than x - lse where it is close to 0
 __device__ __forceinline__ float store_row(const LogpOut& o, long at, const RowStat& a, bool has_target, float tgt) {
     const bool none = a.m == -INFINITY && a.s == 0.f;
     const float ls = logf(a.m == INFINITY ? NAN : a.s), lse = none ? -INFINITY : a.m + ls;
-    if (o.logp) o.logp[at] = !has_target ? 0.f : (tgt == -INFINITY && lse == lse) ? -INFINITY : tgt - lse;
+    if (o.logp) o.logp[at] = !has_target ? 0.f : (tgt == -INFINITY && lse == lse) ? -INFINITY : (tgt - a.m) - ls;
     if (o.entropy) o.entropy[at] = none ? 0.f : ls - a.u / a.s;
     if (o.lse) o.lse[at] = lse;
-    return lse;
+    return ls;
 }
 // the index of row r's outputs; -1 where the column counter points outside them
 __device__ __forceinline__ long row_at(const LogpOut& o, long r) {
@@ -105,9 +106,9 @@ __device__ __forceinline__ long row_at(const LogpOut& o, long r) {
     return c >= 0 && c < o.ld ? r * o.ld + c : -1;
 }
 // one alternative of the row at `at`; key 0: none
-__device__ __forceinline__ void store_top(const LogpOut& o, long at, int i, unsigned long long key, float lse) {
+__device__ __forceinline__ void store_top(const LogpOut& o, long at, int i, unsigned long long key, float m, float ls) {
     if (o.top_id) o.top_id[at * o.top + i] = key ? key_id(key) : -1;
-    if (o.top_logp) o.top_logp[at * o.top + i] = key ? key_value(key) - lse : -INFINITY;
+    if (o.top_logp) o.top_logp[at * o.top + i] = key ? (key_value(key) - m) - ls : -INFINITY;
 }
 
 }  // namespace mmz
