@@ -3,6 +3,7 @@
 // because a decoding step outside a CUDA graph is bound by the host: the checks and the packing take 5 us a call when
 // interpreted, as long as the launch of one or two kernels.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -142,11 +143,12 @@ struct Stream {
     }
 };
 
-// scratch of one call: the allocator gives it to nobody else before the call's stream is through with it
+// Scratch of one call, from the memory of the call's own stream: whoever had the block before used it on that stream, and
+// so will whoever has it next. (A block of the current stream's memory may still be read or written there.)
 at::Tensor own_scratch(size_t bytes, const Stream& st, int dev) {
-    at::Tensor t = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (c10::DeviceIndex)dev));
-    if (st.given) t.record_stream(c10::cuda::getStreamFromExternal(st.raw, (c10::DeviceIndex)dev).unwrap());
-    return t;
+    c10::cuda::OptionalCUDAStreamGuard on;
+    if (st.given) on.reset_stream(c10::cuda::getStreamFromExternal(st.raw, (c10::DeviceIndex)dev));
+    return at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (c10::DeviceIndex)dev));
 }
 // a given one
 void* their_scratch(const char* what, PyObject* o, int dev, unsigned long long* bytes) {

@@ -481,6 +481,35 @@ def test_scratch_of_a_call_on_another_stream(cuda):
     assert all(torch.equal(out, want) for out in outs)
 
 
+@pytest.mark.parametrize("raw", [False, True])
+def test_scratch_is_no_memory_of_the_current_stream(cuda, raw):
+    """A freed tensor of the scratch's size that the current stream has yet to read, and calls without scratch on both
+    streams in turn, nobody waiting: each call's scratch is memory of the stream it runs on."""
+    gen = torch.Generator().manual_seed(19)
+    caches = [filled(gen, 1, 2, 60000, 64, "int8") for _ in "ab"]
+    q = torch.randn((1, 1, 2, HD), generator=gen).to(torch.float16).cuda()
+    need = m.attn8_scratch_bytes(1, 1, 2, 2, 60000)
+    assert need > 0
+    want = [torch.empty_like(q) for _ in "ab"]
+    for c, w in zip(caches, want):
+        m.attn8(q, *c, w, block=64)
+    st = torch.cuda.Stream()
+    on = st.cuda_stream if raw else st
+    outs = [torch.zeros_like(q) for _ in range(41)]
+    held = torch.full((need,), 7, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100000000)  # some 50 ms on the current stream
+    read = held.clone()
+    del held  # its block is free for the current stream, behind the copy
+    m.attn8(q, *caches[0], outs[40], block=64, stream=on)
+    for i in range(0, 40, 2):
+        m.attn8(q, *caches[0], outs[i], block=64)
+        m.attn8(q, *caches[1], outs[i + 1], block=64, stream=on)
+    torch.cuda.synchronize()
+    assert (read == 7).all()
+    assert all(torch.equal(out, want[i & 1]) for i, out in enumerate(outs))
+
+
 def test_refusals(cuda):
     c = cache(1, 2, 64, 32, "int8")
     q = torch.zeros((1, 1, 2, HD), dtype=torch.float16, device="cuda")

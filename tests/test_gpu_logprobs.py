@@ -359,3 +359,29 @@ def test_scoring_on_another_stream(cuda):
     m.linear_logprobs(xd, ed, target, **b, scratch=scratch, stream=st)
     torch.cuda.synchronize()
     assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_scratch_is_no_memory_of_the_current_stream(cuda):
+    """As in the attention's test: a freed tensor that the current stream has yet to read, and calls without scratch on
+    both streams in turn."""
+    gen = torch.Generator().manual_seed(16)
+    states = [grid_states(gen, 50, 3000, 256) for _ in "ab"]
+    states = [(x.cuda(), emb.cuda()) for x, emb in states]
+    target = torch.arange(50, dtype=torch.int32, device="cuda")
+    want = [buffers(50, 5) for _ in "ab"]
+    for (x, emb), o in zip(states, want):
+        m.linear_logprobs(x, emb, target, **o)
+    st = torch.cuda.Stream()
+    outs = [buffers(50, 5) for _ in range(41)]
+    held = torch.full((m.linear_logprobs_scratch_bytes(50, 3000, 256),), 7, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100000000)
+    read = held.clone()
+    del held
+    m.linear_logprobs(*states[0], target, **outs[40], stream=st)
+    for i in range(0, 40, 2):
+        m.linear_logprobs(*states[0], target, **outs[i])
+        m.linear_logprobs(*states[1], target, **outs[i + 1], stream=st)
+    torch.cuda.synchronize()
+    assert (read == 7).all()
+    assert all(torch.equal(o[n], want[i & 1][n]) for i, o in enumerate(outs) for n in o)
