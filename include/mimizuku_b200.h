@@ -243,7 +243,7 @@ typedef struct {
  * lse = log sum e^x; logp = x[target] - lse; entropy = -sum p log p (nats); and the alternatives. Sums in fp32. A target
  * outside [0, vocab) has logp 0 (padding), a suppressed one -inf. Fewer than `top` ids with a logit above -inf: the rest
  * have id -1 and -inf. No such id at all: lse -inf and entropy 0. A NaN or +inf logit makes the row's lse, logp and
- * entropy NaN; a NaN is never an alternative. No counterpart in the reference, whose argmax_tok
+ * entropy NaN; a NaN is never an alternative. Up to 2^31 - 1024 rows and 2^31 - 16 ids. No counterpart in the reference, whose argmax_tok
  * (kernels/whisper.cu:451-493) keeps the choice only. */
 int mmz_token_logprobs(const void* logits, long long ldx, int type, int rows, int vocab, const unsigned char* sup,
                        const mmz_logprobs* out, void* stream);

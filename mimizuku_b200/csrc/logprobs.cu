@@ -376,7 +376,8 @@ int launch_token_logprobs(const void* x, long long ldx, int type, int rows, int 
                           const LogpOut& o, cudaStream_t st) {
     if (rows < 0 || V < 1 || ldx < V) return fail("token_logprobs: rows >= 0, vocab >= 1, ldx >= vocab");
     if (type != 0 && type != 1) return fail("token_logprobs: type is 0 (fp16) or 1 (fp32)");
-    if (V > 0x7ffffff0) return fail("token_logprobs: vocab up to 2^31 - 16");
+    // (a CTA's next row is up to 296 further on)
+    if (V > 0x7ffffff0 || rows > 0x7ffffc00) return fail("token_logprobs: vocab up to 2^31 - 16, rows up to 2^31 - 1024");
     if (logp_check("token_logprobs", o)) return -1;
     if (rows == 0) return 0;
     if (!x || ((uintptr_t)x & (type ? 3 : 1))) return fail("token_logprobs: logits null or not aligned to their type");

@@ -134,6 +134,13 @@ def test_token_logprobs_refuses(bad, word):
     assert b"token_logprobs" in msg and word in msg
 
 
+@pytest.mark.parametrize("bad", [dict(rows=0x7fffffff), dict(rows=0x7ffffc01), dict(rows=0x7fffffff, type=1),
+                                 dict(vocab=0x7fffffff, ldx=0x7fffffff), dict(rows=0x7fffffff, x=None)])
+def test_rows_and_ids_near_2_to_31_are_refused(bad):
+    assert logits(**(dict(vocab=1, ldx=1) | bad)) == -1
+    assert b"token_logprobs: vocab up to 2^31 - 16, rows up to 2^31 - 1024" in L.mmz_last_error()
+
+
 @pytest.mark.parametrize("bad,word", [
     (dict(d=96), b"width"), (dict(d=0), b"width"), (dict(rows=-1), b"rows"), (dict(vocab=0), b"vocab"),
     (dict(top=9), b"alternatives"), (dict(ld=0), b"stride"), (dict(target=None), b"target"), (dict(x=None), b"aligned"),
