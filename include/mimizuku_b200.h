@@ -191,12 +191,12 @@ typedef struct {
  * touched and head: scale = max |x| / 127 (int8) or / 448 (e4m3) over its new tokens, but at least the block's earlier
  * scale where it has tokens before pos[b], whose codes are rounded again onto the new scale when it is larger; code =
  * x / scale, to nearest even. The cache's sequences and heads must not overlap (they may in the calls that read it: a
- * sequence stride of 0 lets several share one cache). Rows behind the new tokens are left as they are (and mean
+ * sequence stride of 0 lets several share one cache), nor its keys and values or their scales. Rows behind the new tokens are left as they are (and mean
  * nothing). An infinity counts as +-65504; a NaN becomes 0 (int8) or stays (e4m3). */
 int mmz_kv8_write(const mmz_kv8* cache, const void* k, const void* v, long long x_seq, long long x_tok, long long x_head,
                   const int* pos, int batch, int n, void* stream);
-/* The values of positions pos[b] .. pos[b] + n - 1 (pos NULL: from 0) as fp16, k and v [batch][n][heads][64]; zeros
- * outside [0, min(lens[b], cap)) (lens NULL: cap). */
+/* The values of positions pos[b] .. pos[b] + n - 1 (pos NULL: from 0) as fp16, k and v [batch][n][heads][64] (no row
+ * of the one over one of the other); zeros outside [0, min(lens[b], cap)) (lens NULL: cap). */
 int mmz_kv8_read(const mmz_kv8* cache, void* k, void* v, long long y_seq, long long y_tok, long long y_head,
                  const int* pos, const int* lens, int batch, int n, void* stream);
 
@@ -243,8 +243,8 @@ typedef struct {
  * lse = log sum e^x; logp = x[target] - lse; entropy = -sum p log p (nats); and the alternatives. Sums in fp32. A target
  * outside [0, vocab) has logp 0 (padding), a suppressed one -inf. Fewer than `top` ids with a logit above -inf: the rest
  * have id -1 and -inf. No such id at all: lse -inf and entropy 0. A NaN or +inf logit makes the row's lse, logp and
- * entropy NaN; a NaN is never an alternative. Up to 2^31 - 1024 rows and 2^31 - 16 ids. No counterpart in the reference, whose argmax_tok
- * (kernels/whisper.cu:451-493) keeps the choice only. */
+ * entropy NaN; a NaN is never an alternative. Up to 2^31 - 1024 rows and 2^31 - 16 ids. No counterpart in
+ * the reference, whose argmax_tok (kernels/whisper.cu:451-493) keeps the choice only. */
 int mmz_token_logprobs(const void* logits, long long ldx, int type, int rows, int vocab, const unsigned char* sup,
                        const mmz_logprobs* out, void* stream);
 /* mmz_token_logprobs of the logits x . emb^T, x [rows][ldx] and emb [vocab][d] fp16 (d a multiple of 64, 16-byte aligned

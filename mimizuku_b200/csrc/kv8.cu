@@ -227,6 +227,9 @@ int launch_kv8_write(const void* k, const void* v, long long x_seq, long long x_
     // two sequences or heads in one place would be written by two blocks at once
     if (!apart((long long)cap * HD, {{batch, c_seq}, {heads, c_head}}) || !apart(most, {{batch, s_seq}, {heads, s_head}}))
         return fail("kv8_write: the cache's sequences and heads overlap");
+    if (meet((uint8_t*)v8 - (uint8_t*)k8, (long long)cap * HD, {{batch, c_seq}, {heads, c_head}}) ||
+        meet(vs - ks, most, {{batch, s_seq}, {heads, s_head}}))
+        return fail("kv8_write: the cache's keys and values overlap");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     const Cache c{(uint8_t*)k8, (uint8_t*)v8, ks, vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head};
@@ -248,6 +251,7 @@ int launch_kv8_read(const void* k8, const void* v8, const float* ks, const float
     if (!within(0x7fffffffl, {batch, heads, 2, tiles})) return fail("kv8_read: more than 2^31 blocks in one call");
     const long grid = (long)batch * heads * 2 * tiles;
     if (!apart(HD, {{batch, y_seq}, {n, y_tok}, {heads, y_head}})) return fail("kv8_read: tokens of k and v overlap");
+    if (meet((h16*)v - (h16*)k, HD, {{batch, y_seq}, {n, y_tok}, {heads, y_head}})) return fail("kv8_read: k and v overlap");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     const Cache c{(uint8_t*)k8, (uint8_t*)v8, (float*)ks, (float*)vs, (long)c_seq, (long)c_head, (long)s_seq, (long)s_head};

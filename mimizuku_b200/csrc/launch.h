@@ -62,6 +62,22 @@ inline bool apart(long long room, std::initializer_list<std::pair<int, long long
     }
     return true;
 }
+// Whether an item of a layout that is apart() meets one of the same layout `by` elements further on: some sum of strides,
+// each up to count - 1 times or as often backwards, comes within `room` of `by`. What a nested layout's inner dimensions
+// span is below the stride outside them, so that a stride fits in as often as the quotient says or once more.
+inline bool meet(long long by, long long room, std::initializer_list<std::pair<int, long long>> dims) {
+    std::pair<unsigned long long, int> d[4];
+    int n = 0;
+    for (const auto& x : dims)
+        if (x.first > 1) d[n++] = {x.second < 0 ? 0ull - (unsigned long long)x.second : (unsigned long long)x.second, x.first};
+    std::sort(d, d + n);
+    auto within_room = [&](auto& self, int i, unsigned long long left) -> bool {  // what is left of |by| by the strides from i - 1 down
+        if (i == 0) return left < (unsigned long long)room;
+        const unsigned long long s = d[i - 1].first, k = left / s, rest = left - k * s, most = d[i - 1].second - 1;
+        return (k <= most && self(self, i - 1, rest)) || (k < most && self(self, i - 1, s - rest));
+    };
+    return within_room(within_room, n, by < 0 ? 0ull - (unsigned long long)by : (unsigned long long)by);
+}
 
 // fp16 tensor maps; swizzle: 0 (none), 64 or 128 (bytes)
 int make_tmap_2d(CUtensorMap* map, const void* base, const uint64_t dims[2], const uint64_t strides[1],

@@ -81,6 +81,17 @@ def test_outputs_in_one_place_are_refused():
         assert b"scratch" in L.mmz_last_error()  # the next check
 
 
+def test_keys_and_values_in_one_place_are_refused():
+    far = 1 << 30
+    # one cache for both, the values a position further on, one sequence's values on the next one's keys; the scales alike
+    for bad in (dict(), dict(v8=A + 64), dict(batch=2, cs=(12800, 6400), v8=A + 12800), dict(v8=A - 6336),
+                dict(v8=A + far), dict(v8=A + far, vs=A + 4), dict(v8=A + far, batch=2, cs=(12800, 6400), vs=A - 8)):
+        assert write(**bad) == -1 and b"kv8_write: the cache's keys and values overlap" in L.mmz_last_error()
+    for bad in (dict(), dict(v=A + 16), dict(v=A + 112, n=3), dict(v=A - 256, n=3, xs=(64, 128, 64)),
+                dict(v=A + 256, n=2, heads=2, xs=(64, 128, 64))):
+        assert read(**bad) == -1 and b"kv8_read: k and v overlap" in L.mmz_last_error()
+
+
 def test_nothing_to_do_is_no_error():
     assert write(batch=0, k=None) == 0 and write(n=0, k=None) == 0
     assert read(batch=0) == 0 and read(n=0) == 0
