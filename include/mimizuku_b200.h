@@ -203,7 +203,7 @@ int mmz_kv8_read(const mmz_kv8* cache, void* k, void* v, long long y_seq, long l
 typedef struct {
     const void* q;                   /* [batch][rows][q_heads][64] fp16 */
     long long q_seq, q_row, q_head;  /* its strides in values */
-    void* out;                       /* the same */
+    void* out;                       /* the same; may be q itself (address and strides), else lies apart from it */
     long long o_seq, o_row, o_head;
     const int* lens;                 /* [batch], NULL: cap */
     void* probs;                     /* [batch][slots][rows][cap] fp16, 16-byte aligned; NULL: none */

@@ -1134,6 +1134,19 @@ int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, 
     const size_t need = p.part + p.stats + p.raws;
     if (need && (!scratch || ((uintptr_t)scratch & 15) || scratch_bytes < need))
         return fail("attn8: scratch too small or not 16-byte aligned");
+    // A block of rows reads all of its q before it writes any of its out, and no q but its own: out may be q itself. Rows
+    // of out over other rows of q would be read after they were written
+    const bool alike = (a.batch < 2 || a.q_seq == a.o_seq) && (a.rows < 2 || a.q_row == a.o_row) && (a.q_heads < 2 || a.q_head == a.o_head);
+    auto span = [&](const __half* p, long seq, long row, long head) {  // first and last value
+        std::pair<__int128, __int128> x((intptr_t)p / 2, (intptr_t)p / 2 + HD - 1);
+        for (const std::pair<int, long>& d : {std::pair<int, long>(a.batch, seq), {a.rows, row}, {a.q_heads, head}})
+            (d.second < 0 ? x.first : x.second) += (__int128)d.second * (d.first - 1);
+        return x;
+    };
+    const auto in = span(a.q, a.q_seq, a.q_row, a.q_head), to = span(a.out, a.o_seq, a.o_row, a.o_head);
+    if (in.first <= to.second && to.first <= in.second && !(alike && a.q == a.out) &&
+        !(alike && !meet(a.out - a.q, HD, {{a.batch, a.o_seq}, {a.rows, a.o_row}, {a.q_heads, a.o_head}})))
+        return fail("attn8: out over q, and not q itself");
     DevCtx& dc = dev_ctx();
     if (!dc.ok) return fail(dc.err);
     float* part = (float*)scratch;

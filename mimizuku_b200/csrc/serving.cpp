@@ -403,10 +403,10 @@ PyMethodDef methods[] = {
      "attn8(q, k8, v8, ks, vs, out, block=64, lens=None, causal=False, scale=0.125, probs=None, pslot=None, scratch=None, "
      "stream=None)\n--\n\n"
      "Attention of q [b][rows][q_heads][64] fp16 over the cache's first lens[b] positions (int32 [b]; None: all of\n"
-     "them), into out of the same shape; causal: the rows are the sequence's last ones, row i sees lens - rows + i + 1\n"
-     "positions. A row that sees nothing gives zeros. probs [b][slots][rows][cap] fp16 receives the probabilities of the\n"
-     "heads with pslot[head] >= 0 (int32 [q_heads]). scratch: a uint8 tensor of attn8_scratch_bytes(...) (allocated here\n"
-     "when None and needed)."},
+     "them), into out of the same shape (q itself, or apart from it); causal: the rows are the sequence's last ones, row i\n"
+     "sees lens - rows + i + 1 positions. A row that sees nothing gives zeros. probs [b][slots][rows][cap] fp16 receives\n"
+     "the probabilities of the heads with pslot[head] >= 0 (int32 [q_heads]). scratch: a uint8 tensor of\n"
+     "attn8_scratch_bytes(...) (allocated here when None and needed)."},
     {"token_logprobs", CALL(token_logprobs),
      "token_logprobs(logits, target, logp, entropy=None, lse=None, top_id=None, top_logp=None, sup=None, col=None, "
      "stream=None)\n--\n\n"

@@ -510,6 +510,29 @@ def test_scratch_is_no_memory_of_the_current_stream(cuda, raw):
     assert all(torch.equal(out, want[i & 1]) for i, out in enumerate(outs))
 
 
+@pytest.mark.parametrize("b,rows,h,group,cap,causal", [
+    (2, 1, 3, 1, 1500, False), (1, 1, 2, 4, 60000, False), (3, 7, 2, 1, 400, True), (2, 30, 4, 1, 200, True),
+    (40, 20, 8, 1, 448, True), (40, 37, 8, 1, 150, True), (1, 2, 1, 8, 9000, False)])
+def test_the_output_in_place_of_the_queries(cuda, b, rows, h, group, cap, causal):
+    """out as q itself, and beside it in one tensor: the same bits as apart from it, whatever the layout of the call."""
+    gen = torch.Generator().manual_seed(cap)
+    c = filled(gen, b, h, cap, 64, "int8")
+    lens = torch.tensor([cap - 5 * i for i in range(b)], dtype=torch.int32, device="cuda")
+    hq = h * group
+    q = torch.randn((b, rows, hq, HD), generator=gen).half().cuda()
+    want = torch.empty_like(q)
+    m.attn8(q, *c, want, block=64, lens=lens, causal=causal)
+    both = torch.zeros((b, rows, 2, hq, HD), dtype=torch.float16, device="cuda")
+    both[:, :, 1] = q
+    m.attn8(both[:, :, 1], *c, both[:, :, 0], block=64, lens=lens, causal=causal)
+    assert torch.equal(both[:, :, 0], want) and torch.equal(both[:, :, 1], q)
+    same = q.clone()
+    m.attn8(same, *c, same, block=64, lens=lens, causal=causal)
+    assert torch.equal(same, want)
+    with pytest.raises(m.MmzError, match="out over q"):
+        m.attn8(both.view(b, rows, 2 * hq, HD)[:, :, 1:hq + 1], *c, both[:, :, 0], block=64, lens=lens, causal=causal)
+
+
 def test_refusals(cuda):
     c = cache(1, 2, 64, 32, "int8")
     q = torch.zeros((1, 1, 2, HD), dtype=torch.float16, device="cuda")

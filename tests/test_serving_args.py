@@ -92,6 +92,16 @@ def test_keys_and_values_in_one_place_are_refused():
         assert read(**bad) == -1 and b"kv8_read: k and v overlap" in L.mmz_last_error()
 
 
+def test_an_output_over_other_rows_of_q_is_refused():
+    dims = dict(batch=2, rows=3, hq=2, hkv=2)
+    for bad in (dict(out=A + 16), dict(out=A - 112), dict(dims, qs=(384, 128, 64), os=(384, 128, 64), out=A + 128),
+                dict(dims, qs=(384, 128, 64), os=(384, 64, 192)),  # the same rows in another order
+                dict(dims, qs=(1152, 384, 64), os=(1152, 384, 64), out=A + 768),
+                dict(dims, qs=(0, 128, 64), os=(384, 128, 64), out=A + 640),
+                dict(dims, qs=(384, 128, 64), os=(-384, 128, 64), out=A + 1536)):
+        assert attend(**bad) == -1 and b"attn8: out over q, and not q itself" in L.mmz_last_error()
+
+
 def test_nothing_to_do_is_no_error():
     assert write(batch=0, k=None) == 0 and write(n=0, k=None) == 0
     assert read(batch=0) == 0 and read(n=0) == 0
