@@ -125,6 +125,12 @@ int narrow(const char* what, const char* name, int64_t x) {
 // a stride of a dimension of `count` (that of a dimension of one may be anything)
 long long step(int64_t count, int64_t stride) { return count > 1 ? (long long)stride : 0; }
 
+bool alike(const at::Tensor& a, const at::Tensor& b) {  // strides, of tensors of one shape
+    for (int64_t i = 0; i < a.dim(); i++)
+        if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+    return true;
+}
+
 struct Stream {
     cudaStream_t raw;
     bool given;  // not the current one, or not known to be
@@ -198,7 +204,7 @@ Cache cache_of(const char* what, PyObject* const* four, long long block, int dev
     const at::Tensor& ks = shaped(what, "ks", four[2], at::kFloat, blocks, dev);
     const at::Tensor& vs = shaped(what, "vs", four[3], at::kFloat, blocks, dev);
     const at::IntArrayRef cs = k8.strides(), ss = ks.strides();
-    if (v8.strides() != cs || vs.strides() != ss) refuse(what, "keys and values of the cache have the same strides");
+    if (!alike(k8, v8) || !alike(ks, vs)) refuse(what, "keys and values of the cache have the same strides");
     if (cs[3] != 1 || (cap > 1 && cs[2] != 64) || (blocks[2] > 1 && ss[2] != 1))
         refuse(what, "a head's rows of the cache, and its scales, lie one after another");
     mmz_kv8 c{k8.data_ptr(), v8.data_ptr(), (float*)ks.data_ptr(), (float*)vs.data_ptr(), step(b, cs[0]), step(h, cs[1]),
@@ -219,7 +225,7 @@ Tokens tokens_of(const char* what, PyObject* ko, PyObject* vo, const Cache& c, i
     const at::Tensor& k = shaped(what, "k", ko, at::kHalf, shape, dev);
     const at::Tensor& v = shaped(what, "v", vo, at::kHalf, shape, dev);
     const at::IntArrayRef s = k.strides();
-    if (v.strides() != s || s[3] != 1) refuse(what, "k and v have the same strides, the last dimension dense");
+    if (!alike(k, v) || s[3] != 1) refuse(what, "k and v have the same strides, the last dimension dense");
     return {k.data_ptr(), v.data_ptr(), step(c.batch, s[0]), step(n, s[1]), step(c.heads, s[2]), narrow(what, "n", n)};
 }
 

@@ -510,6 +510,37 @@ def test_scratch_is_no_memory_of_the_current_stream(cuda, raw):
     assert all(torch.equal(out, want[i & 1]) for i, out in enumerate(outs))
 
 
+def test_strides_of_dimensions_of_one_may_differ(cuda):
+    """One token: keys [b][n][h][64], values head by head and transposed; a cache of one sequence, one head and one block
+    whose values and scales come from larger tensors."""
+    gen = torch.Generator().manual_seed(20)
+    b, h, cap, block = 2, 3, 40, 32
+    k = tokens(gen, b, 1, h).cuda()
+    v = tokens(gen, b, 1, h).cuda()
+    vt = torch.empty((b, h, 1, HD), dtype=torch.float16, device="cuda").transpose(1, 2).copy_(v)
+    assert vt.stride() == (h * HD, HD, HD, 1) != k.stride()
+    a, c = cache(b, h, cap, block, "int8"), cache(b, h, cap, block, "int8")
+    pos = torch.tensor([0, 33], dtype=torch.int32, device="cuda")
+    m.kv8_write(k, v, *a, block=block, pos=pos)
+    m.kv8_write(k, vt, *c, block=block, pos=pos)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+    kb, vb = torch.empty_like(k), torch.empty((b, h, 1, HD), dtype=torch.float16, device="cuda").transpose(1, 2)
+    want = torch.empty_like(k), torch.empty_like(k)
+    m.kv8_read(*c, kb, vb, block=block, pos=pos)
+    m.kv8_read(*c, *want, block=block, pos=pos)
+    assert torch.equal(kb, want[0]) and torch.equal(vb, want[1])
+    small, wide = filled(gen, 1, 1, 20, block, "int8"), cache(4, 5, 20, block, "int8")
+    for x, y in zip(small, wide):
+        y[2:3, 3:4] = x
+    q = torch.randn((1, 1, 2, HD), generator=gen).half().cuda()
+    one, two = torch.empty_like(q), torch.empty_like(q)
+    m.attn8(q, *small, one, block=block)
+    m.attn8(q, small[0], wide[1][2:3, 3:4], small[2], wide[3][2:3, 3:4], two, block=block)
+    assert torch.equal(one, two)
+    with pytest.raises(m.MmzError, match="same strides"):
+        m.kv8_write(k, v[:, :, :1].expand(b, 1, h, HD), *a, block=block)
+
+
 @pytest.mark.parametrize("b,rows,h,group,cap,causal", [
     (2, 1, 3, 1, 1500, False), (1, 1, 2, 4, 60000, False), (3, 7, 2, 1, 400, True), (2, 30, 4, 1, 200, True),
     (40, 20, 8, 1, 448, True), (40, 37, 8, 1, 150, True), (1, 2, 1, 8, 9000, False)])
