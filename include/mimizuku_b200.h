@@ -384,8 +384,9 @@ int mmz_engine_enc_gemm(mmz_engine* e);
 int mmz_engine_set_xkv(mmz_engine* e, int type);
 int mmz_engine_xkv(mmz_engine* e);
 /* on != 0: every decoding step also leaves the log probability of the token it chose and the entropy it was chosen
- * from (mmz_token_logprobs of the step's fp16 logits over the ids that `suppress` leaves; the two begin_suppress ids
- * count). Tokens and times do not change. Takes effect at the next step or capture. Native kernel image only. */
+ * from (mmz_token_logprobs of the step's fp16 logits over the ids that the choice is made from: without `suppress`, and
+ * without the two begin_suppress ids at the first generated position). Tokens and times do not change. Takes effect at
+ * the next step or capture. Native kernel image only. */
 int mmz_engine_set_logprobs(mmz_engine* e, int on);
 int mmz_engine_logprobs(mmz_engine* e);
 /* The last mmz_engine_transcribe's (or _transcribe_audio's) log probabilities and entropies, [n][max_t] each on the

@@ -1049,12 +1049,13 @@ int Engine::step(int b, int prompt_len) {
     const int bs1 = gc_.bs[0], bs2 = gc_.bs[1];
     const int fr = k_->logits_argmax(hb_, d, emb_, dm_.vocab, b, sup_, tok_, done_, ctr_, mt, prompt_len, gc_.eos, bs1,
                                      bs2, st_);
-    // the chosen token's log probability and entropy, at the position that the step has just advanced to
+    // the chosen token's log probability and entropy, at the position that the step has just advanced to, over the ids
+    // that the choice was made from
     auto logp = [&]() {
         if (!logprobs_) return 0;
         k_->launches++;
         const LogpOut o{tok_, logp_, ent_, nullptr, nullptr, nullptr, mt, ctr_, 0};
-        return launch_token_logprobs(logits_, dm_.vocab, 0, b, dm_.vocab, sup_, o, st_);
+        return launch_token_logprobs(logits_, dm_.vocab, 0, b, dm_.vocab, sup_, o, st_, Begin{prompt_len, {bs1, bs2}});
     };
     if (fr != -2) return fr ? fr : logp();  // one kernel did all three (model.rs:714-735)
     const int lr = k_->logits(hb_, d, emb_, logits_, dm_.vocab, b, d, st_);

@@ -180,7 +180,7 @@ int launch_attn8(const Attn8& a, int kind, void* scratch, size_t scratch_bytes, 
 // of hidden states against an embedding (linear_logprobs.cu; scratch of linear_logprobs_scratch_bytes)
 int logp_check(const char* what, const LogpOut& o);
 int launch_token_logprobs(const void* x, long long ldx, int type, int rows, int V, const unsigned char* sup,
-                          const LogpOut& o, cudaStream_t st);
+                          const LogpOut& o, cudaStream_t st, const Begin& begin = {});
 size_t linear_logprobs_scratch_bytes(int rows, int V, int d);
 int launch_linear_logprobs(const void* x, long long ldx, const void* emb, int rows, int V, int d,
                            const unsigned char* sup, const LogpOut& o, void* scratch, size_t scratch_bytes,

@@ -78,11 +78,11 @@ __device__ __forceinline__ unsigned long long mask_of(const unsigned char* sup, 
 using namespace lp;
 
 // grid: rows in turn over gridDim / cl clusters of cl = 2^lg CTAs (cl > 1: one row to a cluster); dynamic shared memory
-// sizeof(Smem)
-template <typename T>
+// sizeof(Smem). BEGIN: `begin` is looked at
+template <typename T, bool BEGIN>
 __global__ void __launch_bounds__(NT + 32, 2)
-    token_logprobs_kernel(const T* x, long ldx, int rows, int V, const unsigned char* sup, LogpOut o, int lg,
-                          unsigned* status, unsigned long long limit_ns) {
+    token_logprobs_kernel(const T* x, long ldx, int rows, int V, const unsigned char* sup, LogpOut o, Begin begin,
+                          int lg, unsigned* status, unsigned long long limit_ns) {
     constexpr int N = Piece<T>::N;
     extern __shared__ __align__(128) uint8_t smem[];
     Smem& sm = *reinterpret_cast<Smem*>(smem);
@@ -145,6 +145,8 @@ __global__ void __launch_bounds__(NT + 32, 2)
     }
     if (cl > 1) cluster_wait();
     if (col < 0) return;
+    const bool begins = BEGIN && col == begin.col;
+    const int b0 = begins ? begin.id[0] : -1, b1 = begins ? begin.id[1] : -1;
     unsigned q = 0;
     bool ok = true;
     for (int r = row0; r < rows; r += step) {
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(NT + 32, 2)
         const int head = w.head, tail = head + w.np * N;
         const long at = row_at(o, r);
         const int t = o.target ? o.target[at] : -1;
-        auto logit = [&](int i) { return sup && sup[i] ? -INFINITY : (float)xr[i]; };
+        auto logit = [&](int i) { return (sup && sup[i]) || (BEGIN && (i == b0 || i == b1)) ? -INFINITY : (float)xr[i]; };
         const bool has = t >= 0 && t < V;
         float tgt = 0.f;
         if (rank == 0 && threadIdx.x == 0 && has) tgt = logit(t);
@@ -165,6 +167,12 @@ __global__ void __launch_bounds__(NT + 32, 2)
 #pragma unroll
                     for (int k = 0; k < N; k++)
                         if (m >> (8 * k) & 0xff) f[k] = -INFINITY;
+            }
+            if (BEGIN && begins) {
+                const int i = head + N * p;
+#pragma unroll
+                for (int k = 0; k < N; k++)
+                    if (i + k == b0 || i + k == b1) f[k] = -INFINITY;
             }
         };
         // the ids outside the pieces: at most 7 before, with the first CTA, and 7 after, with the last
@@ -373,9 +381,10 @@ int logp_check(const char* what, const LogpOut& o) {
 }
 
 int launch_token_logprobs(const void* x, long long ldx, int type, int rows, int V, const unsigned char* sup,
-                          const LogpOut& o, cudaStream_t st) {
+                          const LogpOut& o, cudaStream_t st, const Begin& begin) {
     if (rows < 0 || V < 1 || ldx < V) return fail("token_logprobs: rows >= 0, vocab >= 1, ldx >= vocab");
     if (type != 0 && type != 1) return fail("token_logprobs: type is 0 (fp16) or 1 (fp32)");
+    if (type && begin.col >= 0) return fail("token_logprobs: ids left out of one column only of fp16 logits");
     // (a CTA's next row is up to 296 further on)
     if (V > 0x7ffffff0 || rows > 0x7ffffc00) return fail("token_logprobs: vocab up to 2^31 - 16, rows up to 2^31 - 1024");
     if (logp_check("token_logprobs", o)) return -1;
@@ -403,16 +412,19 @@ int launch_token_logprobs(const void* x, long long ldx, int type, int rows, int 
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return check_pdl(type ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<float>, (const float*)x, (long)ldx, rows, V, sup,
-                                               o, lg, dc.status, dc.limit_ns)
-                          : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<h16>, (const h16*)x, (long)ldx, rows, V, sup, o,
-                                               lg, dc.status, dc.limit_ns),
-                     "token_logprobs");
+    auto run = [&](auto* fn, auto* p) {
+        return check_pdl(cudaLaunchKernelEx(&cfg, fn, p, (long)ldx, rows, V, sup, o, begin, lg, dc.status, dc.limit_ns),
+                         "token_logprobs");
+    };
+    if (type) return run(token_logprobs_kernel<float, false>, (const float*)x);
+    return run(begin.col < 0 ? token_logprobs_kernel<h16, false> : token_logprobs_kernel<h16, true>, (const h16*)x);
 }
 
 void init_logprobs_attrs() {
-    cudaFuncSetAttribute(token_logprobs_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem));
-    cudaFuncSetAttribute(token_logprobs_kernel<h16>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem));
+    auto set = [](auto* fn) { cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem)); };
+    set(token_logprobs_kernel<float, false>);
+    set(token_logprobs_kernel<h16, false>);
+    set(token_logprobs_kernel<h16, true>);
 }
 
 }  // namespace mmz

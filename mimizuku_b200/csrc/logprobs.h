@@ -17,4 +17,10 @@ struct LogpOut {
     int top;
 };
 
+// The engine's decoding step: where the outputs' column is `col`, the ids id[0] and id[1] (-1: none) are left out too, as
+// they are of the choice of the first token after a prompt.
+struct Begin {
+    int col = -1, id[2] = {-1, -1};
+};
+
 }  // namespace mmz

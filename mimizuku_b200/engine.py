@@ -203,9 +203,10 @@ class Engine:
 
     @property
     def logprobs(self):
-        """True: every step leaves the log probability of the token it chose and the entropy it was chosen from;
-        transcribe and transcribe_audio return them too, as logprobs and entropy [n][max_t] (0 outside the generated
-        tokens). False is the default. Native image."""
+        """True: every step leaves the log probability of the token it chose and the entropy it was chosen from, over the
+        ids that may be chosen there (without suppress, and without begin_suppress after the prompt); transcribe and
+        transcribe_audio return them too, as logprobs and entropy [n][max_t] (0 outside the generated tokens). False is
+        the default. Native image."""
         return lib.mmz_engine_logprobs(self._h) == 1
 
     @logprobs.setter

@@ -120,6 +120,55 @@ def test_logprobs_of_a_transcription(cuda, b, kind):
     e.close()
 
 
+@pytest.mark.parametrize("b,graph", [(2, True), (12, True), (3, False)])
+def test_the_first_token_is_chosen_without_the_begin_suppressed(cuda, b, graph):
+    """Both ids that clip 0 would begin with are begin-suppressed: its first token's distribution is without them (and
+    every clip's), the second token's with them. Random weights' logits are nearly equal, so that only 160 ids are left to
+    choose from: two of them weigh some 2 / 160."""
+    cfg, new = m.TINY, 3
+    np_ = len(cfg.prompt)
+    sup = [i for i in range(cfg.vocab) if i % 324]
+    mel, frames = clips(b)
+    prompts = np.tile(np.array([cfg.prompt], np.int32), (b, 1))
+
+    def steps(e, n):
+        """The logits that each of the n generated tokens is chosen from, in 64 bits."""
+        e.reset(prompts)
+        out = []
+        for p in range(np_ - 1 + n):
+            e.step(b, np_)
+            e.sync()
+            if p + 1 >= np_:
+                out.append(view(e, "logits", (b, cfg.vocab)).double().cpu())
+                out[-1][:, sup] = -float("inf")
+        return out
+
+    make = lambda **kw: m.Engine(cfg, bmax=b, eg=min(b, 4), seed=3, suppress=sup, **kw)  # noqa: E731
+    e = make()
+    e.transcribe(mel, frames, max_new=1)  # the clips are encoded
+    ids = steps(e, 1)[0][0].topk(2).indices.tolist()
+    e.close()
+    e = make(begin_suppress=tuple(ids))
+    e.logprobs = True
+    r = e.transcribe(mel, frames, max_new=new, graph=graph)
+    x = steps(e, new)
+    left = torch.logsumexp(x[0], 1)
+    x[0][:, ids] = -float("inf")
+    # what the two weigh shows: 30 times the tolerance below
+    assert (left - torch.logsumexp(x[0], 1))[0] > 3e-3
+    for j in range(new):
+        at = np_ + j
+        lp = torch.log_softmax(x[j], 1)
+        want = lp.gather(1, torch.from_numpy(r["tokens"][:, at].astype(np.int64))[:, None])[:, 0]
+        ent = torch.special.entr(lp.exp()).sum(1)
+        live = torch.from_numpy(r["lens"].astype(np.int64)) > at
+        assert j or (live.all() and not np.isin(r["tokens"][:, at], ids).any())
+        # (as in the test above)
+        assert (torch.from_numpy(r["logprobs"][:, at]).double() - want)[live].abs().max() < 1e-4
+        assert (torch.from_numpy(r["entropy"][:, at]).double() - ent)[live].abs().max() < 1e-3
+    e.close()
+
+
 def test_finished_sequences_are_left_out(cuda):
     """A finished sequence's attention output is zero and its recorded probabilities stay as they were."""
     cfg, b = m.TINY, 12
