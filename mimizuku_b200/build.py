@@ -1,6 +1,6 @@
 """Builds libmimizuku_b200.so in-tree: the sm_100a kernels (nvcc, -gencode arch=compute_100a,code=sm_100a), the C++
-engine and CPU stages, linked against cuBLAS with a static CUDA runtime; and, where torch is installed, the compiled
-calls over torch tensors (_serving.so).
+engine and CPU stages, linked against cuBLAS with a static CUDA runtime; and, where a torch with CUDA is installed, the
+compiled calls over torch tensors (_serving.so).
 
     python mimizuku_b200/build.py [--force] [-j N]      (by path: importing the package needs the library)
 
@@ -62,6 +62,43 @@ def _compile(src, force, hdr_time):
     return obj, None
 
 
+def _build_serving(force, hdr, verbose):
+    """Compiles _serving.so for the Python and torch that run this. Without torch or a torch with CUDA there is nothing to
+    call it with; where it does not compile, the library is whole all the same: a warning, and no module of another torch
+    is left behind (importing the calls says what is missing)."""
+    torch = importlib.util.find_spec("torch")
+    at = torch.submodule_search_locations[0] if torch else None
+    if not at or not os.path.exists(os.path.join(at, "lib", "libc10_cuda.so")):
+        if verbose:
+            print("no torch with CUDA: _serving.so is not built")
+        return
+    with open(os.path.join(at, "version.py")) as f:  # torch's C++ interface changes with its version
+        made_for = f"{sys.version}\n{at}\n{f.read()}"
+    stamp = os.path.join(BUILD, "serving.txt")
+    if not force and os.path.exists(SERVING) and os.path.getmtime(SERVING) >= max(os.path.getmtime(SERVING_SRC), hdr):
+        if os.path.exists(stamp) and open(stamp).read() == made_for:
+            return
+    cmd = [os.environ.get("CXX", "g++")] + CXX_FLAGS + [
+        "-shared", SERVING_SRC, "-o", SERVING + ".tmp", "-I", os.path.join(HERE, "..", "include"),
+        "-isystem", sysconfig.get_path("include"), "-isystem", os.path.join(at, "include"),
+        "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"), f"-L{HERE}",
+        "-l:" + os.path.basename(LIB), "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda",
+        "-lc10", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        for path in (SERVING, stamp):
+            if os.path.exists(path):
+                os.remove(path)
+        print(f"warning: _serving.so (the calls over torch tensors) is not built:\n{' '.join(cmd)}\n{r.stdout}{r.stderr}",
+              file=sys.stderr)
+        return
+    shutil.move(SERVING + ".tmp", SERVING)
+    with open(stamp, "w") as f:
+        f.write(made_for)
+    if verbose:
+        print(f"built {SERVING}")
+
+
 def build(force=False, jobs=None, verbose=False):
     """Compiles every source and links the library; raises RuntimeError with the compiler output on failure."""
     if not os.path.exists(NVCC):
@@ -90,21 +127,7 @@ def build(force=False, jobs=None, verbose=False):
         shutil.move(tmp, LIB)
         if verbose:
             print(f"built {LIB}")
-    torch = importlib.util.find_spec("torch")
-    if torch and (force or not os.path.exists(SERVING) or os.path.getmtime(SERVING) < max(os.path.getmtime(SERVING_SRC), hdr)):
-        at = torch.submodule_search_locations[0]
-        cmd = [os.environ.get("CXX", "g++")] + CXX_FLAGS + [
-            "-shared", SERVING_SRC, "-o", SERVING + ".tmp", "-I", os.path.join(HERE, "..", "include"),
-            "-isystem", sysconfig.get_path("include"), "-isystem", os.path.join(at, "include"),
-            "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"), f"-L{HERE}",
-            "-l:" + os.path.basename(LIB), "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda",
-            "-lc10", "-Wl,-rpath,$ORIGIN"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"build failed:\n{' '.join(cmd)}\n{r.stdout}{r.stderr}")
-        shutil.move(SERVING + ".tmp", SERVING)
-        if verbose:
-            print(f"built {SERVING}")
+    _build_serving(force, hdr, verbose)
     return LIB
 
 

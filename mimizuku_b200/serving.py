@@ -8,8 +8,8 @@ from . import lib
 
 try:
     from ._serving import attn8, kv8_read, kv8_write, linear_logprobs, token_logprobs  # noqa: F401
-except ModuleNotFoundError as e:
-    raise ImportError("mimizuku_b200/_serving.so is missing; build it with `python mimizuku_b200/build.py`") from e
+except ImportError as e:  # not there, or built for another torch or Python
+    raise ImportError(f"mimizuku_b200/_serving.so does not load; build it with `python mimizuku_b200/build.py` ({e})") from e
 
 
 def attn8_scratch_bytes(batch, rows, q_heads, kv_heads, cap, slots=0):
