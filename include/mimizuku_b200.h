@@ -188,11 +188,15 @@ typedef struct {
 
 /* Quantises n tokens per sequence, k and v [batch][n][heads][64] fp16 with shared strides x_seq, x_tok, x_head, into
  * the cache at positions pos[b] .. pos[b] + n - 1 (pos NULL: from 0); tokens outside [0, cap) are left out. Per block
- * touched and head: scale = max |x| / 127 (int8) or / 448 (e4m3) over its new tokens, but at least the block's earlier
- * scale where it has tokens before pos[b], whose codes are rounded again onto the new scale when it is larger; code =
- * x / scale, to nearest even. The cache's sequences and heads must not overlap (they may in the calls that read it: a
- * sequence stride of 0 lets several share one cache), nor its keys and values or their scales. Rows behind the new tokens are left as they are (and mean
- * nothing). An infinity counts as +-65504; a NaN becomes 0 (int8) or stays (e4m3). */
+ * touched and head, with a = max |x| over its new tokens, Q = 127 (int8) or 448 (e4m3) and all roundings to nearest even:
+ *   a new scale          a / Q, rounded to fp32. Its codes are x Q / a, rounded to fp32 (once: the quotient by the scale as
+ *                        it was before its own rounding) and then to a code; 0 where a is 0
+ *   the block's earlier  where the block has tokens before pos[b] and its scale is larger than the new one would be: it
+ *   scale s              stays, and the codes are x / s, rounded to fp32 and then to a code
+ * Where the block has tokens before pos[b] and its scale s changes, their codes c become c s Q / a, rounded in the same
+ * way. The cache's sequences and heads must not overlap (they may in the calls that read it: a sequence stride of 0 lets
+ * several share one cache), nor its keys and values or their scales. Rows behind the new tokens are left as they are (and
+ * mean nothing). An infinity counts as +-65504; a NaN becomes 0 (int8) or stays (e4m3). */
 int mmz_kv8_write(const mmz_kv8* cache, const void* k, const void* v, long long x_seq, long long x_tok, long long x_head,
                   const int* pos, int batch, int n, void* stream);
 /* The values of positions pos[b] .. pos[b] + n - 1 (pos NULL: from 0) as fp16, k and v [batch][n][heads][64] (no row

@@ -8,7 +8,7 @@
 //     code = round_to_even(x / s)  (0 where s is 0: an all-zero block)
 // and, where s grew, the earlier tokens' codes become round_to_even(code * s_old / s): a scale only grows while its
 // block fills, so a code is rounded again at most as often as the block's maximum grows. x / s is the quotient by the
-// unrounded scale, x Q / a, rounded to fp32 once: 1 / s is kept as r + rl, and x / s = x r + x rl with one rounding that
+// unrounded scale, x Q / a (or by the block's earlier scale where that stays), rounded to fp32 once: 1 / s is kept as r + rl, and x / s = x r + x rl with one rounding that
 // counts. (fp16 values often lie halfway between two codes exactly; a product by a rounded 1 / s misses so many of
 // them that 1 code in 21 thousand is the wrong one, a whole step off.)
 //
