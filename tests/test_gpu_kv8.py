@@ -115,6 +115,34 @@ def test_write_and_read(cuda, kind, block, case):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
+def test_codes_at_the_border_between_two(cuda, kind):
+    """New scales only: codes against x Q / a in whole numbers (products of fp16 values and Q, which 64 bits hold exactly),
+    half to even. Some of the values lie exactly halfway between two codes; none may be a step off."""
+    gen = torch.Generator().manual_seed(21)
+    b, h, n, block = 4, 20, 1500, 64
+    k8, v8, ks, vs = cache(b, h, n, block, kind)
+    k = tokens(gen, b, n, h).cuda()
+    m.kv8_write(k, k, k8, v8, ks, vs, block=block)
+    x = torch.nn.functional.pad(k.double().transpose(1, 2), (0, 0, 0, -n % block)).view(b, h, -1, block, HD)
+    a = x.abs().amax((3, 4), keepdim=True)
+    top = KINDS[kind][1]
+    # the step between codes there: 1, or an eighth of the power of two below the quotient (of at least 2^-6)
+    if kind == "int8":
+        step = torch.ones_like(x)
+    else:
+        powers = torch.tensor([2.0 ** i for i in range(-6, 9)], dtype=torch.float64, device="cuda")
+        step = powers[(torch.searchsorted(powers, x.abs() * top / a, right=True) - 1).clamp(min=0)] / 8
+    t = x.abs() * top / step  # exact: step is a power of two
+    f = torch.floor(t / a)
+    f = torch.where(f * a > t, f - 1, torch.where((f + 1) * a <= t, f + 1, f))
+    rest = 2 * (t - f * a) - a
+    up = (rest > 0) | ((rest == 0) & (f % 2 == 1))
+    want = ((f + up) * step * x.sign()).view(b, h, -1, HD)[:, :, :n]
+    assert (rest == 0).sum() > (100 if kind == "int8" else 1000)
+    assert torch.equal(k8.double(), want) and torch.equal(v8.double(), want)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
 def test_write_zero_infinite_and_nan(cuda, kind):
     k = torch.zeros((1, 64, 1, HD), dtype=torch.float16)
     k[0, 16, 0, 3] = float("inf")

@@ -273,6 +273,56 @@ def test_hidden_states(cuda, shape, masked):
     assert m.status()[0] == 0
 
 
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("shape", [(1, 3001, 384, 5), (20, 5000, 1280, 8), (33, 2000, 192, 3), (100, 1000, 1280, 5),
+                                   (130, 3000, 1280, 5), (300, 2500, 320, 8)])
+def test_hidden_states_off_any_grid(cuda, shape, masked):
+    """fp16 states and embeddings as they come, whose partial sums are not exact. A product takes 16 terms at a time: each
+    of them, the sum so far and the new sum lose less than 2^-23 of the largest of these numbers (P, over the whole
+    product, in 64 bits). So a logit is off by at most D = 18 d / 16 2^-23 P (its row's largest), lse and the k-th largest
+    logit by D, a log probability by 2 D, and the entropy, whose derivatives -p (log p + H) sum to 2 H at most in
+    magnitude, by 2 H D (a tenth more for its second order, D being below 0.01). The alternatives are those of logits that
+    lie so close to the exact ones: their own logits come within 2 D of the k-th largest, and where no two of the
+    largest top + 1 are that close, they are the same."""
+    rows, V, d, top = shape
+    gen = torch.Generator().manual_seed(rows + d)
+    x = torch.randn((rows, d), generator=gen).half()
+    emb = (torch.randn((V, d), generator=gen) * (1.6 / d ** 0.5)).half()
+    target = torch.randint(0, V, (rows,), generator=gen, dtype=torch.int32)
+    sup = (torch.rand(V, generator=gen) < 0.3).to(torch.uint8) if masked else None
+    xd, ed = x.cuda(), emb.cuda()
+    o = buffers(rows, top)
+    m.linear_logprobs(xd, ed, target.cuda(), **o, sup=None if sup is None else sup.cuda())
+    logits, D = np.empty((rows, V)), np.empty(rows)
+    e64 = ed.double()
+    for r in range(rows):
+        terms = e64 * xd[r].double()
+        sums = terms.view(V, d // 16, 16).sum(2).cumsum(1)
+        logits[r] = sums[:, -1].cpu().numpy()
+        D[r] = 18 * d / 16 * 2.0 ** -23 * max(terms.abs().max().item(), sums.abs().max().item())
+    assert D.max() < 0.01
+    want, tol, etol = reference(logits, target.numpy(), None if sup is None else sup.numpy(), top + 1)
+    near(o["lse"], want["lse"], tol + D)
+    fin = np.where(np.isinf(want["logp"]), 0, np.abs(want["logp"]))
+    near(o["logp"], want["logp"], tol + fin * 2.0 ** -22 + 2 * D)
+    near(o["entropy"], want["entropy"], etol + 2.2 * want["entropy"] * D)
+    tlp = want["top_logp"]
+    near(o["top_logp"], tlp[:, :top], (tol + 2 * D)[:, None] + np.abs(tlp[:, :top]) * 2.0 ** -22)
+    ids = o["top_id"].cpu().numpy()
+    if sup is not None:
+        logits[:, sup.numpy() != 0] = -np.inf
+    clear = 0
+    for r in range(rows):
+        assert len(set(ids[r])) == top
+        kth = tlp[r, :top] + want["lse"][r]
+        assert (np.abs(logits[r, ids[r]] - kth) <= 2 * D[r] + 1e-12).all()
+        if (-np.diff(tlp[r]) > 2 * D[r]).all():
+            assert np.array_equal(ids[r], want["top_id"][r, :top])
+            clear += 1
+    assert clear > 0.8 * rows
+    assert m.status()[0] == 0
+
+
 def test_hidden_states_ties_and_rows_that_repeat(cuda):
     """Equal embedding rows tie (the lower id first), equal hidden states give equal rows, a zero state a uniform one."""
     gen = torch.Generator().manual_seed(12)
