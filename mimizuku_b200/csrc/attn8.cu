@@ -24,8 +24,10 @@
 //   flat     up to 8 rows and too few pairs for a cluster each to fill the GPU (long caches): a fixed number of warps,
 //            each with an equal share of all sequences' and heads' chunks in a row, whatever the lengths; a pair's parts on
 //            several warps join in a second kernel
-// Measured (calls in a CUDA graph): 32 sequences x 20 heads x 1500 positions, int8, 28 us = 4.3 TB/s, with 6 heads recorded
-// 31; 3 sequences of up to 131072 positions and 5 key heads x 4, e4m3, 32 us = 3.9 TB/s; one sequence of 20 heads 5.5 us.
+// Measured (calls in a CUDA graph): 32 sequences x 20 heads x 1500 positions, int8, 29 us = 4.3 TB/s, with 6 heads recorded
+// 32; 3 sequences of up to 131072 positions and 5 key heads x 4, e4m3, 33 us = 3.8 TB/s; one sequence of 20 heads 5.3 us.
+// What bounds the first two is not the bytes (DRAM 48 and 52 %): a chunk is 870 to 920 instructions of a warp, and 2 to 3
+// warps to a scheduler cover half of their latencies (46 to 51 % of the issue slots used).
 #include "attn8.h"
 #include "fp8_cache.cuh"
 #include "launch.h"

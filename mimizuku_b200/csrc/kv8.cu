@@ -8,14 +8,15 @@
 //     code = round_to_even(x / s)  (0 where s is 0: an all-zero block)
 // and, where s grew, the earlier tokens' codes become round_to_even(code * s_old / s): a scale only grows while its
 // block fills, so a code is rounded again at most as often as the block's maximum grows. x / s is the quotient by the
-// unrounded scale, x Q / a (or by the block's earlier scale where that stays), rounded to fp32 once: 1 / s is kept as r + rl, and x / s = x r + x rl with one rounding that
-// counts. (fp16 values often lie halfway between two codes exactly; a product by a rounded 1 / s misses so many of
-// them that 1 code in 21 thousand is the wrong one, a whole step off.)
+// unrounded scale, x Q / a (or by the block's earlier scale where that stays), rounded to fp32 once: 1 / s is kept as
+// r + rl, and x / s = x r + x rl with one rounding that counts. (fp16 values often lie halfway between two codes exactly; a
+// product by a rounded 1 / s misses so many of them that 1 code in 22 thousand is the wrong one, a whole step off.)
 //
 // Bound by memory: 2 bytes read and 1 written per value (and the reverse to read). 32 x 20 heads x 1500 tokens, keys and
-// values: written in 71 us = 5.2 TB/s, read back in 55 us = 6.7 TB/s. A warp takes 32 tokens of one block (8 lanes to a token, 16
-// bytes each), so that its 8 loads are all in flight before the maximum is known and the values are read once; blocks
-// of 64 and 128 tokens are shared by 2 and 4 warps of the CTA, which exchange their maxima in shared memory.
+// values: written in 71 us = 5.2 TB/s, read back in 55 to 59 us (369 MB, of whose 246 MB written 58 are still in L2 at the
+// end: no memory rate). A warp takes 32 tokens of one block (8 lanes to a token, 16 bytes each), so that its 8 loads are all
+// in flight before the maximum is known and the values are read once; blocks of 64 and 128 tokens are shared by 2 and 4
+// warps of the CTA, which exchange their maxima in shared memory.
 #include "fp8_cache.cuh"
 #include "launch.h"
 

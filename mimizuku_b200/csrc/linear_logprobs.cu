@@ -15,7 +15,7 @@
 //   more             linear_pair_kernel: tiles of 256 x 256 on pairs of CTAs (cta_group::2). Bound by the tensor cores
 //                    (at a width of 1280 a tile's products take about five times its epilogue)
 // Measured, 51866 ids: 32 rows of width 1280 33 us (in the form for 128 rows 35; one row of width 384 17 and 22), 128 rows
-// 35 us (in pairs 43), 256 rows 43, 7168 rows 670 us = 1420 TFLOP/s.
+// 35 us (in pairs 43), 256 rows 44, 7168 rows 700 us = 1350 TFLOP/s in a burst, 800 = 1190 back to back under the power cap.
 // All: a TMA producer and an MMA issuer (one warp each) feed two TMEM accumulators in turn, the epilogue works on one
 // while the other fills. Every wait is bounded; a CTA that gives up lets its copies land, waits for its MMAs and frees its
 // TMEM.

@@ -18,6 +18,22 @@
                                                            tensor-core GEMM; mode 1: fc1 with GELU (12000 x 5120 x 1280)
     python -m mimizuku_b200.profile_kernels gemv [m] [n k] the decoder's gemv at m sequences (default 8) over the
                                                            large-v3 logits (51866 x 1280) or n x k
+    python -m mimizuku_b200.profile_kernels kv8            32 sequences x 20 heads x 1500 tokens into the 8-bit cache
+                                                           (int8, block 64) and back
+    python -m mimizuku_b200.profile_kernels attn8 [case]   attention over it: cross (32 x 20 x 1500, 6 heads recorded),
+                                                           prompt (223 causal rows, 8 x 20 heads) or long (0, 65536 and
+                                                           131072 positions, 5 key heads x 4, e4m3)
+    python -m mimizuku_b200.profile_kernels logprobs [r]   token_logprobs of r rows (default 1792) of 51865 fp32 logits,
+                                                           8 alternatives
+    python -m mimizuku_b200.profile_kernels hidden [r]     linear_logprobs of r rows (default 32) of width 1280 against
+                                                           51866 ids, 5 alternatives
+    python -m mimizuku_b200.profile_kernels xkv [b]        prints the times of the large-v3 engine at batch b (default 32)
+                                                           by cache type: the encode of all clips, and a decoding step
+                                                           (graph replay) without and with log probabilities
+
+Run so, the package is imported before torch and its cuBLAS is the CUDA toolkit's. A program that imports torch first, as
+bench.py does, has torch's, and other times where the engine calls it:
+    python -c "import torch; from mimizuku_b200.profile_kernels import main; main(['xkv', '32'])"
 """
 import sys
 
@@ -144,6 +160,80 @@ def main(argv):
         for _ in range(4):
             m.align_cost(align, rc[:n], rc[n:], np_, mt, na, cost, n=n)
             m.dtw_times(cost, rc[:n], rc[n:], mt, times, n=n)
+    elif which == "kv8":
+        b, h, n, block = 32, 20, 1500, 64
+        k, v = (torch.randn(b, n, h, 64, device="cuda").half() for _ in "kv")
+        k8, v8 = (torch.zeros(b, h, n, 64, device="cuda", dtype=torch.int8) for _ in "kv")
+        ks, vs = (torch.zeros(b, h, -(-n // block), device="cuda") for _ in "kv")
+        for _ in range(4):
+            m.kv8_write(k, v, k8, v8, ks, vs, block=block)
+            m.kv8_read(k8, v8, ks, vs, k, v, block=block)
+    elif which == "attn8":
+        case = argv[1] if len(argv) > 1 else "cross"
+        b, rows, h, group, cap, block, kind, slots, lens = {
+            "cross": (32, 1, 20, 1, 1500, 64, "int8", 6, [1500] * 32),
+            "prompt": (8, 223, 20, 1, 448, 16, "int8", 0, [150 + 298 * i // 7 for i in range(8)]),
+            "long": (3, 1, 5, 4, 131072, 128, "e4m3", 0, [0, 65536, 131072])}[case]
+        k8, v8 = ((torch.randn(b, h, cap, 64, device="cuda") * 36).clamp(-127, 127) for _ in "kv")
+        k8, v8 = (x.to(torch.int8 if kind == "int8" else torch.float8_e4m3fn) for x in (k8, v8))
+        ks, vs = (torch.rand(b, h, -(-cap // block), device="cuda") / 36 for _ in "kv")
+        q = torch.randn(b, rows, h * group, 64, device="cuda").half()
+        out, ln = torch.empty_like(q), torch.tensor(lens, device="cuda", dtype=torch.int32)
+        probs = pslot = None
+        if slots:
+            probs = torch.empty(b, slots, rows, cap, device="cuda", dtype=torch.float16)
+            pslot = torch.tensor([i if i < slots else -1 for i in range(h * group)], device="cuda", dtype=torch.int32)
+        for _ in range(4):
+            m.attn8(q, k8, v8, ks, vs, out, block=block, lens=ln, causal=case == "prompt", probs=probs, pslot=pslot)
+    elif which in ("logprobs", "hidden"):
+        r = int(argv[1]) if len(argv) > 1 else 1792 if which == "logprobs" else 32
+        top = 8 if which == "logprobs" else 5
+        target = torch.randint(0, 51865, (r,), device="cuda", dtype=torch.int32)
+        logp, ent, lse = (torch.empty(r, device="cuda") for _ in range(3))
+        more = dict(entropy=ent, lse=lse, top_id=torch.empty(r, top, device="cuda", dtype=torch.int32),
+                    top_logp=torch.empty(r, top, device="cuda"))
+        if which == "logprobs":
+            x = torch.randn(r, 51865, device="cuda") * 2.5
+            for _ in range(4):
+                m.token_logprobs(x, target, logp, **more)
+        else:
+            x, emb = torch.randn(r, 1280, device="cuda").half(), (torch.randn(51866, 1280, device="cuda") * 0.045).half()
+            for _ in range(4):
+                m.linear_logprobs(x, emb, target, logp, **more)
+    elif which == "xkv":
+        import numpy as np
+        b, cfg = int(argv[1]) if len(argv) > 1 else 32, m.LARGE_V3
+        eg = min(8, b)
+        e = m.Engine(cfg, bmax=b, eg=eg, device=0, seed=1234, suppress=[cfg.eos])
+        mel16 = (torch.randn(eg, cfg.n_mels, 3000, device="cuda") * 0.3).half()
+        st = torch.cuda.ExternalStream(e.stream)
+
+        def timed(call, n):
+            a, z = (torch.cuda.Event(enable_timing=True) for _ in "az")
+            e.sync()
+            a.record(st)
+            for _ in range(n):
+                call()
+            z.record(st)
+            e.sync()
+            return a.elapsed_time(z) / n
+
+        best = {}  # the kinds in turn, the smallest of five each
+        for kind in 5 * ("fp16", "int8", "e4m3"):
+            e.xkv = kind
+            got = [timed(lambda: [e.encode(mel16.data_ptr(), min(eg, b - g), g) for g in range(0, b, eg)], 1)]
+            for on in (False, True):
+                e.logprobs = on
+                e.reset(np.tile(np.array(cfg.prompt, np.int32), (b, 1)))
+                e.capture(b, len(cfg.prompt))
+                for _ in range(len(cfg.prompt) + 16):
+                    e.replay()
+                got.append(timed(e.replay, 60))
+            best[kind] = [min(x) for x in zip(got, best.get(kind, got))]
+        for kind, (enc, step, with_lp) in best.items():
+            print(f"{b} sequences, cross k/v {kind}: encode {enc:.2f} ms, step {step:.3f} ms, with log probabilities "
+                  f"{with_lp:.3f} ms")
+        e.close()
     else:
         raise SystemExit(__doc__)
     torch.cuda.synchronize()
