@@ -538,6 +538,46 @@ def test_scratch_is_no_memory_of_the_current_stream(cuda, raw):
     assert all(torch.equal(out, want[i & 1]) for i, out in enumerate(outs))
 
 
+def test_captured_calls_without_scratch(cuda):
+    """Calls that allocate their scratch inside a capture, on the captured stream and on one that joins it, replayed beside
+    eager calls and those of two threads on streams of their own; the default stream by number."""
+    import threading
+    gen = torch.Generator().manual_seed(22)
+    caches = [filled(gen, 1, 2, 60000, 64, "int8") for _ in range(3)]
+    q = torch.randn((1, 1, 2, HD), generator=gen).to(torch.float16).cuda()
+    assert m.attn8_scratch_bytes(1, 1, 2, 2, 60000) > 0
+    want = [torch.empty_like(q) for _ in caches]
+    for c, w in zip(caches, want):
+        m.attn8(q, *c, w, block=64, stream=0)
+    torch.cuda.synchronize()
+    outs = [torch.zeros_like(q) for _ in caches]
+    st, other, g = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        other.wait_stream(st)
+        m.attn8(q, *caches[0], outs[0], block=64)
+        m.attn8(q, *caches[1], outs[1], block=64, stream=other)
+        m.attn8(q, *caches[2], outs[2], block=64)
+        st.wait_stream(other)
+    eager = [[torch.zeros_like(q) for _ in range(20)] for _ in range(3)]
+
+    def calls(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for out in eager[k]:
+                m.attn8(q, *caches[k], out, block=64)
+
+    threads = [threading.Thread(target=calls, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for out in eager[2]:
+        g.replay()
+        m.attn8(q, *caches[2], out, block=64)
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    assert all(torch.equal(out, w) for outs3, w in zip(eager, want) for out in outs3)
+
+
 def test_strides_of_dimensions_of_one_may_differ(cuda):
     """One token: keys [b][n][h][64], values head by head and transposed; a cache of one sequence, one head and one block
     whose values and scales come from larger tensors."""
