@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 #include <utility>
 
@@ -15,7 +16,7 @@
 namespace mmz {
 
 struct DevCtx {
-    bool inited = false;
+    std::atomic<bool> inited{false};  // set when the rest is: a thread that finds it set uses the rest without a lock
     bool ok = false;
     const char* err = "device context not initialised";
     unsigned* status = nullptr;            // device address of the status word (4 x u32)

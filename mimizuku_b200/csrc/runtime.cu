@@ -47,7 +47,6 @@ static DevCtx g_ctx[64];
 // Fills c for device dev (current): device checks, the status word's device address, kernel attributes. Called with
 // g_mu held; c.ok is set only at the end, so a context that was ok stays usable while it is refreshed.
 static void init_ctx(DevCtx& c, int dev) {
-    c.inited = true;
     cudaDeviceProp prop;
     if (cudaGetDeviceProperties(&prop, dev) != cudaSuccess) {
         c.ok = false;
@@ -100,7 +99,10 @@ DevCtx& dev_ctx() {
     DevCtx& c = g_ctx[dev];
     if (c.inited) return c;
     std::lock_guard<std::mutex> lk(g_mu);
-    if (!c.inited) init_ctx(c, dev);
+    if (!c.inited) {
+        init_ctx(c, dev);
+        c.inited = true;
+    }
     return c;
 }
 
@@ -109,6 +111,7 @@ DevCtx& dev_ctx_refresh() {
     if (dev < 0) return dev_ctx();
     std::lock_guard<std::mutex> lk(g_mu);
     init_ctx(g_ctx[dev], dev);
+    g_ctx[dev].inited = true;
     return g_ctx[dev];
 }
 
